@@ -37,7 +37,7 @@ def build_port() -> str:
 
 def build_ref(ck_ref: str = "/root/reference") -> str | None:
     """Compile the reference-backed checker when the reference tree is present."""
-    if not os.path.isdir(ck_ref):
+    if not os.path.isdir(os.path.join(ck_ref, "include", "ck")):
         return REF_SO if os.path.exists(REF_SO) else None
     src = os.path.join(HERE, "ref_shim.cpp")
     if not os.path.exists(REF_SO) or os.path.getmtime(REF_SO) < os.path.getmtime(src):
