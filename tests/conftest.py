@@ -19,6 +19,14 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run on the GPU box)")
 
 
+def pytest_collection_modifyitems(items):
+    # the drop-in binaries are CK's own sources: they exist only where the CK tree was mounted when the examples were built
+    if not os.path.isdir(os.path.join(ROOT, "examples", "_ref_build")):
+        for item in items:
+            if item.originalname.endswith("_dropin"):
+                item.add_marker(pytest.mark.skip(reason="examples/_ref_build was not built: no CK tree was mounted"))
+
+
 @pytest.fixture(scope="session")
 def port():
     from oracle import binding
