@@ -30,6 +30,10 @@ FLAG_TILE_128, FLAG_TILE_256, FLAG_LOCKSTEP, FLAG_WAVES_2X4 = 1, 2, 4, 8
 FLAG_DIRECT_STORE, FLAG_GROUP8, FLAG_DEQUANT_IN_L, FLAG_GENERIC, FLAG_F8_NO_SPECIALS = 32, 64, 512, 1024, 2048
 FLAG_MFMA_32X32 = 4096
 FLAG_PINGPONG = 8192
+FLAG_BF16_RTN = 16384
+# wq_quant_op, wq_activation
+QUANT_ROWS, QUANT_RMSNORM, QUANT_GATED = range(3)
+ACT_SILU, ACT_FASTGELU = range(2)
 # wq_epilogue
 (EPI_PASSTHROUGH, EPI_FASTGELU, EPI_MULTIPLY_ADD_FASTGELU, EPI_MULTIPLY_MULTIPLY,
  EPI_MULTIPLY_MULTIPLY_FASTGELU, EPI_ACT_MUL_CLAMP, EPI_ADD, EPI_ADD_FASTGELU, EPI_MULTIPLY,
@@ -41,7 +45,7 @@ EXPORTS = (
     "wqgemm_launch", "wqgemm_run_timed", "wqgemm_type_string", "wqgemm_kernel_name",
     "wqgemm_pack_int4", "wqgemm_pack_int4_host", "wqgemm_preshuffle_int4", "wqgemm_preshuffle_int4_host", "wqgemm_preshuffle_int8", "wqgemm_preshuffle_int8_host", "wqgemm_reduce_finalize", "wqgemm_splitk_kread",
     "wqgemm_run_timed_rotating", "wqgemm_launch_noalloc", "wqgemm_splitk_multi_workspace_bytes",
-    "wqgemm_splitk_multi_step",
+    "wqgemm_splitk_multi_step", "wqgemm_quant_size", "wqgemm_quantize",
 )
 
 
@@ -64,6 +68,18 @@ class Problem(C.Structure):
     ]
 
 
+class Quant(C.Structure):
+    """``struct wqgemm_quant``."""
+    _fields_ = [
+        ("op", C.c_int32), ("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("activation", C.c_int32),
+        ("M", C.c_int32), ("K", C.c_int32), ("group_k", C.c_int32),
+        ("ldx", C.c_int32), ("ldx2", C.c_int32), ("ld_residual_out", C.c_int32), ("ldq", C.c_int32), ("ld_scale", C.c_int32),
+        ("eps", C.c_float),
+        ("x", C.c_void_p), ("x2", C.c_void_p), ("weight", C.c_void_p), ("q", C.c_void_p), ("scale", C.c_void_p),
+        ("residual_out", C.c_void_p),
+    ]
+
+
 class WqError(RuntimeError):
     def __init__(self, status: int, msg: str):
         super().__init__(f"wqgemm status {status}: {msg}")
@@ -82,6 +98,12 @@ def _load() -> C.CDLL:
     if L.wqgemm_problem_size() != C.sizeof(Problem):
         raise ImportError(f"{LIB_PATH}: built with a wqgemm_problem of {L.wqgemm_problem_size()} bytes, this binding "
                           f"describes {C.sizeof(Problem)}: rebuild the library (make -C composable_kernel_amd/csrc)")
+    L.wqgemm_quant_size.restype = C.c_size_t
+    if L.wqgemm_quant_size() != C.sizeof(Quant):
+        raise ImportError(f"{LIB_PATH}: built with a wqgemm_quant of {L.wqgemm_quant_size()} bytes, this binding describes "
+                          f"{C.sizeof(Quant)}: rebuild the library (make -C composable_kernel_amd/csrc)")
+    L.wqgemm_quantize.restype = C.c_int
+    L.wqgemm_quantize.argtypes = [C.POINTER(Quant), C.c_void_p]
     L.wqgemm_last_error.restype = C.c_char_p
     L.wqgemm_is_supported.restype = C.c_int
     L.wqgemm_is_supported.argtypes = [P]
@@ -242,6 +264,18 @@ def reduce_finalize(p: Problem, partials_ptr: int, k_batch: int, stream: int | N
 
 def splitk_kread(K: int, k_batch: int, granule: int = 64) -> int:
     return int(lib.wqgemm_splitk_kread(K, k_batch, granule))
+
+
+def quantize(d: Quant, stream: int | None = None) -> None:
+    check(lib.wqgemm_quantize(C.byref(d), stream))
+
+
+def f8_problem(a, a_scale, b, b_scale, c, M, N, K, *, a_dtype=F8_E4M3FN, b_dtype=F8_E4M3FN, c_dtype=BF16, **kw) -> Problem:
+    """fp8 x fp8 Problem with block-wise scales (128 x 128 of the weights, 1 x 128 of the activations by default); the
+    remaining keywords are fpAintB_problem's."""
+    kw.setdefault("scale_block", (1, 128, 128))
+    return fpAintB_problem(a, b, None, c, M, N, K, a_dtype=a_dtype, b_dtype=b_dtype, c_dtype=c_dtype, a_block_scale=a_scale,
+                           b_block_scale=b_scale, **kw)
 
 
 def fpAintB_problem(a, b, scale, c, M, N, K, *, a_dtype=F16, b_dtype=I4_PACKED, lda=None, ldb=None,

@@ -1,0 +1,29 @@
+// Parameters and launch functions of the fp8 x fp8 kernels (wq_gemm_f8f8.h, compiled in wq_inst_f8f8.hip).
+#pragma once
+
+#include "wq_device.h"
+
+namespace wq {
+
+struct F8F8Params
+{
+    const uint8_t* a;
+    const uint8_t* b;
+    const float* sa;
+    const float* sb;
+    void* c; // fp32 slabs [z][M][ldc] when partial
+    int M, N, K;
+    int lda, ldb, ldc;
+    int bm, bn, ld_sa, ld_sb;
+    int k_begin, k_end, k_per_z; // slices start on multiples of 128
+    int partial;
+    int tiles_m, tiles_n, group_m;
+    float fnuz; // 2^-(number of FNUZ operands)
+    int bf16_rtn; // bf16 outputs rounded to nearest even under every epilogue (else truncated, as everywhere in this engine)
+    EpilogueArgs epi;
+};
+
+int launch_f8f8(int kernel, const F8F8Params& p, int k_batch, hipStream_t s);
+void launch_reduce_f8f8(const float* slabs, int k_batch, int ld_part, const F8F8Params& p, hipStream_t s);
+
+} // namespace wq

@@ -1,0 +1,69 @@
+// Translation unit of the row quantisers (wq_quantize.h): kernel selection and launch.
+#include <hip/hip_runtime.h>
+
+#include "wqgemm.h"
+#include "wq_quantize.h"
+
+namespace wq {
+
+namespace {
+
+template <int OP, bool BF16>
+void launch_groups(const QuantParams& p, hipStream_t s)
+{
+    const int chunks  = (p.K + 511) / 512;
+    const long waves  = (long)p.M * chunks;
+    const long blocks = (waves + 3) / 4;
+    // (a resident grid walks what is left: 8 workgroups of 4 waves fill a CU)
+    hipLaunchKernelGGL((wq_quantize_groups<OP, BF16>), dim3((unsigned)(blocks < 256 * 8 ? blocks : 256 * 8)), dim3(256), 0, s, p, chunks);
+}
+
+template <int OP, bool BF16, bool GROUPED>
+void launch_row(const QuantParams& p, hipStream_t s)
+{
+    // threads: enough for one piece each up to 1024 when rows are few (latency), else 256 with the row in registers
+    const long pieces = ((long)p.K + 7) / 8;
+    int T             = p.M >= 512 ? 256 : 1024;
+    while(T > 64 && pieces <= T / 2)
+        T >>= 1;
+    if(pieces > 4L * T)
+        T = 1024;
+    const long r = (pieces + T - 1) / T;
+    const dim3 grid((unsigned)p.M), block((unsigned)T);
+    if(r <= 1)
+        hipLaunchKernelGGL((wq_quantize_row<OP, BF16, GROUPED, 1>), grid, block, 0, s, p);
+    else if(r <= 2)
+        hipLaunchKernelGGL((wq_quantize_row<OP, BF16, GROUPED, 2>), grid, block, 0, s, p);
+    else if(r <= 4)
+        hipLaunchKernelGGL((wq_quantize_row<OP, BF16, GROUPED, 4>), grid, block, 0, s, p);
+    else
+        hipLaunchKernelGGL((wq_quantize_row<OP, BF16, GROUPED, 0>), grid, block, 0, s, p);
+}
+
+template <bool BF16>
+void launch_typed(const QuantParams& p, int op, bool grouped, hipStream_t s)
+{
+    if(op == WQ_QUANT_RMSNORM)
+        grouped ? launch_row<1, BF16, true>(p, s) : launch_row<1, BF16, false>(p, s);
+    else if(op == WQ_QUANT_GATED)
+        grouped ? launch_groups<2, BF16>(p, s) : launch_row<2, BF16, false>(p, s);
+    else
+        grouped ? launch_groups<0, BF16>(p, s) : launch_row<0, BF16, false>(p, s);
+}
+
+} // namespace
+
+void launch_quantize(const wqgemm_quant* d, hipStream_t s)
+{
+    QuantParams p;
+    p.x = d->x, p.x2 = d->x2, p.weight = d->weight, p.q = (uint8_t*)d->q, p.scale = d->scale, p.residual_out = d->residual_out;
+    p.M = d->M, p.K = d->K;
+    p.ldx = d->ldx, p.ldx2 = d->ldx2, p.ld_res = d->ld_residual_out, p.ldq = d->ldq, p.ld_scale = d->ld_scale;
+    p.weight_f32 = d->weight_dtype == WQ_F32;
+    p.act        = d->activation;
+    p.eps        = d->eps;
+    const bool grouped = d->group_k > 0;
+    d->dtype == WQ_BF16 ? launch_typed<true>(p, d->op, grouped, s) : launch_typed<false>(p, d->op, grouped, s);
+}
+
+} // namespace wq

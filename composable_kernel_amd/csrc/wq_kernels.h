@@ -967,6 +967,7 @@ struct GenericParams
     const float* sa;
     const float* sb;
     int bm, bn, bk, ld_sa, ld_sb;
+    int bf16_rtn; // fp8 weights: bf16 outputs rounded to nearest even instead of truncated
 };
 
 // 8-bit weights (K, N) row-major (N contiguous, ld = ldb) -> (N, K) with K contiguous, the operand order of the
@@ -1090,6 +1091,10 @@ __global__ __launch_bounds__(256) void wq_gemm_generic(const GenericParams p)
             const uint8_t x = ((const uint8_t*)p.a)[m * p.a_sm + k * p.a_sk];
             va              = p.a_dtype == 8 /*WQ_F8_E4M3FN*/ ? f8_e4m3fn_to_f32(x) : f8_fnuz_to_f32(x);
             vb              = (float)q;
+            if(p.b_dtype == 8 /*WQ_F8_E4M3FN*/)
+                vb = f8_e4m3fn_to_f32((uint8_t)q);
+            else if(p.b_dtype == 2 /*WQ_F8_FNUZ*/)
+                vb = f8_fnuz_to_f32((uint8_t)q);
             if(p.sa)
             {
                 // example/65_gemm_multiply_multiply/gemm_multiply_multiply_xdl_fp8_ab_scale.cpp:262-283: both operands are
@@ -1103,8 +1108,12 @@ __global__ __launch_bounds__(256) void wq_gemm_generic(const GenericParams p)
     if(p.partial)
         ((float*)p.c)[(size_t)blockIdx.z * p.M * p.ldc + (size_t)m * p.ldc + n] = acc;
     else
-        ((uint16_t*)p.c)[(size_t)m * p.ldc + n] =
-            cvt_out16(apply_epilogue(p.epi, acc, m, n), p.epi.c_dtype);
+    {
+        float y = apply_epilogue(p.epi, acc, m, n);
+        if(p.bf16_rtn && p.epi.c_dtype == 1 /*WQ_BF16*/)
+            y = convert_bf16_rtn_bits(y);
+        ((uint16_t*)p.c)[(size_t)m * p.ldc + n] = cvt_out16(y, p.epi.c_dtype);
+    }
 }
 
 // Split-K of the int8 x int8 GEMM: sum the int32 slabs (exact in any order), then the requantisation of the kernels above.

@@ -14,6 +14,7 @@
 #define WQ_MAIN_TU
 #include "wqgemm.h"
 #include "wq_kernels.h"
+#include "wq_f8f8.h"
 
 // The 256-tile kernels are compiled one translation unit per (activation, weight format) pair
 // (wq_inst_256.hip) so that the build runs in parallel.
@@ -25,6 +26,7 @@ int launch_256_f8(const GemmParams& gp, dim3 grid, hipStream_t s, int variant); 
 int launch_256_w32(const GemmParams& gp, dim3 grid, hipStream_t s, int ak);    // wq_inst_256_w32.hip
 int launch_skinny(int ak, int bk, const GemmParams& gp, dim3 grid, hipStream_t s, int nmb, int p); // wq_inst_skinny.hip
 int launch_skinny_ws(int ak, int bk, const GemmParams& gp, dim3 grid, int lds_bytes, hipStream_t s, int p);
+void launch_quantize(const wqgemm_quant* d, hipStream_t s); // wq_inst_quantize.hip
 } // namespace wq
 
 // Scratch of wqgemm_launch_noalloc: lives in the code object, so every GPU the library's kernels are loaded on holds
@@ -66,6 +68,7 @@ enum Route
     ROUTE_F8_MFMA256,
     ROUTE_SKINNY,
     ROUTE_SKINNY_WS,
+    ROUTE_F8F8,
     ROUTE_GENERIC
 };
 
@@ -83,6 +86,7 @@ struct Plan
     bool auto_split = false; // split-K chosen by the planner (small-M kernel, short grids of the 128-tile kernel): needs, and is dropped without, a workspace
     bool f8_fused   = false; // fp8 activations widened inside the small-M whole-image kernel (no image in the workspace)
     bool split_256  = false; // the planner's split-K is what put this problem on the 256-tile kernel
+    int f8f8       = 0;     // ROUTE_F8F8: wq::F8F8Kernel
     bool via_colb = false; // row-major 8-bit B: transpose into the workspace, then the K-contiguous matrix-core kernels
     bool via_f16  = false; // fp8 FNUZ activations: convert to fp16 in the workspace, then the fp16 MFMA kernel
 };
@@ -90,6 +94,7 @@ struct Plan
 bool is16(int dt) { return dt == WQ_F16 || dt == WQ_BF16; }
 bool is_i4(int dt) { return dt == WQ_I4_PACKED || dt == WQ_I4_PRESHUFFLED; } // two nibbles per byte, either unit order
 bool is_preshuf(int dt) { return dt == WQ_I4_PRESHUFFLED || dt == WQ_I8_PRESHUFFLED; }
+bool is_f8(int dt) { return dt == WQ_F8_FNUZ || dt == WQ_F8_E4M3FN; }
 bool has_block_scales(const wqgemm_problem* p) { return p->a_block_scale != nullptr || p->b_block_scale != nullptr; }
 
 // Epilogues of the floating-point family and the D vectors each one reads.
@@ -134,6 +139,63 @@ int check_fp_epilogue(const wqgemm_problem* p)
     return WQ_OK;
 }
 
+// Both block-scale tables present and well formed.
+int check_block_scales(const wqgemm_problem* p)
+{
+    if(!p->a_block_scale || !p->b_block_scale)
+        return fail(WQ_ERR_INVALID, "block-wise scales come in pairs: a_block_scale and b_block_scale");
+    if(p->scale_block_m < 1 || p->scale_block_n < 1 || p->scale_block_k < 1)
+        return fail(WQ_ERR_INVALID, "scale_block_m / _n / _k must be positive");
+    const int kblocks = (p->K - 1) / p->scale_block_k + 1;
+    if(p->ld_a_scale < 0 || p->ld_b_scale < 0 || (p->ld_a_scale != 0 && p->ld_a_scale < kblocks) ||
+       (p->ld_b_scale != 0 && p->ld_b_scale < kblocks))
+        return fail(WQ_ERR_INVALID, "ld_a_scale / ld_b_scale must be 0 or at least ceil(K / scale_block_k) = %d", kblocks);
+    // (K slices and k_batch: every kernel indexes the scale tables with the absolute k, and the fp32 partials already
+    // carry the scales, so the slabs sum like any others)
+    if((uintptr_t)p->a_block_scale % 4 != 0 || (uintptr_t)p->b_block_scale % 4 != 0)
+        return fail(WQ_ERR_INVALID, "block scales are fp32: 4-byte aligned pointers");
+    return WQ_OK;
+}
+
+// fp8 weights: called by make_plan once sizes, layouts and the K slice are validated.
+int make_plan_f8f8(const wqgemm_problem* p, Plan& plan)
+{
+    const bool slice = plan.to_c;
+    if(!is_f8(p->a_dtype) || !has_block_scales(p))
+        return fail(WQ_ERR_UNSUPPORTED, "fp8 weights go with fp8 activations and block-wise scales of both operands");
+    if(p->scale || p->scale_group_k != 0)
+        return fail(WQ_ERR_UNSUPPORTED, "fp8 weights take their scales from b_block_scale: scale must be NULL");
+    if(const int rc = check_block_scales(p); rc != WQ_OK)
+        return rc;
+    if(!slice && !is16(p->c_dtype))
+        return fail(WQ_ERR_UNSUPPORTED, "C must be fp16 or bf16");
+    if(p->flags & ~(WQ_FLAG_GENERIC | WQ_FLAG_F8_NO_SPECIALS | WQ_FLAG_BF16_RTN))
+        return fail(WQ_ERR_UNSUPPORTED, "fp8 weights: flags other than GENERIC, F8_NO_SPECIALS and BF16_RTN have no meaning");
+    if(const int rc = check_fp_epilogue(p); rc != WQ_OK)
+        return rc;
+    if((p->flags & WQ_FLAG_BF16_RTN) && p->epilogue == WQ_EPI_MULTIPLY_ADD)
+        return fail(WQ_ERR_UNSUPPORTED, "the bit-pattern MultiplyAdd epilogue has no rounding to choose");
+    if((uintptr_t)p->c % (slice ? 4 : 2) != 0)
+        return fail(WQ_ERR_INVALID, "C must be aligned to its elements");
+    // The matrix core decodes E4M3FN; of FNUZ it cannot express three encodings.  A K step is one scale block, a wave's 32
+    // columns lie in one column block.
+    const bool fnuz = p->a_dtype == WQ_F8_FNUZ || p->b_dtype == WQ_F8_FNUZ;
+    const bool mfma = !(p->flags & WQ_FLAG_GENERIC) && (!fnuz || (p->flags & WQ_FLAG_F8_NO_SPECIALS)) && p->a_layout == WQ_ROW_MAJOR &&
+                      p->b_layout == WQ_COL_MAJOR && p->scale_block_k == 128 && p->scale_block_n % 32 == 0 &&
+                      plan.k_begin % 128 == 0; // (k_batch slices are whole blocks: k_per_z is a multiple of 128 there)
+    if(!mfma)
+    {
+        if((p->M + 15) / 16 > 65535)
+            return fail(WQ_ERR_UNSUPPORTED, "the general kernel takes at most 1048560 rows (M = %d)", p->M);
+        plan.route = ROUTE_GENERIC;
+        return WQ_OK;
+    }
+    if((long)((p->M + 127) / 128) * ((p->N + 127) / 128) > 0x7FFFFFFFL)
+        return fail(WQ_ERR_UNSUPPORTED, "too many tiles for one launch");
+    plan.route = ROUTE_F8F8;
+    return WQ_OK;
+}
+
 // Validate and choose a kernel.  Returns WQ_OK and fills plan, or an error status with message.
 int make_plan(const wqgemm_problem* p, Plan& plan, bool have_workspace = true)
 {
@@ -143,8 +205,10 @@ int make_plan(const wqgemm_problem* p, Plan& plan, bool have_workspace = true)
         return fail(WQ_ERR_INVALID, "M, N, K must be positive (got %d, %d, %d)", p->M, p->N, p->K);
     if(!p->a || !p->b || !p->c)
         return fail(WQ_ERR_INVALID, "a, b and c must be non-null device pointers");
-    if(p->flags & ~(WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256 | WQ_FLAG_LOCKSTEP | WQ_FLAG_WAVES_2X4 | WQ_FLAG_DIRECT_STORE | WQ_FLAG_GROUP8 | WQ_FLAG_DEQUANT_IN_L | WQ_FLAG_GENERIC | WQ_FLAG_F8_NO_SPECIALS | WQ_FLAG_MFMA_32X32 | WQ_FLAG_PINGPONG))
+    if(p->flags & ~(WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256 | WQ_FLAG_LOCKSTEP | WQ_FLAG_WAVES_2X4 | WQ_FLAG_DIRECT_STORE | WQ_FLAG_GROUP8 | WQ_FLAG_DEQUANT_IN_L | WQ_FLAG_GENERIC | WQ_FLAG_F8_NO_SPECIALS | WQ_FLAG_MFMA_32X32 | WQ_FLAG_PINGPONG | WQ_FLAG_BF16_RTN))
         return fail(WQ_ERR_INVALID, "unknown bits in flags");
+    if((p->flags & WQ_FLAG_BF16_RTN) && !is_f8(p->b_dtype))
+        return fail(WQ_ERR_UNSUPPORTED, "WQ_FLAG_BF16_RTN goes with fp8 weights (elsewhere: WQ_EPI_CONVERT_BF16_RTN)");
     if(p->c_layout != WQ_ROW_MAJOR)
         return fail(WQ_ERR_UNSUPPORTED, "only row-major C is implemented");
     if(p->a_layout != WQ_ROW_MAJOR && p->a_layout != WQ_COL_MAJOR)
@@ -182,6 +246,10 @@ int make_plan(const wqgemm_problem* p, Plan& plan, bool have_workspace = true)
     // (trailing slices may be empty when K is small: they store zero partials)
     if(plan.partial && (p->N % 4 != 0 || p->ldc % 4 != 0))
         return fail(WQ_ERR_UNSUPPORTED, "split-K needs N and ldc to be multiples of 4");
+
+    // ---- fp8 x fp8 with block-wise scales of both operands --------------------------------------
+    if(is_f8(p->b_dtype))
+        return make_plan_f8f8(p, plan);
 
     // ---- int8 x int8 requantised GEMM (example/14, client_example/09) ------------------------
     if(p->a_dtype == WQ_I8 && has_block_scales(p))
@@ -304,16 +372,8 @@ int make_plan(const wqgemm_problem* p, Plan& plan, bool have_workspace = true)
             return fail(WQ_ERR_INVALID, "block-wise scales come in pairs: a_block_scale and b_block_scale");
         if(is16(p->a_dtype))
             return fail(WQ_ERR_UNSUPPORTED, "block-wise scales of both operands go with fp8 activations (16-bit activations: scale_group_k)");
-        if(p->scale_block_m < 1 || p->scale_block_n < 1 || p->scale_block_k < 1)
-            return fail(WQ_ERR_INVALID, "scale_block_m / _n / _k must be positive");
-        const int kblocks = (p->K + p->scale_block_k - 1) / p->scale_block_k;
-        if(p->ld_a_scale < 0 || p->ld_b_scale < 0 || (p->ld_a_scale != 0 && p->ld_a_scale < kblocks) ||
-           (p->ld_b_scale != 0 && p->ld_b_scale < kblocks))
-            return fail(WQ_ERR_INVALID, "ld_a_scale / ld_b_scale must be 0 or at least ceil(K / scale_block_k) = %d", kblocks);
-        // (K slices and k_batch: every kernel indexes the scale tables with the absolute k, and the fp32 partials already
-        // carry the scales, so the slabs sum like any others)
-        if((uintptr_t)p->a_block_scale % 4 != 0 || (uintptr_t)p->b_block_scale % 4 != 0)
-            return fail(WQ_ERR_INVALID, "block scales are fp32: 4-byte aligned pointers");
+        if(const int rc = check_block_scales(p); rc != WQ_OK)
+            return rc;
     }
     if(!slice)
     {
@@ -435,7 +495,7 @@ int make_plan(const wqgemm_problem* p, Plan& plan, bool have_workspace = true)
     }
     // fp8 activations x packed int4 weights on the fp8 matrix core (scales arrive through the epilogue).
     // FNUZ bytes qualify only when the caller excludes the three encodings E4M3FN cannot express.
-    const bool is_f8 = p->a_dtype == WQ_F8_FNUZ || p->a_dtype == WQ_F8_E4M3FN;
+    const bool a_f8 = is_f8(p->a_dtype);
     // The fp8 kernel and the 32x32-MFMA kernel address A and B through buffer resources with 32-bit byte offsets: at most
     // 2 GiB per operand there (the bound the reference puts on every operand,
     // include/ck/tensor_operation/gpu/grid/gridwise_fpAintB_gemm_wmma.hpp:501-507); the other kernels index with 64 bits.
@@ -445,8 +505,8 @@ int make_plan(const wqgemm_problem* p, Plan& plan, bool have_workspace = true)
     const uint64_t b_span = preshuf                         ? (uint64_t)p->N * (uint64_t)p->ldb / b_div
                             : p->b_layout == WQ_COL_MAJOR ? (((uint64_t)p->N - 1) * (uint64_t)p->ldb + (uint64_t)p->K) / b_div
                                                           : (((uint64_t)p->K - 1) * (uint64_t)p->ldb + (uint64_t)p->N) / b_div;
-    const bool fits_32bit = a_span * (is_f8 || p->a_dtype == WQ_I8 ? 1 : 2) <= 0x7FFFFFFFull && b_span <= 0x7FFFFFFFull;
-    if(is_f8 && fits_32bit && !(p->flags & WQ_FLAG_GENERIC) && (p->a_dtype == WQ_F8_E4M3FN || (p->flags & WQ_FLAG_F8_NO_SPECIALS)) &&
+    const bool fits_32bit = a_span * (a_f8 || p->a_dtype == WQ_I8 ? 1 : 2) <= 0x7FFFFFFFull && b_span <= 0x7FFFFFFFull;
+    if(a_f8 && fits_32bit && !(p->flags & WQ_FLAG_GENERIC) && (p->a_dtype == WQ_F8_E4M3FN || (p->flags & WQ_FLAG_F8_NO_SPECIALS)) &&
        is_i4(p->b_dtype) && !(preshuf && (p->flags & WQ_FLAG_PINGPONG)) && !p->scale && p->a_layout == WQ_ROW_MAJOR && p->N % 256 == 0 &&
        (!ab_scaled || (p->scale_block_k == 128 && p->scale_block_n % 32 == 0 && p->K / 128 <= 640 &&
                        !(p->flags & WQ_FLAG_PINGPONG))) &&
@@ -662,6 +722,22 @@ void f16_image_of_a(const wqgemm_problem* p, void* workspace, hipStream_t s, wq:
     gp.a     = a16;
     gp.scale = ones;
     gp.lda   = p->K;
+}
+
+// Columns of a split-K slab of the fp8 x fp8 kernels: whole groups of four, so that odd N splits like any other.
+int f8f8_ld_part(const wqgemm_problem* p) { return (p->N + 3) & ~3; }
+
+wq::F8F8Params f8f8_params(const wqgemm_problem* p)
+{
+    wq::F8F8Params gp{};
+    gp.a = (const uint8_t*)p->a, gp.b = (const uint8_t*)p->b, gp.c = p->c;
+    gp.M = p->M, gp.N = p->N, gp.K = p->K;
+    gp.lda = p->lda, gp.ldb = p->ldb, gp.ldc = p->ldc;
+    gp.fnuz     = (p->a_dtype == WQ_F8_FNUZ ? 0.5f : 1.f) * (p->b_dtype == WQ_F8_FNUZ ? 0.5f : 1.f);
+    gp.bf16_rtn = (p->flags & WQ_FLAG_BF16_RTN) ? 1 : 0;
+    gp.epi      = epilogue_of(p);
+    set_block_scales(gp, p);
+    return gp;
 }
 
 int launch_main(const wqgemm_problem* p, const Plan& plan, void* workspace, hipStream_t s)
@@ -893,6 +969,19 @@ int launch_main(const wqgemm_problem* p, const Plan& plan, void* workspace, hipS
         hipLaunchKernelGGL(wq::wq_gemm_i8_mfma_128, dim3(gp.tiles_m * gp.tiles_n, 1, plan.partial ? plan.k_batch : 1), dim3(256), 0,
                            s, gp);
     }
+    else if(plan.route == ROUTE_F8F8)
+    {
+        wq::F8F8Params gp = f8f8_params(p);
+        gp.k_begin = plan.k_begin, gp.k_end = plan.k_end, gp.k_per_z = plan.k_per_z;
+        gp.partial = plan.partial ? 1 : 0;
+        gp.c       = out;
+        if(plan.partial && !plan.to_c)
+            gp.ldc = f8f8_ld_part(p);
+        gp.tiles_m = (p->M + 127) / 128, gp.tiles_n = (p->N + 127) / 128;
+        gp.group_m = std::min(gp.tiles_m, 8);
+        if(wq::launch_f8f8(plan.f8f8, gp, plan.k_batch, s) != WQ_OK)
+            return fail(WQ_ERR_HIP, "fp8 x fp8 kernel launch failed: %s", hipGetErrorString(hipGetLastError()));
+    }
     else
     {
         wq::GenericParams gp;
@@ -922,6 +1011,7 @@ int launch_main(const wqgemm_problem* p, const Plan& plan, void* workspace, hipS
         gp.partial = plan.partial ? 1 : 0;
         gp.a_dtype = p->a_dtype;
         gp.b_dtype = p->b_dtype;
+        gp.bf16_rtn = (p->flags & WQ_FLAG_BF16_RTN) ? 1 : 0;
         gp.epi     = epilogue_of(p);
         gp.scale_group_k = p->scale_group_k > 0 ? p->scale_group_k : 0;
         gp.ld_scale      = p->ld_scale > 0 ? p->ld_scale : p->N;
@@ -943,6 +1033,12 @@ int launch_reduce(const wqgemm_problem* p, const float* partials, int k_batch, h
     {
         hipLaunchKernelGGL(wq::wq_reduce_requant_i8, dim3(blocks), dim3(256), 0, s, (const int32_t*)partials, k_batch, p->M, p->N,
                            (int8_t*)p->c, p->ldc, p->epilogue, p->requant_scale, (const int32_t*)p->d0);
+        WQ_HIP(hipGetLastError());
+        return WQ_OK;
+    }
+    if(is_f8(p->b_dtype) && p->c_dtype != WQ_F32)
+    {
+        wq::launch_reduce_f8f8(partials, k_batch, f8f8_ld_part(p), f8f8_params(p), s);
         WQ_HIP(hipGetLastError());
         return WQ_OK;
     }
@@ -1039,6 +1135,8 @@ int wqgemm_is_supported(const wqgemm_problem* p)
 
 static size_t plan_workspace_bytes(const wqgemm_problem* p, const Plan& plan)
 {
+    if(plan.partial && !plan.to_c && plan.route == ROUTE_F8F8)
+        return (size_t)plan.k_batch * p->M * f8f8_ld_part(p) * sizeof(float);
     if(plan.partial && !plan.to_c)
         return (size_t)plan.k_batch * p->M * p->N * sizeof(float) + (plan.via_colb ? (size_t)p->K * p->N : 0);
     if(plan.via_f16)
@@ -1292,6 +1390,9 @@ int wqgemm_type_string(const wqgemm_problem* p, char* buf, size_t n)
                  "LdsDmaA, DirectB, ConvertInRegister, KBatch%d%s>",
                  dt_name(p->a_dtype), dt_name(p->b_dtype), dt_name(p->c_dtype), plan.k_batch,
                  !has_block_scales(p) ? "" : p->scale_block_m % 128 == 0 ? ", ABScalePer128K" : ", ABScalePer128K_RowScaleA");
+    else if(plan.route == ROUTE_F8F8)
+        snprintf(buf, n, "DeviceGemmMultiD_ABScale_Mfma_gfx950<%s, 16x16x128_f8f6f4, %s, %s, %s, KBatch%d>", "256, 128, 128, 128",
+                 dt_name(p->a_dtype), dt_name(p->b_dtype), dt_name(p->c_dtype), plan.k_batch);
     else if(plan.route == ROUTE_SKINNY_WS)
         snprintf(buf, n, "DeviceFpAintBGemm_SmallM_gfx950<256, 16, 16, 16x16x32, %s, %s, %s, StreamB, WavesSplitK>",
                  dt_name(p->a_dtype), dt_name(p->b_dtype), dt_name(p->c_dtype));
@@ -1329,11 +1430,52 @@ int wqgemm_kernel_name(const wqgemm_problem* p, char* buf, size_t n)
              : plan.route == ROUTE_I8_SKINNY  ? "wq_gemm_i8_skinny"
              : plan.route == ROUTE_I8_MFMA256 ? "wq_gemm_i8_mfma_256"
              : plan.route == ROUTE_F8_MFMA256 ? (!has_block_scales(p) ? "wq_gemm_f8_mfma_256" : p->scale_block_m % 128 == 0 ? "wq_gemm_f8_mfma_256_abscale" : "wq_gemm_f8_mfma_256_abscale_rows")
+             : plan.route == ROUTE_F8F8 ? "wq_gemm_f8f8_any"
              : plan.route == ROUTE_SKINNY ? "wq_gemm_skinny"
              : plan.route == ROUTE_SKINNY_WS
                  ? ((size_t)p->M * ((plan.k_end - plan.k_begin) * 2 + 16) <= 40 * 1024 ? "wq_gemm_skinny_ws" : "wq_gemm_skinny_wsc")
              : plan.route == ROUTE_MFMA128 ? "wq_gemm_mfma_128"
                                            : "wq_gemm_generic");
+    return WQ_OK;
+}
+
+size_t wqgemm_quant_size(void) { return sizeof(wqgemm_quant); }
+
+int wqgemm_quantize(const wqgemm_quant* q, void* stream)
+{
+    if(!q)
+        return fail(WQ_ERR_INVALID, "quantize: null descriptor");
+    if(q->op != WQ_QUANT_ROWS && q->op != WQ_QUANT_RMSNORM && q->op != WQ_QUANT_GATED)
+        return fail(WQ_ERR_INVALID, "quantize: unknown op %d", q->op);
+    if(q->M <= 0 || q->K <= 0)
+        return fail(WQ_ERR_INVALID, "quantize: M and K must be positive (got %d, %d)", q->M, q->K);
+    if(!is16(q->dtype))
+        return fail(WQ_ERR_UNSUPPORTED, "quantize: inputs must be fp16 or bf16");
+    if(q->group_k != 0 && q->group_k != 128)
+        return fail(WQ_ERR_UNSUPPORTED, "quantize: group_k must be 128, or 0 for one scale per row (got %d)", q->group_k);
+    if(!q->x || !q->q || !q->scale)
+        return fail(WQ_ERR_INVALID, "quantize: x, q and scale must be non-null device pointers");
+    const bool norm = q->op == WQ_QUANT_RMSNORM, gated = q->op == WQ_QUANT_GATED;
+    if(norm && !q->weight)
+        return fail(WQ_ERR_INVALID, "quantize: the norm needs its weight");
+    if(norm && q->weight_dtype != q->dtype && q->weight_dtype != WQ_F32)
+        return fail(WQ_ERR_UNSUPPORTED, "quantize: the norm's weight must have the inputs' type or be fp32");
+    if(norm && !(q->eps >= 0.f))
+        return fail(WQ_ERR_INVALID, "quantize: eps must not be negative");
+    if(gated && !q->x2)
+        return fail(WQ_ERR_INVALID, "quantize: the gated activation needs x2");
+    if(gated && q->activation != WQ_ACT_SILU && q->activation != WQ_ACT_FASTGELU)
+        return fail(WQ_ERR_INVALID, "quantize: unknown activation %d", q->activation);
+    if((!norm && q->residual_out) || (!norm && !gated && q->x2) || (!norm && q->weight))
+        return fail(WQ_ERR_INVALID, "quantize: an operand that op %d does not take is set", q->op);
+    const int groups = q->group_k ? (q->K - 1) / q->group_k + 1 : 1;
+    if(q->ldx < q->K || q->ldq < q->K || q->ld_scale < groups || (q->x2 && q->ldx2 < q->K) || (q->residual_out && q->ld_residual_out < q->K))
+        return fail(WQ_ERR_INVALID, "quantize: a stride is shorter than its row");
+    if((uintptr_t)q->x % 2 || (uintptr_t)q->x2 % 2 || (uintptr_t)q->residual_out % 2 || (uintptr_t)q->scale % 4 ||
+       (uintptr_t)q->weight % (q->weight_dtype == WQ_F32 ? 4 : 2))
+        return fail(WQ_ERR_INVALID, "quantize: pointers must be aligned to their elements");
+    wq::launch_quantize(q, (hipStream_t)stream);
+    WQ_HIP(hipGetLastError());
     return WQ_OK;
 }
 

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import capi
-from .weights import PackedWeights
+from .weights import BlockF8Weights, PackedWeights
 
 _DT = {torch.float16: capi.F16, torch.bfloat16: capi.BF16}
 _EPILOGUES = {"none": capi.EPI_PASSTHROUGH, "fastgelu": capi.EPI_FASTGELU, "add": capi.EPI_ADD,
@@ -103,3 +103,283 @@ class WqLinear(torch.nn.Module):
         y = fpaintb_linear(x.reshape(-1, self.in_features), self.weight, self.scale, self.bits, self.epilogue, self.bias,
                            self.layout)
         return y.reshape(*lead, self.out_features)
+
+
+# ---- fp8 activations and weights with block-wise scales ----------------------------------------------------------------
+#
+# The operators of an 8-bit layer: rmsnorm_fp8, gated_fp8 and quantize_fp8 make e4m3fn activations with fp32 scales (one per
+# 128 consecutive values, or one per row), fp8_linear multiplies them with e4m3fn weights that carry one scale per 128 x 128
+# block.  All are inference-only, run on the current stream of the operands' device, allocate through torch's caching
+# allocator only, and can be captured into a graph.  Called plainly they go straight to the C ABI; while torch.compile
+# traces, and as torch.ops.wqgemm.*, they are the custom operators registered below.
+
+_F8 = torch.float8_e4m3fn
+_ACTIVATIONS = {"silu": capi.ACT_SILU, "fastgelu": capi.ACT_FASTGELU}
+_INT_MAX = 2 ** 31 - 1
+
+
+def _inference_only(name, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} is inference-only: call it under torch.no_grad() or with tensors that need no gradient")
+
+
+def _same_device(name, x, **others):
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} runs on the GPU only")
+    for k, t in others.items():
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name}: {k} is on {t.device}, the first operand on {x.device}")
+
+
+def _rows(t, cols):
+    """(tensor, rows, row stride): t as rows of `cols` contiguous elements, copied only if its layout cannot be read as such."""
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
+    m = t.shape[0]
+    ld = t.stride(0) if m > 1 else cols
+    if (t.stride(1) != 1 and cols > 1) or ld < cols:
+        t, ld = t.contiguous(), cols
+    if m > _INT_MAX or ld > _INT_MAX:
+        raise ValueError("at most 2^31 - 1 rows, columns and elements between rows")
+    return t, m, ld
+
+
+def _launch_on(device, call, *args):
+    """call(*args, stream) with `device` current: the library launches on the current device."""
+    if torch.cuda.current_device() == device.index:
+        call(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            call(*args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _fp8_linear(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype):
+    _same_device("fp8_linear", x, x_scale=x_scale, weight=weight, weight_scale=weight_scale, bias=bias)
+    if x.dtype != _F8 or weight.dtype != _F8:
+        raise TypeError(f"x and weight must be float8_e4m3fn, got {x.dtype} and {weight.dtype}")
+    if x_scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
+        raise TypeError("x_scale and weight_scale must be float32")
+    if out_dtype not in _DT:
+        raise TypeError(f"out_dtype must be float16 or bfloat16, got {out_dtype}")
+    if epilogue not in _EPILOGUES:
+        raise ValueError(f"unknown epilogue {epilogue!r}")
+    if (bias is None) != (epilogue in ("none", "fastgelu")):
+        raise ValueError("bias goes with the add / add_fastgelu epilogues only")
+    if x.dim() < 1 or weight.dim() != 2:
+        raise ValueError("x must be (..., K) and weight (N, K)")
+    N, K = weight.shape
+    lead = x.shape[:-1]
+    if x.shape[-1] != K or K == 0 or N == 0:
+        raise ValueError(f"x {tuple(x.shape)} does not go with a weight of shape {(N, K)}")
+    kb = (K + 127) >> 7
+    if x_scale.shape != (*lead, kb):
+        raise ValueError(f"x_scale must have shape {(*lead, kb)}, got {tuple(x_scale.shape)}")
+    if weight_scale.shape != ((N + 127) >> 7, kb):
+        raise ValueError(f"weight_scale must have shape {((N + 127) >> 7, kb)}, got {tuple(weight_scale.shape)}")
+    if bias is not None:
+        if bias.shape != (N,) or bias.dtype != out_dtype:
+            raise ValueError(f"bias must have shape {(N,)} and the output's dtype {out_dtype}, got {tuple(bias.shape)} {bias.dtype}")
+        bias = bias.contiguous()
+    y = torch.empty((*lead, N), dtype=out_dtype, device=x.device)
+    if y.numel() == 0:
+        return y
+    x, M, lda = _rows(x, K)
+    x_scale, _, ld_a_scale = _rows(x_scale, kb)
+    weight, _, ldb = _rows(weight, K)
+    weight_scale, _, ld_b_scale = _rows(weight_scale, kb)
+    p = capi.f8_problem(x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(), y.data_ptr(), M, N, K,
+                        c_dtype=_DT[out_dtype], lda=lda, ldb=ldb, ldc=N, ld_a_scale=ld_a_scale, ld_b_scale=ld_b_scale,
+                        epilogue=_EPILOGUES[epilogue], d0=bias.data_ptr() if bias is not None else None,
+                        flags=capi.FLAG_BF16_RTN)
+    nbytes = capi.workspace_bytes(p)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    _launch_on(x.device, capi.launch, p, ws.data_ptr() if nbytes else None)
+    return y
+
+
+def _quantized_outputs(x, K, group_k):
+    if group_k not in (0, 128):
+        raise ValueError(f"group_k must be 128, or 0 for one scale per row, got {group_k}")
+    groups = (K + 127) >> 7 if group_k else 1
+    return torch.empty(x.shape, dtype=_F8, device=x.device), torch.empty((*x.shape[:-1], groups), dtype=torch.float32, device=x.device), groups
+
+
+def _quant_rows_input(name, x):
+    if x.dtype not in _DT:
+        raise TypeError(f"{name}: inputs must be float16 or bfloat16, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"{name}: inputs must be (..., K) with K > 0")
+    return x.shape[-1]
+
+
+def _quantize(op, x, x2, weight, activation, eps, group_k, q, scale, groups, residual_out):
+    K = x.shape[-1]
+    d = capi.Quant()
+    x, M, d.ldx = _rows(x, K)
+    d.op, d.dtype, d.M, d.K, d.group_k, d.ldq, d.ld_scale = op, _DT[x.dtype], M, K, group_k, K, groups
+    d.x, d.q, d.scale = x.data_ptr(), q.data_ptr(), scale.data_ptr()
+    if x2 is not None:
+        x2, _, d.ldx2 = _rows(x2, K)
+        d.x2 = x2.data_ptr()
+    if op == capi.QUANT_RMSNORM:
+        d.weight, d.eps = weight.data_ptr(), eps
+        d.weight_dtype = capi.F32 if weight.dtype == torch.float32 else d.dtype
+        if residual_out is not None:
+            d.residual_out, d.ld_residual_out = residual_out.data_ptr(), K
+    elif op == capi.QUANT_GATED:
+        d.activation = activation
+    _launch_on(x.device, capi.quantize, d)
+
+
+def _quantize_fp8(x, group_k):
+    _same_device("quantize_fp8", x)
+    K = _quant_rows_input("quantize_fp8", x)
+    q, scale, groups = _quantized_outputs(x, K, group_k)
+    if q.numel():
+        _quantize(capi.QUANT_ROWS, x, None, None, 0, 0.0, group_k, q, scale, groups, None)
+    return q, scale
+
+
+def _gated_fp8(gate, up, activation, group_k):
+    _same_device("gated_fp8", gate, up=up)
+    K = _quant_rows_input("gated_fp8", gate)
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}")
+    if up.shape != gate.shape or up.dtype != gate.dtype:
+        raise ValueError(f"gate and up must have one shape and dtype, got {tuple(gate.shape)} {gate.dtype} and {tuple(up.shape)} {up.dtype}")
+    q, scale, groups = _quantized_outputs(gate, K, group_k)
+    if q.numel():
+        _quantize(capi.QUANT_GATED, gate, up, None, _ACTIVATIONS[activation], 0.0, group_k, q, scale, groups, None)
+    return q, scale
+
+
+def _rmsnorm_fp8(x, weight, residual, eps, group_k):
+    _same_device("rmsnorm_fp8", x, weight=weight, residual=residual)
+    K = _quant_rows_input("rmsnorm_fp8", x)
+    if weight.shape != (K,) or weight.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"weight must have shape {(K,)} and dtype {x.dtype} or float32, got {tuple(weight.shape)} {weight.dtype}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError(f"residual must have x's shape and dtype, got {tuple(residual.shape)} {residual.dtype}")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    q, scale, groups = _quantized_outputs(x, K, group_k)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+    if q.numel():
+        _quantize(capi.QUANT_RMSNORM, x, residual, weight.contiguous(), 0, eps, group_k, q, scale, groups, out)
+    return q, scale, out
+
+
+@torch.library.custom_op("wqgemm::fp8_linear", mutates_args=())
+def _fp8_linear_op(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                   bias: torch.Tensor | None, epilogue: str, out_dtype: torch.dtype) -> torch.Tensor:
+    return _fp8_linear(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype)
+
+
+@_fp8_linear_op.register_fake
+def _(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype):
+    return x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=out_dtype)
+
+
+@torch.library.custom_op("wqgemm::quantize_fp8", mutates_args=())
+def _quantize_fp8_op(x: torch.Tensor, group_k: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return _quantize_fp8(x, group_k)
+
+
+@torch.library.custom_op("wqgemm::gated_fp8", mutates_args=())
+def _gated_fp8_op(gate: torch.Tensor, up: torch.Tensor, activation: str, group_k: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return _gated_fp8(gate, up, activation, group_k)
+
+
+@torch.library.custom_op("wqgemm::rmsnorm_fp8", mutates_args=())
+def _rmsnorm_fp8_op(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None, eps: float,
+                    group_k: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    q, scale, out = _rmsnorm_fp8(x, weight, residual, eps, group_k)
+    return q, scale, out if out is not None else x.new_empty(0)  # (an operator's results are all tensors)
+
+
+def _fake_quantized(x, group_k):
+    return x.new_empty(x.shape, dtype=_F8), x.new_empty((*x.shape[:-1], (x.shape[-1] + 127) // 128 if group_k else 1), dtype=torch.float32)
+
+
+@_quantize_fp8_op.register_fake
+def _(x, group_k):
+    return _fake_quantized(x, group_k)
+
+
+@_gated_fp8_op.register_fake
+def _(gate, up, activation, group_k):
+    return _fake_quantized(gate, group_k)
+
+
+@_rmsnorm_fp8_op.register_fake
+def _(x, weight, residual, eps, group_k):
+    return (*_fake_quantized(x, group_k), x.new_empty(x.shape if residual is not None else 0))
+
+
+def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+               bias: torch.Tensor | None = None, epilogue: str = "none",
+               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """y[..., n] = epilogue( sum_k x[..., k] x_scale[..., k // 128] weight[n, k] weight_scale[n // 128, k // 128] [, bias[n]] ).
+
+    x (..., K) and weight (N, K) float8_e4m3fn; x_scale (..., ceil(K / 128)) and weight_scale (ceil(N / 128), ceil(K / 128))
+    float32; bias (N,) of out_dtype, with the "add" / "add_fastgelu" epilogues ("none" and "fastgelu" go without).  Sums in
+    fp32, one rounding to nearest even into out_dtype (float16 or bfloat16).  Any N and K; fastest where K is a multiple of 16
+    and the rows are 16-byte aligned."""
+    _inference_only("fp8_linear", x, x_scale, weight, weight_scale, bias)
+    if torch.compiler.is_compiling():
+        return _fp8_linear_op(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype)
+    return _fp8_linear(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype)
+
+
+def quantize_fp8(x: torch.Tensor, group_k: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
+    """x (..., K) float16 / bfloat16 -> (q, scale) with x ~ q * scale: q float8_e4m3fn of x's shape, scale float32 of shape
+    (..., ceil(K / 128)), one per 128 consecutive values, or (..., 1) for group_k = 0.  scale = max|x| / 448 of its group
+    (groups below 1e-12: as if the maximum were that); a NaN makes its whole group NaN."""
+    _inference_only("quantize_fp8", x)
+    return _quantize_fp8_op(x, group_k) if torch.compiler.is_compiling() else _quantize_fp8(x, group_k)
+
+
+def gated_fp8(gate: torch.Tensor, up: torch.Tensor, activation: str = "silu",
+              group_k: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
+    """quantize_fp8 of activation(gate) * up, evaluated in fp32 (activation "silu" or "fastgelu").  gate and up may be the
+    two halves of one projection's output (row-strided views are read in place)."""
+    _inference_only("gated_fp8", gate, up)
+    return (_gated_fp8_op if torch.compiler.is_compiling() else _gated_fp8)(gate, up, activation, group_k)
+
+
+def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                group_k: int = 128) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """h = x + residual; returns (q, scale) = quantize_fp8 of h / sqrt(mean(h^2) + eps) * weight, and h rounded to x's dtype
+    (None without a residual).  The norm sees h unrounded; weight (K,) has x's dtype or float32."""
+    _inference_only("rmsnorm_fp8", x, weight, residual)
+    if torch.compiler.is_compiling():
+        q, scale, out = _rmsnorm_fp8_op(x, weight, residual, eps, group_k)
+        return q, scale, out if residual is not None else None
+    return _rmsnorm_fp8(x, weight, residual, eps, group_k)
+
+
+class Fp8Linear(torch.nn.Module):
+    """Inference-only linear layer over e4m3fn weights with 128 x 128 block scales (see ``weights.quantize_fp8_blocks`` /
+    ``weights.load_fp8_blocks``).
+
+    forward takes float16 / bfloat16 activations, which it quantises by 128 itself and answers in their dtype, or an already
+    quantised pair (q, scale) -- what rmsnorm_fp8, gated_fp8 and quantize_fp8 return first -- answered in ``out_dtype``."""
+
+    def __init__(self, bw: BlockF8Weights, bias: torch.Tensor | None = None, epilogue: str = "none", device="cuda",
+                 out_dtype: torch.dtype = torch.bfloat16):
+        super().__init__()
+        if epilogue not in ("none", "fastgelu"):
+            raise ValueError(f"epilogue must be 'none' or 'fastgelu' (a bias is added in front of it), got {epilogue!r}")
+        self.in_features, self.out_features, self.out_dtype = bw.K, bw.N, out_dtype
+        self.register_buffer("weight", torch.from_numpy(bw.weight.copy()).view(_F8).to(device))
+        self.register_buffer("weight_scale", torch.from_numpy(bw.scale.copy()).to(device))
+        self.register_buffer("bias", None if bias is None else bias.to(device=device, dtype=torch.float32))
+        self.epilogue = epilogue if bias is None else {"none": "add", "fastgelu": "add_fastgelu"}[epilogue]
+
+    def forward(self, x):
+        if isinstance(x, (tuple, list)):
+            q, scale, out_dtype = x[0], x[1], self.out_dtype
+        else:
+            (q, scale), out_dtype = quantize_fp8(x), x.dtype
+        bias = None if self.bias is None else self.bias.to(out_dtype)
+        return fp8_linear(q, scale, self.weight, self.weight_scale, bias, self.epilogue, out_dtype)

@@ -201,3 +201,64 @@ def load_packed(path: str) -> PackedWeights:
     if pw.group_k < 0 or (pw.group_k and pw.K % pw.group_k) or pw.weight.shape != want or pw.scale.shape != want_s:
         raise ValueError(f"{path}: array shapes do not match N = {pw.N}, K = {pw.K}, bits = {pw.bits}, group_k = {pw.group_k}")
     return pw
+
+
+# ---- fp8 weights with one scale per 128 x 128 block ---------------------------------------------------------------
+
+F8_FORMAT = "wqgemm-weights-f8-1"
+F8_BLOCK = 128
+F8_MAX = 448.0  # largest finite e4m3fn value
+
+
+@dataclass
+class BlockF8Weights:
+    """e4m3fn weights of a linear layer with one fp32 scale per 128 outputs x 128 inputs (the last block of either direction
+    may be shorter): w[n, k] = f8(weight[n, k]) * scale[n // 128, k // 128]."""
+    weight: np.ndarray  # uint8 (N, K): e4m3fn bit patterns, K contiguous
+    scale: np.ndarray   # float32 (ceil(N / 128), ceil(K / 128))
+    N: int
+    K: int
+
+    def __post_init__(self):
+        want = (-(-self.N // F8_BLOCK), -(-self.K // F8_BLOCK))
+        if self.weight.shape != (self.N, self.K) or self.weight.dtype != np.uint8:
+            raise ValueError(f"weight must be uint8 of shape {(self.N, self.K)}, got {self.weight.dtype} {self.weight.shape}")
+        if self.scale.shape != want or self.scale.dtype != np.float32:
+            raise ValueError(f"scale must be float32 of shape {want}, got {self.scale.dtype} {self.scale.shape}")
+
+
+def quantize_fp8_blocks(w: np.ndarray) -> BlockF8Weights:
+    """Round-to-nearest e4m3fn quantisation of w (N, K); a block's scale is its largest magnitude / 448 (blocks of zeros:
+    as if that were 1e-12)."""
+    import torch
+
+    t = torch.from_numpy(np.array(w, np.float32))
+    if t.dim() != 2 or t.numel() == 0:
+        raise ValueError("w must be a non-empty (N, K) array")
+    if not bool(torch.isfinite(t).all()):
+        raise ValueError("w holds infinities or NaN")
+    N, K = t.shape
+    nb, kb = -(-N // F8_BLOCK), -(-K // F8_BLOCK)
+    p = torch.nn.functional.pad(t, (0, kb * F8_BLOCK - K, 0, nb * F8_BLOCK - N)).view(nb, F8_BLOCK, kb, F8_BLOCK)
+    s = p.abs().amax(dim=(1, 3)).clamp(min=1e-12) / F8_MAX
+    q = (p / s[:, None, :, None]).clamp(-F8_MAX, F8_MAX).view(nb * F8_BLOCK, kb * F8_BLOCK)[:N, :K]
+    return BlockF8Weights(q.to(torch.float8_e4m3fn).contiguous().view(torch.uint8).numpy(), s.numpy(), N, K)
+
+
+def dequantize_fp8_blocks(bw: BlockF8Weights) -> np.ndarray:
+    """fp32 (N, K) of the stored bytes and scales."""
+    import torch
+
+    v = torch.from_numpy(bw.weight).view(torch.float8_e4m3fn).float().numpy()
+    return v * bw.scale.repeat(F8_BLOCK, 0)[:bw.N].repeat(F8_BLOCK, 1)[:, :bw.K]
+
+
+def save_fp8_blocks(path: str, bw: BlockF8Weights) -> None:
+    np.savez(path, format=np.array(F8_FORMAT), weight=bw.weight, scale=bw.scale, N=np.array(bw.N), K=np.array(bw.K))
+
+
+def load_fp8_blocks(path: str) -> BlockF8Weights:
+    with np.load(path, allow_pickle=False) as z:
+        if "format" not in z or str(z["format"]) != F8_FORMAT:
+            raise ValueError(f"{path} is not a {F8_FORMAT} file")
+        return BlockF8Weights(z["weight"], z["scale"], int(z["N"]), int(z["K"]))

@@ -91,6 +91,7 @@ typedef enum wq_epilogue
 #define WQ_FLAG_F8_NO_SPECIALS 2048 /* WQ_F8_FNUZ activations hold none of the bytes 0x7F, 0xFF (+-240) and 0x80 (NaN): allows the fp8 matrix-core kernel, which reads FNUZ bytes as E4M3FN / 2 and cannot express those three */
 #define WQ_FLAG_MFMA_32X32 4096 /* 256-tile kernel built on v_mfma_f32_32x32x16 (packed int4 weights; tuning A/B) */
 #define WQ_FLAG_PINGPONG 8192 /* fp8 x int4 kernel in its four-section ping-pong form instead of the software-pipelined default (tuning A/B) */
+#define WQ_FLAG_BF16_RTN 16384 /* fp8 weights: bf16 outputs rounded to nearest even under every epilogue instead of truncated */
 #define WQ_FLAG_GROUP8 64       /* walk tiles in groups of 8 tile rows instead of the cost-minimising group (tuning A/B) */
 
 /* One GEMM problem: C[M,N] = epilogue( sum_k A[m,k] * dequant(B[k,n], scale[n]) ).
@@ -156,7 +157,15 @@ typedef struct wqgemm_problem
      * token --, no more than 640 K tiles) sums each 128-k block exactly on the matrix core and applies a_scale * b_scale to the block's sum: the same value up
      * to fp32 rounding (identical when the scales are powers of two).  ld_a_scale >= ceil(K / scale_block_k),
      * ld_b_scale >= ceil(K / scale_block_k); 0 = exactly that.  k_batch and K slices (k_begin / k_end) combine with it: the tables
-     * are indexed with the absolute k, and the fp32 partials carry the scales. */
+     * are indexed with the absolute k, and the fp32 partials carry the scales.
+     *
+     * fp8 WEIGHTS (b_dtype WQ_F8_E4M3FN or WQ_F8_FNUZ, one byte per element; the operand types of that example itself) go with
+     * fp8 activations and these block scales, both tables required.  scale_block_k = 128, scale_block_n a multiple of 32,
+     * K-contiguous operands (A row-major, B column-major) and K slices that start on multiples of 128 run on the matrix core
+     * for any M, N, K, any strides and any scale_block_m, the sum of each 128-k block scaled in fp32; fastest with a, b 16-byte
+     * aligned, lda, ldb and K multiples of 16.  Anything else runs on the general kernel.  On the matrix core FNUZ bytes need
+     * WQ_FLAG_F8_NO_SPECIALS, for both operands; without it problems with an FNUZ operand run on the general kernel.
+     * c_dtype is fp16 or bf16; WQ_FLAG_BF16_RTN chooses the rounding of bf16 outputs, under every epilogue. */
     const void* a_block_scale;
     const void* b_block_scale;
     int32_t scale_block_m, scale_block_n, scale_block_k;
@@ -260,6 +269,59 @@ int wqgemm_pack_int4(const int8_t* q, int32_t ldq, int32_t K, int32_t N, uint8_t
  * WQ_ERR_INVALID if a value lies outside -8..7. */
 int wqgemm_pack_int4_host(const int8_t* q, int32_t ldq, int32_t K, int32_t N, uint8_t* out,
                           int32_t ld_bytes);
+
+/* ---- activations to 8 bits ------------------------------------------------------------------------------------------
+ * Quantisation of M rows of K 16-bit values to WQ_F8_E4M3FN bytes with fp32 scales, alone or fused behind the function that
+ * makes the rows: what the fp8 paths of wqgemm_launch take as A.  No counterpart in the reference, whose fp8 examples generate
+ * their operands on the host.
+ *   y[m, k]     = x[m, k]                                               WQ_QUANT_ROWS
+ *               = act(x[m, k]) * x2[m, k]                               WQ_QUANT_GATED    (x gate, x2 up)
+ *               = h[m, k] / sqrt(mean_k h[m, k]^2 + eps) * weight[k]    WQ_QUANT_RMSNORM, h = x + x2 (x2 = residual, NULL: h = x);
+ *                                                                       residual_out, unless NULL, receives h rounded to dtype
+ *   scale[m, g] = max(max |y| over group g, 1e-12) / 448,   q[m, k] = e4m3fn(y / scale[m, g]), round to nearest even
+ * evaluated in fp32 without further roundings of h or y.  group_k = 128: ceil(K / 128) scales per row -- with
+ * ld_scale = ld_a_scale the a_block_scale table of a problem with scale_block_m = 1, scale_block_k = 128; group_k = 0: one
+ * scale per row (ld_scale = 1 makes it the d1 operand of the MultiplyMultiply epilogues).  A NaN anywhere in a group makes
+ * its scale and all its bytes NaN; an infinity makes the scale infinite and its own bytes NaN.
+ * All strides count elements of their tensor and no alignment beyond an element's own is required (16-byte aligned rows
+ * are fastest).  residual_out may be x or x2 themselves (same pointer and stride); no other outputs may overlap an input.
+ * Rows are independent: a row's result does not depend on M. */
+typedef enum wq_quant_op
+{
+    WQ_QUANT_ROWS    = 0,
+    WQ_QUANT_RMSNORM = 1,
+    WQ_QUANT_GATED   = 2
+} wq_quant_op;
+
+typedef enum wq_activation
+{
+    WQ_ACT_SILU     = 0, /* x / (1 + exp(-x)) */
+    WQ_ACT_FASTGELU = 1  /* the FastGelu of WQ_EPI_FASTGELU */
+} wq_activation;
+
+typedef struct wqgemm_quant
+{
+    int32_t op;           /* wq_quant_op                                                */
+    int32_t dtype;        /* WQ_F16 or WQ_BF16: x, x2, residual_out                     */
+    int32_t weight_dtype; /* RMSNORM: dtype or WQ_F32                                   */
+    int32_t activation;   /* GATED: wq_activation                                       */
+    int32_t M, K;
+    int32_t group_k;      /* 128, or 0 = one scale per row                              */
+    int32_t ldx, ldx2, ld_residual_out, ldq, ld_scale; /* elements; each at least a row's length */
+    float eps;            /* RMSNORM: >= 0                                              */
+    const void* x;
+    const void* x2;
+    const void* weight;
+    void* q;
+    float* scale;
+    void* residual_out;
+} wqgemm_quant;
+
+/* sizeof(wqgemm_quant) as the library was built with (see wqgemm_problem_size). */
+size_t wqgemm_quant_size(void);
+
+/* Enqueue the quantisation on `stream`: one kernel, no workspace, no allocation, no synchronisation, capturable. */
+int wqgemm_quantize(const wqgemm_quant* q, void* stream);
 
 /* Re-order WQ_I4_PACKED weights (column n at packed + n*ld_bytes) into WQ_I4_PRESHUFFLED, the offline layout in
  * which every wave-wide weight fetch of the tile kernels is one contiguous kilobyte (the role of the pre-shuffled B of
