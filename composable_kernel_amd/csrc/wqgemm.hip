@@ -169,8 +169,8 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan)
         return rc;
     if(!slice && !is16(p->c_dtype))
         return fail(WQ_ERR_UNSUPPORTED, "C must be fp16 or bf16");
-    if(p->flags & ~(WQ_FLAG_GENERIC | WQ_FLAG_F8_NO_SPECIALS | WQ_FLAG_BF16_RTN))
-        return fail(WQ_ERR_UNSUPPORTED, "fp8 weights: flags other than GENERIC, F8_NO_SPECIALS and BF16_RTN have no meaning");
+    if(p->flags & ~(WQ_FLAG_GENERIC | WQ_FLAG_F8_NO_SPECIALS | WQ_FLAG_BF16_RTN | WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256))
+        return fail(WQ_ERR_UNSUPPORTED, "fp8 weights: flags other than GENERIC, F8_NO_SPECIALS, BF16_RTN and TILE_* have no meaning");
     if(const int rc = check_fp_epilogue(p); rc != WQ_OK)
         return rc;
     if((p->flags & WQ_FLAG_BF16_RTN) && p->epilogue == WQ_EPI_MULTIPLY_ADD)
@@ -190,8 +190,20 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan)
         plan.route = ROUTE_GENERIC;
         return WQ_OK;
     }
-    if((long)((p->M + 127) / 128) * ((p->N + 127) / 128) > 0x7FFFFFFFL)
+    if(p->M > 0x7FFFFF00 || p->N > 0x7FFFFF00 || (long)((p->M + 127) / 128) * ((p->N + 127) / 128) > 0x7FFFFFFFL)
         return fail(WQ_ERR_UNSUPPORTED, "too many tiles for one launch");
+    // The kernels that load 16 bytes at a time: aligned rows, slices that end on whole pieces, distances inside a tile in 32 bits.
+    const int ld_sa = std::max(p->ld_a_scale, (p->K - 1) / 128 + 1), ld_sb = std::max(p->ld_b_scale, (p->K - 1) / 128 + 1);
+    const bool wide = p->lda % 16 == 0 && p->ldb % 16 == 0 && (uintptr_t)p->a % 16 == 0 && (uintptr_t)p->b % 16 == 0 &&
+                      plan.k_end % 16 == 0 && p->lda <= 1 << 22 && p->ldb <= 1 << 22 && ld_sa <= 1 << 20 && ld_sb <= 1 << 20 && p->K > 384;
+    const long tiles256 = (long)((p->M + 255) / 256) * ((p->N + 255) / 256);
+    plan.f8f8           = !wide ? wq::F8F8_ANY : tiles256 * plan.k_batch >= 128 ? wq::F8F8_256 : wq::F8F8_128;
+    if(wide && (p->flags & WQ_FLAG_TILE_256))
+        plan.f8f8 = wq::F8F8_256;
+    else if(wide && (p->flags & WQ_FLAG_TILE_128))
+        plan.f8f8 = wq::F8F8_128;
+    else if(p->flags & (WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256))
+        return fail(WQ_ERR_UNSUPPORTED, "fp8 weights: WQ_FLAG_TILE_* needs 16-byte aligned rows and K a multiple of 16 above 384");
     plan.route = ROUTE_F8F8;
     return WQ_OK;
 }
@@ -727,6 +739,8 @@ void f16_image_of_a(const wqgemm_problem* p, void* workspace, hipStream_t s, wq:
 // Columns of a split-K slab of the fp8 x fp8 kernels: whole groups of four, so that odd N splits like any other.
 int f8f8_ld_part(const wqgemm_problem* p) { return (p->N + 3) & ~3; }
 
+const char* const kF8F8Names[] = {"wq_gemm_f8f8_any", "wq_gemm_f8f8_128", "wq_gemm_f8f8_256"};
+
 wq::F8F8Params f8f8_params(const wqgemm_problem* p)
 {
     wq::F8F8Params gp{};
@@ -977,8 +991,17 @@ int launch_main(const wqgemm_problem* p, const Plan& plan, void* workspace, hipS
         gp.c       = out;
         if(plan.partial && !plan.to_c)
             gp.ldc = f8f8_ld_part(p);
-        gp.tiles_m = (p->M + 127) / 128, gp.tiles_n = (p->N + 127) / 128;
-        gp.group_m = std::min(gp.tiles_m, 8);
+        const int bm = wq::f8f8_bm(plan.f8f8), bn = wq::f8f8_bn(plan.f8f8);
+        gp.tiles_m = (p->M + bm - 1) / bm, gp.tiles_n = (p->N + bn - 1) / bn;
+        // (group_m as for the other tile kernels: g rows of A plus run / g columns of B per XCD)
+        const int run = (gp.tiles_m * gp.tiles_n + 7) / 8;
+        long best     = 0;
+        for(int g = 1; g <= 16 && g <= gp.tiles_m; g *= 2)
+        {
+            const long cost = (long)g * bm + (long)((run + g - 1) / g) * bn;
+            if(!best || cost <= best)
+                best = cost, gp.group_m = g;
+        }
         if(wq::launch_f8f8(plan.f8f8, gp, plan.k_batch, s) != WQ_OK)
             return fail(WQ_ERR_HIP, "fp8 x fp8 kernel launch failed: %s", hipGetErrorString(hipGetLastError()));
     }
@@ -1391,7 +1414,10 @@ int wqgemm_type_string(const wqgemm_problem* p, char* buf, size_t n)
                  dt_name(p->a_dtype), dt_name(p->b_dtype), dt_name(p->c_dtype), plan.k_batch,
                  !has_block_scales(p) ? "" : p->scale_block_m % 128 == 0 ? ", ABScalePer128K" : ", ABScalePer128K_RowScaleA");
     else if(plan.route == ROUTE_F8F8)
-        snprintf(buf, n, "DeviceGemmMultiD_ABScale_Mfma_gfx950<%s, 16x16x128_f8f6f4, %s, %s, %s, KBatch%d>", "256, 128, 128, 128",
+        snprintf(buf, n, "DeviceGemmMultiD_ABScale_Mfma_gfx950<%s, 16x16x128_f8f6f4, %s, %s, %s, KBatch%d>",
+                 plan.f8f8 == wq::F8F8_256   ? "512, 256, 256, 128, LdsDmaA, DirectB"
+                 : plan.f8f8 == wq::F8F8_128 ? "256, 128, 128, 128, LdsDmaA, DirectB"
+                                             : "256, 128, 128, 128, AnyAlignment",
                  dt_name(p->a_dtype), dt_name(p->b_dtype), dt_name(p->c_dtype), plan.k_batch);
     else if(plan.route == ROUTE_SKINNY_WS)
         snprintf(buf, n, "DeviceFpAintBGemm_SmallM_gfx950<256, 16, 16, 16x16x32, %s, %s, %s, StreamB, WavesSplitK>",
@@ -1430,7 +1456,7 @@ int wqgemm_kernel_name(const wqgemm_problem* p, char* buf, size_t n)
              : plan.route == ROUTE_I8_SKINNY  ? "wq_gemm_i8_skinny"
              : plan.route == ROUTE_I8_MFMA256 ? "wq_gemm_i8_mfma_256"
              : plan.route == ROUTE_F8_MFMA256 ? (!has_block_scales(p) ? "wq_gemm_f8_mfma_256" : p->scale_block_m % 128 == 0 ? "wq_gemm_f8_mfma_256_abscale" : "wq_gemm_f8_mfma_256_abscale_rows")
-             : plan.route == ROUTE_F8F8 ? "wq_gemm_f8f8_any"
+             : plan.route == ROUTE_F8F8 ? kF8F8Names[plan.f8f8]
              : plan.route == ROUTE_SKINNY ? "wq_gemm_skinny"
              : plan.route == ROUTE_SKINNY_WS
                  ? ((size_t)p->M * ((plan.k_end - plan.k_begin) * 2 + 16) <= 40 * 1024 ? "wq_gemm_skinny_ws" : "wq_gemm_skinny_wsc")

@@ -47,7 +47,7 @@ def test_fnuz_with_the_promise_runs_on_the_matrix_core():
     (dict(scale_block=(0, 128, 128)), "positive"), (dict(scale_block=(1, 128, -1)), "positive"),
     (dict(ld_a_scale=7), "ld_a_scale"), (dict(ld_b_scale=7), "ld_a_scale / ld_b_scale"), (dict(sa=FAKE + 2), "aligned"),
     (dict(c=FAKE + 1), "aligned"), (dict(epilogue=capi.EPI_ACT_MUL_CLAMP), "epilogue"), (dict(epilogue=capi.EPI_ADD), "d0"),
-    (dict(scale_group_k=128), "scale must be NULL"), (dict(flags=capi.FLAG_TILE_256), "flags"), (dict(flags=capi.FLAG_PINGPONG), "flags"),
+    (dict(scale_group_k=128), "scale must be NULL"), (dict(flags=capi.FLAG_MFMA_32X32), "flags"), (dict(flags=capi.FLAG_TILE_256, lda=1032), "TILE"), (dict(flags=capi.FLAG_PINGPONG), "flags"),
     (dict(epilogue=capi.EPI_MULTIPLY_ADD, d0=FAKE, d1=FAKE, flags=capi.FLAG_BF16_RTN), "rounding"),
     (dict(M=0), "positive"), (dict(K=0), "positive"), (dict(lda=0), "positive"), (dict(ldc=100), "ldc"), (dict(a=None), "non-null"),
     (dict(k_begin=0, k_end=128), "fp32 partials"), (dict(k_batch=2, N=510), "multiples of 4"),
