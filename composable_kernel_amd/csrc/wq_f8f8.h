@@ -8,8 +8,8 @@ namespace wq {
 enum F8F8Kernel
 {
     F8F8_ANY = 0, // 128 x 128, any alignment and K
-    F8F8_128,     // 128 x 128, four waves side by side, two workgroups per CU
-    F8F8_256      // 256 x 256, eight waves side by side
+    F8F8_128,     // 128 x 128, four waves, two workgroups per CU
+    F8F8_256      // 256 x 256, eight waves
 };
 constexpr int f8f8_bm(int kernel) { return kernel == F8F8_256 ? 256 : 128; }
 constexpr int f8f8_bn(int kernel) { return kernel == F8F8_256 ? 256 : 128; }

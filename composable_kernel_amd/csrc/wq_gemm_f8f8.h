@@ -187,45 +187,50 @@ __global__ __launch_bounds__(256) void wq_gemm_f8f8_any(const F8F8Params p)
 }
 
 // ---------------------------------------------------------------------------------------------
-// BM x BN tile for 16-byte aligned operands: MT row blocks of 16, WAVES waves of 32 columns side by side.
+// BM x BN tile for 16-byte aligned operands: WR x WC waves, each MT row blocks x NT column blocks of 16.
 //
-// Every wave streams its own operands between its own MFMAs (the schedule of wq_gemm_256_f8s.h, without a conversion):
-//   * weights go straight to registers: with the waves side by side each weight is needed by one wave, so a lane loads the 32
-//     bytes of each of its two columns, two K tiles ahead (three register sets);
-//   * activations: a ring of four LDS slots filled by LDS-DMA three K tiles ahead, read back LEAD row blocks ahead;
+// Both operands pass through LDS (LDS-DMA, 8 rows of 128 bytes per piece).  Weights fetched straight into the registers of the
+// MFMA were slower: a wave's load then touches 16 rows, and the vector cache takes one access per lane instead of one per 64
+// bytes, 2048 cycles per 256 x 256 x 128 step, as long as its MFMAs (205 us at 4096 x 11008 x 4096 with 32 columns a wave, 222
+// with 64, two workgroups per CU).
+//   * two LDS slots of a whole K tile; each half of a tile's rows has a barrier of its own, in front of the row block that first
+//     reads the next half, and refills what the half before it has freed: every piece is issued at least a K tile's time before
+//     its barrier.  Weights live in registers for a K tile: read at its end, each column block behind the last MFMA that needs
+//     the old one, so that their slot is free for most of it;
 //   * scales: once per four K tiles the row scales of those four travel as one 16-byte LDS-DMA piece per row (every row's scales
 //     lie in a cache line of their own, so fetching them tile by tile would move a line per row and tile, as much as the
 //     activations themselves), and the column blocks' the same way; needs four K tiles in all, K > 384;
-//   * the block sums of a row block (two MFMAs from a zero accumulator) are folded into the accumulators behind the next row
-//     block's MFMAs, acc = fma(sum, sa * sb, acc): the fused multiply-adds neither wait for a result nor hold back an MFMA;
-//   * one s_barrier per K tile.
-// VMEM bookkeeping (in-order completion, counted waits): tile t issues B(t + 2) x 4 in its first row block and, behind its
-// barrier in front of row block MT - LEAD, one scale piece and A(t + 3) x A_DMA.  The barrier needs A(t + 1), issued at the end
-// of tile t - 2; behind it: B(t + 1) x 4, S, A(t + 2) x A_DMA, B(t + 2) x 4.  The scale piece of tiles 4 j .. 4 j + 3 is issued
-// at the end of tile 4 j - 3, in front of A(4 j): the barrier of tile 4 j - 1, which waits for A(4 j), covers it.  (The tile
-// body has no branch: the compiler would sink the fused multiply-adds behind it and keep every block sum alive.)
+//   * a block sum is one MFMA from a zero accumulator.  The sums of a row block are folded into the accumulators,
+//     acc = fma(sum, sa * sb, acc), each just in front of the next row block's MFMA that overwrites it: NT MFMAs after it was
+//     issued, so that neither waits for the other.
+// VMEM bookkeeping (in-order completion, counted waits).  Behind barrier(t, 0), in front of row block MT / 2 - 1 of tile t:
+// A(t + 2) first half, B(t + 2), one scale piece [group (t, 0)]; behind barrier(t, 1), in front of row block MT - 1: A(t + 2)
+// second half [group (t, 1)].  barrier(t, 0) needs group (t - 2, 1) = A(t) second half, barrier(t, 1) needs group (t - 1, 0) =
+// A(t + 1) first half, B(t + 1), scales: two groups, one of each kind, were issued behind either.  Each wave also waits for its
+// own LDS reads in front of a barrier: what the pieces behind it overwrite has been read by everybody.  (The tile body has no
+// branch: the compiler would sink the fused multiply-adds behind it and keep every block sum alive.)
 // Tiles past the last one are loaded through a resource of zero records: no memory access.  TAIL: the last K tile is partial
 // (K a multiple of 16): its 16-byte pieces past the end are sent out of range, which reads as zeros.
 // ---------------------------------------------------------------------------------------------
-template <int MT_, int WAVES_>
+template <int MT_, int NT_, int WR_, int WC_>
 struct F8F8Tile
 {
-    static constexpr int MT = MT_, WAVES = WAVES_, NT = 2;
-    static constexpr int BM = MT * 16, BN = WAVES * 32, BK = 128, THREADS = WAVES * 64, NBUF = 4;
-    static constexpr int A_TILE  = BM * BK;
-    static constexpr int A_DMA   = A_TILE / 1024 / WAVES;
-    static constexpr int LEAD    = 3, WIN = LEAD + 1;
-    static constexpr int RING    = NBUF * A_TILE;
-    static constexpr int S_ROWS  = BM * 16;        // four K tiles of row scales
-    static constexpr int S_SLOT  = S_ROWS + 1024;  // + one piece for the column blocks (lanes 0 .. WAVES - 1)
-    static constexpr int S_OFF   = RING;
-    static constexpr int C_PITCH = BN * 2 + 16;    // 16-bit image of the C tile
-    static constexpr int F_PITCH = BN * 4 + 16;    // fp32 image of half of it
+    static constexpr int MT = MT_, NT = NT_, WR = WR_, WC = WC_, WAVES = WR * WC;
+    static constexpr int BM = WR * MT * 16, BN = WC * NT * 16, BK = 128, THREADS = WAVES * 64;
+    static constexpr int A_TILE  = BM * BK, B_TILE = BN * BK, SLOT = A_TILE + B_TILE;
+    static constexpr int A_DMA   = BM / 16 / WAVES; // pieces per wave and half of A
+    static constexpr int B_DMA   = BN / 8 / WAVES;
+    static constexpr int S_ROWS  = BM * 16;       // four K tiles of row scales
+    static constexpr int S_SLOT  = S_ROWS + 1024; // + one piece for the column blocks (lanes 0 .. BN / 32 - 1)
+    static constexpr int S_OFF   = 2 * SLOT;
     static constexpr int S_DUMP  = S_OFF + 2 * S_SLOT;
+    static constexpr int C_PITCH = BN * 2 + 16;   // 16-bit image of the C tile
+    static constexpr int F_PITCH = BN * 4 + 16;   // fp32 image of half of it
     static constexpr int LDS_MAIN = S_DUMP + 1024;
     static constexpr int LDS_C    = BM * C_PITCH > BM / 2 * F_PITCH ? BM * C_PITCH : BM / 2 * F_PITCH;
     static constexpr int LDS_BYTES = LDS_MAIN > LDS_C ? LDS_MAIN : LDS_C;
     static_assert(BM / 64 < WAVES, "one scale piece per 64 rows and one for the columns, a wave each");
+    static_assert(MT % 2 == 0 && NT % 2 == 0 && A_DMA * 16 * WAVES == BM && B_DMA * 8 * WAVES == BN, "whole pieces");
     static_assert(LDS_BYTES <= 160 * 1024, "LDS");
 };
 
@@ -234,7 +239,7 @@ __device__ __forceinline__ void f8f8_epilogue(const F8F8Params& p, const f4_t (&
                                               int lane)
 {
     constexpr int MT = T::MT, NT = T::NT;
-    const int fr = lane & 15, fq = lane >> 4, col = wave * 32 + fq * 4;
+    const int fr = lane & 15, fq = lane >> 4, row = wave / T::WC * (MT * 16) + fr, col = wave % T::WC * (NT * 16) + fq * 4;
     const int kind = p.epi.kind;
     if(!p.partial && (kind == 0 || kind == 14))
     {
@@ -248,7 +253,7 @@ __device__ __forceinline__ void f8f8_epilogue(const F8F8Params& p, const f4_t (&
                 f4_t v = acc[nt][mt];
                 if(rtn)
                     v = f4_t{convert_bf16_rtn_bits(v[0]), convert_bf16_rtn_bits(v[1]), convert_bf16_rtn_bits(v[2]), convert_bf16_rtn_bits(v[3])};
-                *(u2_t*)(lds + (mt * 16 + fr) * T::C_PITCH + (col + nt * 16) * 2) = bf ? pack_out4<true>(v) : pack_out4<false>(v);
+                *(u2_t*)(lds + (row + mt * 16) * T::C_PITCH + (col + nt * 16) * 2) = bf ? pack_out4<true>(v) : pack_out4<false>(v);
             }
         __syncthreads();
         constexpr int CH = T::BN / 8; // 16-byte pieces of a row
@@ -274,7 +279,8 @@ __device__ __forceinline__ void f8f8_epilogue(const F8F8Params& p, const f4_t (&
         }
         return;
     }
-    // half the rows at a time as fp32; the epilogue and the edges in one rolled loop
+    // half of every wave's rows at a time as fp32; the epilogue and the edges in one rolled loop
+    const int row_h = wave / T::WC * (MT * 8) + fr;
 #pragma unroll
     for(int ph = 0; ph < 2; ++ph)
     {
@@ -284,13 +290,14 @@ __device__ __forceinline__ void f8f8_epilogue(const F8F8Params& p, const f4_t (&
         for(int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for(int mi = 0; mi < MT / 2; ++mi)
-                *(f4_t*)(lds + (mi * 16 + fr) * T::F_PITCH + (col + nt * 16) * 4) = acc[nt][ph * (MT / 2) + mi];
+                *(f4_t*)(lds + (row_h + mi * 16) * T::F_PITCH + (col + nt * 16) * 4) = acc[nt][ph * (MT / 2) + mi];
         __syncthreads();
 #pragma unroll 2
         for(int i = threadIdx.x; i < T::BM / 2 * (T::BN / 4); i += T::THREADS)
         {
             const int r = i / (T::BN / 4), n = (i % (T::BN / 4)) * 4;
-            f8f8_store4(p, *(const f4_t*)(lds + r * T::F_PITCH + n * 4), m0 + ph * (T::BM / 2) + r, n0 + n);
+            const int m = r / (MT * 8) * (MT * 16) + ph * (MT * 8) + r % (MT * 8);
+            f8f8_store4(p, *(const f4_t*)(lds + r * T::F_PITCH + n * 4), m0 + m, n0 + n);
         }
     }
 }
@@ -304,10 +311,12 @@ __device__ __forceinline__ void for_each_constant(F& f, std::integer_sequence<in
 template <class T, bool TAIL>
 __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
 {
-    constexpr int MT = T::MT, NT = T::NT, LEAD = T::LEAD, WIN = T::WIN, AD = T::A_DMA;
+    constexpr int MT = T::MT, NT = T::NT, MH = MT / 2;
+    using std::integral_constant;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave / T::WC, wc = wave % T::WC;
     const int fr = lane & 15, fq = lane >> 4;
     int tm, tn;
     tile_coords(xcd_remap(blockIdx.x, p.tiles_m * p.tiles_n), p.tiles_m, p.tiles_n, p.group_m, tm, tn);
@@ -340,39 +349,39 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
     const __amdgpu_buffer_rsrc_t null_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)p.a, 0, 0, 0x00020000);
     constexpr uint32_t OUT = 0x80000000u; // an offset past every resource
 
-    uint32_t a_run[AD];
-#pragma unroll
-    for(int i = 0; i < AD; ++i)
-        a_run[i] = (uint32_t)((wave * AD + i) * 8) * (uint32_t)p.lda + k0;
-    const int a_chunk     = ((lane & 7) ^ f8_a_swz(lane >> 3)) << 4;
-    const uint32_t a_lane = (uint32_t)(lane >> 3) * p.lda + a_chunk;
-    const int k_last      = k1 - k0 - (ntiles - 1) * T::BK; // bytes of the last K tile
-    const uint32_t a_tail = a_chunk < k_last ? a_lane : OUT;
-    const uint32_t b_bad0 = fq * 32 < k_last ? 0u : OUT, b_bad1 = fq * 32 + 16 < k_last ? 0u : OUT;
-    uint32_t b_voff[NT];
-#pragma unroll
-    for(int nt = 0; nt < NT; ++nt)
-        b_voff[nt] = (uint32_t)(wave * 32 + nt * 16 + fr) * (uint32_t)p.ldb + fq * 32;
-
-    auto dma_a = [&](const __amdgpu_buffer_rsrc_t& rsrc, int slot, int i, bool last) __attribute__((always_inline)) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + slot * T::A_TILE + (wave * AD + i) * 1024), 16,
-                                                 TAIL && last ? a_tail : a_lane, a_run[i], 0, 0);
-        a_run[i] += T::BK;
+    // A piece: 8 rows of 128 bytes, a row's 16-byte chunks permuted on the source side (f8_a_swz) so that the fragment reads are
+    // free of bank conflicts.  Half h of A: row blocks h * MH .. of every wave row.
+    const int chunk       = ((lane & 7) ^ f8_a_swz(lane >> 3)) << 4;
+    const uint32_t a_lane = (uint32_t)(lane >> 3) * (uint32_t)p.lda + chunk;
+    const uint32_t b_lane = (uint32_t)(lane >> 3) * (uint32_t)p.ldb + chunk;
+    const bool past       = chunk >= k1 - k0 - (ntiles - 1) * T::BK; // this lane's chunk of the last K tile lies past its end
+    auto a_row = [&](int h, int i) __attribute__((always_inline)) {
+        const int q = wave * T::A_DMA + i;
+        return q / MT * (MT * 16) + h * (MT * 8) + q % MT * 8;
     };
-    auto load_b = [&](const __amdgpu_buffer_rsrc_t& rsrc, i8v_t(&dst)[NT], int tile) __attribute__((always_inline)) {
-        const uint32_t soff = __builtin_amdgcn_readfirstlane(k0 + tile * T::BK);
-        const bool last     = TAIL && tile == ntiles - 1;
+    uint32_t a_run[2][T::A_DMA], b_run[T::B_DMA];
 #pragma unroll
-        for(int nt = 0; nt < NT; ++nt)
-        {
-            const u4_t lo = __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, last ? b_voff[nt] | b_bad0 : b_voff[nt], soff, 0));
-            const u4_t hi = __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (last ? b_voff[nt] | b_bad1 : b_voff[nt]) + 16, soff, 0));
-            dst[nt]       = f8f8_frag(lo, hi);
-        }
+    for(int i = 0; i < T::A_DMA; ++i)
+#pragma unroll
+        for(int h = 0; h < 2; ++h)
+            a_run[h][i] = (uint32_t)a_row(h, i) * (uint32_t)p.lda + k0;
+#pragma unroll
+    for(int i = 0; i < T::B_DMA; ++i)
+        b_run[i] = (uint32_t)((wave * T::B_DMA + i) * 8) * (uint32_t)p.ldb + k0;
+    auto lds_at = [&](int at) __attribute__((always_inline)) { return (__attribute__((address_space(3))) void*)(lds + at); };
+    auto dma_a = [&](const __amdgpu_buffer_rsrc_t& rsrc, int slot, int h, int i, bool last) __attribute__((always_inline)) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, lds_at(slot * T::SLOT + a_row(h, i) * 128), 16, TAIL && last && past ? OUT : a_lane,
+                                                 a_run[h][i], 0, 0);
+        a_run[h][i] += T::BK;
+    };
+    auto dma_b = [&](const __amdgpu_buffer_rsrc_t& rsrc, int slot, int i, bool last) __attribute__((always_inline)) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, lds_at(slot * T::SLOT + T::A_TILE + (wave * T::B_DMA + i) * 1024), 16,
+                                                 TAIL && last && past ? OUT : b_lane, b_run[i], 0, 0);
+        b_run[i] += T::BK;
     };
 
     // Scale pieces: waves 0 .. BM / 64 - 1 fetch the scales of 64 rows each, the others all the same piece with the column
-    // blocks' (one lane per wave of columns); four consecutive K tiles per lane, 16 bytes from a 4-byte aligned address.
+    // blocks' (one lane per 32 columns); four consecutive K tiles per lane, 16 bytes from a 4-byte aligned address.
     const bool s_is_row = wave < T::BM / 64;
     __amdgpu_buffer_rsrc_t s_rsrc;
     uint32_t s_lane;
@@ -384,9 +393,9 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
         const __amdgpu_buffer_rsrc_t sa = resource(p.sa + (size_t)ra * (size_t)p.ld_sa, ((long)(ra_last - ra) * p.ld_sa + kblocks) * 4);
         const __amdgpu_buffer_rsrc_t sb = resource(p.sb + (size_t)rb * (size_t)p.ld_sb, ((long)(rb_last - rb) * p.ld_sb + kblocks) * 4);
         s_rsrc = s_is_row ? sa : sb;
-        const int row = min(m0 + (wave < T::BM / 64 ? wave : 0) * 64 + lane, p.M - 1) / p.bm - ra;
+        const int row = min(m0 + (s_is_row ? wave : 0) * 64 + lane, p.M - 1) / p.bm - ra;
         const int blk = min(n0 + lane * 32, p.N - 1) / p.bn - rb;
-        s_lane = s_is_row ? (uint32_t)row * (uint32_t)p.ld_sa * 4u : lane < T::WAVES ? (uint32_t)blk * (uint32_t)p.ld_sb * 4u : OUT;
+        s_lane = s_is_row ? (uint32_t)row * (uint32_t)p.ld_sa * 4u : lane < T::BN / 32 ? (uint32_t)blk * (uint32_t)p.ld_sb * 4u : OUT;
     }
     // the four scales of tile `tile`'s group: from 4 (tile / 4), or the last four of the table row
     const int s_end = (p.K + T::BK - 1) / T::BK - kt0 - 4;
@@ -394,144 +403,129 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
     // (not due: a piece of zeros into a place nobody reads, so that every tile issues the same number of pieces)
     auto dma_s = [&](int tile, bool due) __attribute__((always_inline)) {
         const int at = due ? T::S_OFF + ((tile >> 2) & 1) * T::S_SLOT + (s_is_row ? wave * 1024 : T::S_ROWS) : T::S_DUMP;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(due ? s_rsrc : null_rsrc, (__attribute__((address_space(3))) void*)(lds + at), 16, s_lane,
-                                                 (uint32_t)(kt0 + s_first(tile)) * 4u, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(due ? s_rsrc : null_rsrc, lds_at(at), 16, s_lane, (uint32_t)(kt0 + s_first(tile)) * 4u, 0, 0);
     };
 
-    int a_off[2]; // this lane's two 16-byte chunks of row fr of row block 0 (swizzled position inside the 128-byte row)
+    // this lane's two 16-byte chunks of row fr of a 16-row block (swizzled position inside the 128-byte row)
+    const int f_lo = fr * 128 + (((2 * fq) ^ f8_a_swz(fr)) << 4), f_hi = fr * 128 + (((2 * fq + 1) ^ f8_a_swz(fr)) << 4);
+    i8v_t af[2], bf[NT];
+    auto read_frag = [&](const uint8_t* block) __attribute__((always_inline)) { return f8f8_frag(*(const u4_t*)(block + f_lo), *(const u4_t*)(block + f_hi)); };
+    auto read_a = [&](int slot, int mt) __attribute__((always_inline)) { return read_frag(lds + slot * T::SLOT + (wr * MT + mt) * 2048); };
+    auto read_b = [&](int slot, int nt) __attribute__((always_inline)) { return read_frag(lds + slot * T::SLOT + T::A_TILE + (wc * NT + nt) * 2048); };
+    auto group0 = [&](int tile, bool s_due, int slot) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t ra = tile < ntiles ? a_rsrc : null_rsrc, rb = tile < ntiles ? b_rsrc : null_rsrc;
+        dma_s(tile, s_due && tile < ntiles);
 #pragma unroll
-    for(int h = 0; h < 2; ++h)
-        a_off[h] = fr * 128 + (((2 * fq + h) ^ f8_a_swz(fr)) << 4);
-    i8v_t af[WIN];
-    i8v_t bf[3][NT]; // weights of tiles t, t + 1, t + 2 (by tile mod 3)
-    auto read_a = [&](int slot, int mt, auto win) __attribute__((always_inline)) {
-        const uint8_t* sp = lds + slot * T::A_TILE + mt * 16 * 128;
-        af[decltype(win)::value] = f8f8_frag(*(const u4_t*)(sp + a_off[0]), *(const u4_t*)(sp + a_off[1]));
+        for(int i = 0; i < T::A_DMA; ++i)
+            dma_a(ra, slot, 0, i, tile == ntiles - 1);
+#pragma unroll
+        for(int i = 0; i < T::B_DMA; ++i)
+            dma_b(rb, slot, i, tile == ntiles - 1);
     };
-
-    // ---- prologue: S(0..3), A(0), B(0), A(1), B(1), A(2); tile 0 complete, first LEAD fragments fetched ----
-    dma_s(0, true);
+    auto group1 = [&](int tile, int slot) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t ra = tile < ntiles ? a_rsrc : null_rsrc;
 #pragma unroll
-    for(int i = 0; i < AD; ++i)
-        dma_a(a_rsrc, 0, i, ntiles == 1);
-    load_b(b_rsrc, bf[0], 0);
+        for(int i = 0; i < T::A_DMA; ++i)
+            dma_a(ra, slot, 1, i, tile == ntiles - 1);
+    };
+    constexpr int G0 = 1 + T::A_DMA + T::B_DMA, G1 = T::A_DMA;
+
+    group0(0, true, 0);
     __builtin_amdgcn_sched_barrier(0); // (issue order is part of the vmcnt arithmetic)
-    {
-        const __amdgpu_buffer_rsrc_t a1 = ntiles > 1 ? a_rsrc : null_rsrc, b1 = ntiles > 1 ? b_rsrc : null_rsrc;
-        const __amdgpu_buffer_rsrc_t a2 = ntiles > 2 ? a_rsrc : null_rsrc;
-#pragma unroll
-        for(int i = 0; i < AD; ++i)
-            dma_a(a1, 1, i, ntiles == 2);
-        __builtin_amdgcn_sched_barrier(0);
-        load_b(b1, bf[1], 1);
-        __builtin_amdgcn_sched_barrier(0);
-        dma_s(0, false); // (the place of a tile's scale piece in the count)
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for(int i = 0; i < AD; ++i)
-            dma_a(a2, 2, i, ntiles == 3);
-    }
+    group1(0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    group0(1, false, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    group1(1, 1);
     __builtin_amdgcn_sched_barrier(0);
     clear_acc();
-    wait_vmcnt<2 * AD + 1 + 2 * NT>(); // S(0), A(0), B(0) done
+    wait_vmcnt<G0 + 2 * G1>(); // group (0, 0) done
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    read_a(0, 0, std::integral_constant<int, 0>{});
-    read_a(0, 1, std::integral_constant<int, 1>{});
-    read_a(0, 2, std::integral_constant<int, 2>{});
-    static_assert(LEAD == 3 && MT % WIN == 0, "prologue fetches LEAD fragments; a row block's window entry must not depend on the tile");
+#pragma unroll
+    for(int nt = 0; nt < NT; ++nt)
+        bf[nt] = read_b(0, nt);
+    af[0] = read_a(0, 0);
     __builtin_amdgcn_sched_barrier(0);
 
-    f4_t pend[2][NT]; // block sums of this and the previous row block (by row block parity), not yet folded in
-    int slot = 0, t = 0;
-    auto tile_body = [&](auto set) __attribute__((always_inline)) {
-        constexpr int P = decltype(set)::value, P2 = (P + 2) % 3;
-        const int slot1 = (slot + 1) & 3, slot3 = (slot + 3) & 3;
-        const __amdgpu_buffer_rsrc_t b2 = t + 2 < ntiles ? b_rsrc : null_rsrc;
-        const __amdgpu_buffer_rsrc_t a3 = t + 3 < ntiles ? a_rsrc : null_rsrc;
-        const bool a3_last              = t + 3 == ntiles - 1;
-        const uint8_t* sp               = lds + T::S_OFF + ((t >> 2) & 1) * T::S_SLOT + (t - s_first(t)) * 4;
-        const float* row_s              = (const float*)(sp + fr * 16);                      // row 16 mt + fr at [64 mt]
-        const float sb                  = *(const float*)(sp + T::S_ROWS + wave * 16) * p.fnuz;
-        float s_cur = row_s[0], s_prev = 0.f;
+    f4_t pend[NT];        // block sums not yet folded in: of the previous row block
+    float s_fold[NT / 2]; // and their factors, per 32 columns
+#pragma unroll
+    for(int nt = 0; nt < NT; ++nt)
+        pend[nt] = f4_t{0.f, 0.f, 0.f, 0.f}, s_fold[nt / 2] = 0.f;
+    for(int t = 0; t < ntiles; ++t)
+    {
+        const int slot    = t & 1;
+        const uint8_t* sp = lds + T::S_OFF + ((t >> 2) & 1) * T::S_SLOT + (t - s_first(t)) * 4;
+        const float* row_s = (const float*)(sp + (wr * MT * 16 + fr) * 16); // row 16 mt + fr at [64 mt]
+        float sb[NT / 2];
+#pragma unroll
+        for(int h = 0; h < NT / 2; ++h)
+            sb[h] = *(const float*)(sp + T::S_ROWS + (wc * (NT / 2) + h) * 16) * p.fnuz;
+        float s_row = row_s[0];
 
         auto row_block = [&](auto mt_c) __attribute__((always_inline)) {
-            constexpr int mt = decltype(mt_c)::value, w = mt % WIN, wn = (mt + LEAD) % WIN, cur = mt & 1, prv = cur ^ 1;
-            if constexpr(mt == MT - LEAD)
+            constexpr int mt = decltype(mt_c)::value, prev = (mt + MT - 1) % MT;
+            if constexpr(mt == MH - 1 || mt == MT - 1)
             {
-                // tile t + 1 complete for everybody; every wave is past its reads of tile t - 1, whose slot is free
-                wait_vmcnt<AD + 1 + 4 * NT>();
+                wait_vmcnt<G0 + G1>();
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if constexpr(mt + LEAD < MT)
-                read_a(slot, mt + LEAD, std::integral_constant<int, wn>{});
-            else
-                read_a(slot1, mt + LEAD - MT, std::integral_constant<int, wn>{});
-            if constexpr(mt == 0)
-                load_b(b2, bf[P2], t + 2); // (its set held tile t - 1's)
-            if constexpr(mt == MT - LEAD)
-                dma_s(t + 3, (t & 3) == 1 && t + 3 < ntiles); // (the slot of tiles t - 5 .. t - 2)
-            if constexpr(mt >= MT - LEAD)
-            {
-                constexpr int i0 = mt - (MT - LEAD), per = (AD + LEAD - 1) / LEAD;
-#pragma unroll
-                for(int i = i0 * per; i < (i0 + 1) * per && i < AD; ++i)
-                    dma_a(a3, slot3, i, a3_last);
-            }
-            const float ps = s_prev;
-            s_prev         = s_cur * sb;
             if constexpr(mt + 1 < MT)
-                s_cur = row_s[64 * (mt + 1)];
+                af[(mt + 1) & 1] = read_a(slot, mt + 1);
+            else
+                af[0] = read_a(slot ^ 1, 0);
+            float s_now[NT / 2];
+#pragma unroll
+            for(int h = 0; h < NT / 2; ++h)
+                s_now[h] = s_row * sb[h];
+            if constexpr(mt + 1 < MT)
+                s_row = row_s[64 * (mt + 1)];
+            if constexpr(mt == MH - 1)
+                group0(t + 2, (t & 3) == 2, slot); // (scale slot: of tiles t - 6 .. t - 3)
+            if constexpr(mt == MT - 1)
+                group1(t + 2, slot);
             const f4_t zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for(int nt = 0; nt < NT; ++nt)
-                pend[cur][nt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[P][nt], af[w], zero, 0, 0, 0, 0, 0, 0);
-            if constexpr(mt > 0)
             {
-                const f4_t sv = {ps, ps, ps, ps};
-#pragma unroll
-                for(int nt = 0; nt < NT; ++nt)
-                    acc[nt][mt - 1] = __builtin_elementwise_fma(pend[prv][nt], sv, acc[nt][mt - 1]);
+                const float f  = s_fold[nt / 2];
+                acc[nt][prev] = __builtin_elementwise_fma(pend[nt], f4_t{f, f, f, f}, acc[nt][prev]);
+                pend[nt]      = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[nt], af[mt & 1], zero, 0, 0, 0, 0, 0, 0);
+                if constexpr(mt == MT - 1)
+                    bf[nt] = read_b(slot ^ 1, nt);
             }
-            if constexpr(mt == MT - 1) // (nothing is carried across the tile boundary)
+#pragma unroll
+            for(int h = 0; h < NT / 2; ++h)
+                s_fold[h] = s_now[h];
+#pragma unroll
+            for(int nt = 0; nt < NT; ++nt)
             {
-                const f4_t sv = {s_prev, s_prev, s_prev, s_prev};
-#pragma unroll
-                for(int nt = 0; nt < NT; ++nt)
-                    acc[nt][mt] = __builtin_elementwise_fma(pend[cur][nt], sv, acc[nt][mt]);
+                __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, mt == MT - 1 ? 2 : 1, 0);
             }
-            // both MFMAs first, the fragment reads and the vector work in their shadow
-            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 10, 0);
             __builtin_amdgcn_sched_barrier(0);
         };
         for_each_constant(row_block, std::make_integer_sequence<int, MT>{});
-        slot = slot1;
-        ++t;
-    };
-    for(;;)
+    }
+#pragma unroll
+    for(int nt = 0; nt < NT; ++nt)
     {
-        tile_body(std::integral_constant<int, 0>{});
-        if(t == ntiles)
-            break;
-        tile_body(std::integral_constant<int, 1>{});
-        if(t == ntiles)
-            break;
-        tile_body(std::integral_constant<int, 2>{});
-        if(t == ntiles)
-            break;
+        const float f   = s_fold[nt / 2];
+        acc[nt][MT - 1] = __builtin_elementwise_fma(pend[nt], f4_t{f, f, f, f}, acc[nt][MT - 1]);
     }
     wait_vmcnt<0>(); // (null-resource loads of tiles past the end still count)
-    __syncthreads(); // every wave is done with the ring before it becomes the C tile image
+    __syncthreads(); // every wave is done with the slots before they become the C tile image
     f8f8_epilogue<T>(p, acc, lds, m0, n0, wave, lane);
 }
 
 template <bool TAIL>
-__global__ __launch_bounds__(512, 2) void wq_gemm_f8f8_256(const F8F8Params p) { f8f8_tile_body<F8F8Tile<16, 8>, TAIL>(p); }
+__global__ __launch_bounds__(512, 2) void wq_gemm_f8f8_256(const F8F8Params p) { f8f8_tile_body<F8F8Tile<8, 4, 2, 4>, TAIL>(p); }
 template <bool TAIL>
-__global__ __launch_bounds__(256, 2) void wq_gemm_f8f8_128(const F8F8Params p) { f8f8_tile_body<F8F8Tile<8, 4>, TAIL>(p); }
+__global__ __launch_bounds__(256, 2) void wq_gemm_f8f8_128(const F8F8Params p) { f8f8_tile_body<F8F8Tile<4, 4, 2, 2>, TAIL>(p); }
 
 // Split-K: out[m, n] = epilogue(sum_z slab[z][m][n]), z ascending, for any N (ld_part is N rounded up to 4).
 __global__ __launch_bounds__(256) void wq_reduce_f8f8(const float* __restrict__ slabs, int k_batch, int ld_part, F8F8Params p)

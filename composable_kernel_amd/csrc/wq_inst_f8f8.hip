@@ -37,9 +37,9 @@ int launch_f8f8(int kernel, const F8F8Params& p, int k_batch, hipStream_t s)
     switch(kernel)
     {
     case F8F8_256:
-        return tail ? launch_tile<F8F8Tile<16, 8>, wq_gemm_f8f8_256<true>>(p, grid, s) : launch_tile<F8F8Tile<16, 8>, wq_gemm_f8f8_256<false>>(p, grid, s);
+        return tail ? launch_tile<F8F8Tile<8, 4, 2, 4>, wq_gemm_f8f8_256<true>>(p, grid, s) : launch_tile<F8F8Tile<8, 4, 2, 4>, wq_gemm_f8f8_256<false>>(p, grid, s);
     case F8F8_128:
-        return tail ? launch_tile<F8F8Tile<8, 4>, wq_gemm_f8f8_128<true>>(p, grid, s) : launch_tile<F8F8Tile<8, 4>, wq_gemm_f8f8_128<false>>(p, grid, s);
+        return tail ? launch_tile<F8F8Tile<4, 4, 2, 2>, wq_gemm_f8f8_128<true>>(p, grid, s) : launch_tile<F8F8Tile<4, 4, 2, 2>, wq_gemm_f8f8_128<false>>(p, grid, s);
     default: hipLaunchKernelGGL(wq_gemm_f8f8_any, grid, dim3(256), 0, s, p); return WQ_OK;
     }
 }

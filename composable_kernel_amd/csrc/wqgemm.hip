@@ -1415,8 +1415,8 @@ int wqgemm_type_string(const wqgemm_problem* p, char* buf, size_t n)
                  !has_block_scales(p) ? "" : p->scale_block_m % 128 == 0 ? ", ABScalePer128K" : ", ABScalePer128K_RowScaleA");
     else if(plan.route == ROUTE_F8F8)
         snprintf(buf, n, "DeviceGemmMultiD_ABScale_Mfma_gfx950<%s, 16x16x128_f8f6f4, %s, %s, %s, KBatch%d>",
-                 plan.f8f8 == wq::F8F8_256   ? "512, 256, 256, 128, LdsDmaA, DirectB"
-                 : plan.f8f8 == wq::F8F8_128 ? "256, 128, 128, 128, LdsDmaA, DirectB"
+                 plan.f8f8 == wq::F8F8_256   ? "512, 256, 256, 128, LdsDma"
+                 : plan.f8f8 == wq::F8F8_128 ? "256, 128, 128, 128, LdsDma"
                                              : "256, 128, 128, 128, AnyAlignment",
                  dt_name(p->a_dtype), dt_name(p->b_dtype), dt_name(p->c_dtype), plan.k_batch);
     else if(plan.route == ROUTE_SKINNY_WS)
