@@ -195,8 +195,8 @@ __global__ __launch_bounds__(256) void wq_gemm_f8f8_any(const F8F8Params p)
 // with 64, two workgroups per CU).
 //   * two LDS slots of a whole K tile; each half of a tile's rows has a barrier of its own, in front of the row block that first
 //     reads the next half, and refills what the half before it has freed: every piece is issued at least a K tile's time before
-//     its barrier.  Weights live in registers for a K tile: read at its end, each column block behind the last MFMA that needs
-//     the old one, so that their slot is free for most of it;
+//     its barrier.  Weights live in registers for a K tile, in two sets: the next tile's are read while this one is multiplied,
+//     a column block per row block (read all at a tile's end they held every wave up behind 80 KiB of LDS reads at once);
 //   * scales: once per four K tiles the row scales of those four travel as one 16-byte LDS-DMA piece per row (every row's scales
 //     lie in a cache line of their own, so fetching them tile by tile would move a line per row and tile, as much as the
 //     activations themselves), and the column blocks' the same way; needs four K tiles in all, K > 384;
@@ -205,9 +205,9 @@ __global__ __launch_bounds__(256) void wq_gemm_f8f8_any(const F8F8Params p)
 //     issued, so that neither waits for the other.
 // VMEM bookkeeping (in-order completion, counted waits).  Behind barrier(t, 0), in front of row block MT / 2 - 1 of tile t:
 // A(t + 2) first half, B(t + 2), one scale piece [group (t, 0)]; behind barrier(t, 1), in front of row block MT - 1: A(t + 2)
-// second half [group (t, 1)].  barrier(t, 0) needs group (t - 2, 1) = A(t) second half, barrier(t, 1) needs group (t - 1, 0) =
-// A(t + 1) first half, B(t + 1), scales: two groups, one of each kind, were issued behind either.  Each wave also waits for its
-// own LDS reads in front of a barrier: what the pieces behind it overwrite has been read by everybody.  (The tile body has no
+// second half [group (t, 1)].  barrier(t, 0) needs group (t - 2, 1) = A(t) second half and group (t - 1, 0) = A(t + 1) first half,
+// B(t + 1), scales: one group (t - 1, 1) was issued behind.  barrier(t, 1) makes room only.  Each wave also waits for its own LDS
+// reads in front of a barrier: what the pieces behind it overwrite has been read by everybody.  (The tile body has no
 // branch: the compiler would sink the fused multiply-adds behind it and keep every block sum alive.)
 // Tiles past the last one are loaded through a resource of zero records: no memory access.  TAIL: the last K tile is partial
 // (K a multiple of 16): its 16-byte pieces past the end are sent out of range, which reads as zeros.
@@ -230,7 +230,7 @@ struct F8F8Tile
     static constexpr int LDS_C    = BM * C_PITCH > BM / 2 * F_PITCH ? BM * C_PITCH : BM / 2 * F_PITCH;
     static constexpr int LDS_BYTES = LDS_MAIN > LDS_C ? LDS_MAIN : LDS_C;
     static_assert(BM / 64 < WAVES, "one scale piece per 64 rows and one for the columns, a wave each");
-    static_assert(MT % 2 == 0 && NT % 2 == 0 && A_DMA * 16 * WAVES == BM && B_DMA * 8 * WAVES == BN, "whole pieces");
+    static_assert(MT % 2 == 0 && NT % 2 == 0 && NT % (MT / 2) == 0 && A_DMA * 16 * WAVES == BM && B_DMA * 8 * WAVES == BN, "whole pieces");
     static_assert(LDS_BYTES <= 160 * 1024, "LDS");
 };
 
@@ -408,7 +408,7 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
 
     // this lane's two 16-byte chunks of row fr of a 16-row block (swizzled position inside the 128-byte row)
     const int f_lo = fr * 128 + (((2 * fq) ^ f8_a_swz(fr)) << 4), f_hi = fr * 128 + (((2 * fq + 1) ^ f8_a_swz(fr)) << 4);
-    i8v_t af[2], bf[NT];
+    i8v_t af[2], bf[2][NT]; // fragments of row blocks mt, mt + 1; weights of tiles t, t + 1 (by tile parity)
     auto read_frag = [&](const uint8_t* block) __attribute__((always_inline)) { return f8f8_frag(*(const u4_t*)(block + f_lo), *(const u4_t*)(block + f_hi)); };
     auto read_a = [&](int slot, int mt) __attribute__((always_inline)) { return read_frag(lds + slot * T::SLOT + (wr * MT + mt) * 2048); };
     auto read_b = [&](int slot, int nt) __attribute__((always_inline)) { return read_frag(lds + slot * T::SLOT + T::A_TILE + (wc * NT + nt) * 2048); };
@@ -444,7 +444,7 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for(int nt = 0; nt < NT; ++nt)
-        bf[nt] = read_b(0, nt);
+        bf[0][nt] = read_b(0, nt);
     af[0] = read_a(0, 0);
     __builtin_amdgcn_sched_barrier(0);
 
@@ -453,9 +453,9 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
 #pragma unroll
     for(int nt = 0; nt < NT; ++nt)
         pend[nt] = f4_t{0.f, 0.f, 0.f, 0.f}, s_fold[nt / 2] = 0.f;
-    for(int t = 0; t < ntiles; ++t)
-    {
-        const int slot    = t & 1;
+    int t = 0;
+    auto tile_body = [&](auto parity) __attribute__((always_inline)) {
+        constexpr int slot = decltype(parity)::value;
         const uint8_t* sp = lds + T::S_OFF + ((t >> 2) & 1) * T::S_SLOT + (t - s_first(t)) * 4;
         const float* row_s = (const float*)(sp + (wr * MT * 16 + fr) * 16); // row 16 mt + fr at [64 mt]
         float sb[NT / 2];
@@ -468,7 +468,8 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
             constexpr int mt = decltype(mt_c)::value, prev = (mt + MT - 1) % MT;
             if constexpr(mt == MH - 1 || mt == MT - 1)
             {
-                wait_vmcnt<G0 + G1>();
+                if constexpr(mt == MH - 1)
+                    wait_vmcnt<G1>();
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
                 __builtin_amdgcn_sched_barrier(0);
@@ -483,6 +484,10 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
                 s_now[h] = s_row * sb[h];
             if constexpr(mt + 1 < MT)
                 s_row = row_s[64 * (mt + 1)];
+            constexpr int BPER = mt >= MH - 1 && mt < MT - 1 ? NT / MH : 0;
+#pragma unroll
+            for(int i = 0; i < BPER; ++i)
+                bf[slot ^ 1][(mt - (MH - 1)) * BPER + i] = read_b(slot ^ 1, (mt - (MH - 1)) * BPER + i);
             if constexpr(mt == MH - 1)
                 group0(t + 2, (t & 3) == 2, slot); // (scale slot: of tiles t - 6 .. t - 3)
             if constexpr(mt == MT - 1)
@@ -493,9 +498,7 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
             {
                 const float f  = s_fold[nt / 2];
                 acc[nt][prev] = __builtin_elementwise_fma(pend[nt], f4_t{f, f, f, f}, acc[nt][prev]);
-                pend[nt]      = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[nt], af[mt & 1], zero, 0, 0, 0, 0, 0, 0);
-                if constexpr(mt == MT - 1)
-                    bf[nt] = read_b(slot ^ 1, nt);
+                pend[nt]      = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[slot][nt], af[mt & 1], zero, 0, 0, 0, 0, 0, 0);
             }
 #pragma unroll
             for(int h = 0; h < NT / 2; ++h)
@@ -505,11 +508,21 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
             {
                 __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, mt == MT - 1 ? 2 : 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1 + BPER, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         };
         for_each_constant(row_block, std::make_integer_sequence<int, MT>{});
+        ++t;
+    };
+    for(;;)
+    {
+        tile_body(integral_constant<int, 0>{});
+        if(t == ntiles)
+            break;
+        tile_body(integral_constant<int, 1>{});
+        if(t == ntiles)
+            break;
     }
 #pragma unroll
     for(int nt = 0; nt < NT; ++nt)
