@@ -26,13 +26,14 @@ struct F8F8Params
     int bm, bn, ld_sa, ld_sb;
     int k_begin, k_end, k_per_z; // slices start on multiples of 128
     int partial;
+    int slices;                  // K slices (split-K)
     int tiles_m, tiles_n, group_m;
     float fnuz; // 2^-(number of FNUZ operands)
     int bf16_rtn; // bf16 outputs rounded to nearest even under every epilogue (else truncated, as everywhere in this engine)
     EpilogueArgs epi;
 };
 
-int launch_f8f8(int kernel, const F8F8Params& p, int k_batch, hipStream_t s);
+int launch_f8f8(int kernel, const F8F8Params& p, hipStream_t s);
 void launch_reduce_f8f8(const float* slabs, int k_batch, int ld_part, const F8F8Params& p, hipStream_t s);
 
 } // namespace wq

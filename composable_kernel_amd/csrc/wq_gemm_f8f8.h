@@ -24,14 +24,14 @@ __device__ __forceinline__ uint16_t f8f8_cvt16(const F8F8Params& p, float v)
 
 // Four consecutive outputs (n .. n+3) of row m: epilogue, conversion, store; columns at and past N are left alone.
 // (the kind is resolved at run time: this runs once per four outputs, outside the unrolled fragment loops)
-__device__ __forceinline__ void f8f8_store4(const F8F8Params& p, f4_t v, int m, int n)
+__device__ __forceinline__ void f8f8_store4(const F8F8Params& p, f4_t v, int m, int n, int z)
 {
     if(m >= p.M || n >= p.N)
         return;
     const int cols = min(p.N - n, 4);
     if(p.partial)
     {
-        float* c = (float*)p.c + ((size_t)blockIdx.z * p.M + m) * (size_t)p.ldc + n;
+        float* c = (float*)p.c + ((size_t)z * p.M + m) * (size_t)p.ldc + n;
         if(cols == 4)
             __builtin_memcpy(c, &v, 16);
         else
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256) void wq_gemm_f8f8_any(const F8F8Params p)
         for(int i = 0; i < 4; ++i)
         {
             const int r = i * 8 + (threadIdx.x >> 5), c = (threadIdx.x & 31) * 4;
-            f8f8_store4(p, *(const f4_t*)(lds_c + r * T::C_PITCH + c), m0 + ph * 32 + r, n0 + c);
+            f8f8_store4(p, *(const f4_t*)(lds_c + r * T::C_PITCH + c), m0 + ph * 32 + r, n0 + c, blockIdx.z);
         }
         __syncthreads();
     }
@@ -195,27 +195,29 @@ __global__ __launch_bounds__(256) void wq_gemm_f8f8_any(const F8F8Params p)
 // with 64, two workgroups per CU).
 //   * two LDS slots of a whole K tile; each half of a tile's rows has a barrier of its own, in front of the row block that first
 //     reads the next half, and refills what the half before it has freed: every piece is issued at least a K tile's time before
-//     its barrier.  Weights live in registers for a K tile, in two sets: the next tile's are read while this one is multiplied,
-//     a column block per row block (read all at a tile's end they held every wave up behind 80 KiB of LDS reads at once);
+//     its barrier.  Weights live in registers for a K tile: read at its end, each column block behind the last MFMA that needs
+//     the old one, so that their slot is free for most of it.  Activations are read LEAD row blocks ahead;
 //   * scales: once per four K tiles the row scales of those four travel as one 16-byte LDS-DMA piece per row (every row's scales
 //     lie in a cache line of their own, so fetching them tile by tile would move a line per row and tile, as much as the
 //     activations themselves), and the column blocks' the same way; needs four K tiles in all, K > 384;
 //   * a block sum is one MFMA from a zero accumulator.  The sums of a row block are folded into the accumulators,
 //     acc = fma(sum, sa * sb, acc), each just in front of the next row block's MFMA that overwrites it: NT MFMAs after it was
 //     issued, so that neither waits for the other.
-// VMEM bookkeeping (in-order completion, counted waits).  Behind barrier(t, 0), in front of row block MT / 2 - 1 of tile t:
-// A(t + 2) first half, B(t + 2), one scale piece [group (t, 0)]; behind barrier(t, 1), in front of row block MT - 1: A(t + 2)
-// second half [group (t, 1)].  barrier(t, 0) needs group (t - 2, 1) = A(t) second half and group (t - 1, 0) = A(t + 1) first half,
-// B(t + 1), scales: one group (t - 1, 1) was issued behind.  barrier(t, 1) makes room only.  Each wave also waits for its own LDS
-// reads in front of a barrier: what the pieces behind it overwrite has been read by everybody.  (The tile body has no
+// VMEM bookkeeping (in-order completion, counted waits).  Behind barrier(t, 0), in front of row block MT / 2 - LEAD of tile t:
+// A(t + 2) first half, B(t + 2), one scale piece [group (t, 0)]; behind barrier(t, 1), in front of row block MT - LEAD: A(t + 2)
+// second half [group (t, 1)].  barrier(t, 0) needs group (t - 2, 1) = A(t) second half, barrier(t, 1) needs group (t - 1, 0) =
+// A(t + 1) first half, B(t + 1), scales: two groups, one of each kind, were issued behind either.  Each wave also waits for its
+// own LDS reads in front of a barrier: what the pieces behind it overwrite has been read by everybody.  (The tile body has no
 // branch: the compiler would sink the fused multiply-adds behind it and keep every block sum alive.)
+// STREAM (epilogues with at most a bias per column and a FastGelu): a workgroup walks tiles blockIdx.x, + gridDim.x, ... and
+// issues the next tile's first loads before this one's outputs leave.
 // Tiles past the last one are loaded through a resource of zero records: no memory access.  TAIL: the last K tile is partial
 // (K a multiple of 16): its 16-byte pieces past the end are sent out of range, which reads as zeros.
 // ---------------------------------------------------------------------------------------------
-template <int MT_, int NT_, int WR_, int WC_>
+template <int MT_, int NT_, int WR_, int WC_, int LEAD_>
 struct F8F8Tile
 {
-    static constexpr int MT = MT_, NT = NT_, WR = WR_, WC = WC_, WAVES = WR * WC;
+    static constexpr int MT = MT_, NT = NT_, WR = WR_, WC = WC_, WAVES = WR * WC, LEAD = LEAD_, WIN = LEAD + 1;
     static constexpr int BM = WR * MT * 16, BN = WC * NT * 16, BK = 128, THREADS = WAVES * 64;
     static constexpr int A_TILE  = BM * BK, B_TILE = BN * BK, SLOT = A_TILE + B_TILE;
     static constexpr int A_DMA   = BM / 16 / WAVES; // pieces per wave and half of A
@@ -224,63 +226,109 @@ struct F8F8Tile
     static constexpr int S_SLOT  = S_ROWS + 1024; // + one piece for the column blocks (lanes 0 .. BN / 32 - 1)
     static constexpr int S_OFF   = 2 * SLOT;
     static constexpr int S_DUMP  = S_OFF + 2 * S_SLOT;
-    static constexpr int C_PITCH = BN * 2 + 16;   // 16-bit image of the C tile
-    static constexpr int F_PITCH = BN * 4 + 16;   // fp32 image of half of it
-    static constexpr int LDS_MAIN = S_DUMP + 1024;
-    static constexpr int LDS_C    = BM * C_PITCH > BM / 2 * F_PITCH ? BM * C_PITCH : BM / 2 * F_PITCH;
-    static constexpr int LDS_BYTES = LDS_MAIN > LDS_C ? LDS_MAIN : LDS_C;
+    static constexpr int ST_PITCH = NT * 32 + 16;  // a wave's own 16-bit image of one row block
+    static constexpr int ST_OFF   = S_DUMP + 1024;
+    static constexpr int F_PITCH  = BN * 4 + 16;   // fp32 image of half the tile
+    static constexpr int LDS_MAIN = ST_OFF + WAVES * 16 * ST_PITCH;
+    static constexpr int LDS_BYTES = LDS_MAIN > BM / 2 * F_PITCH ? LDS_MAIN : BM / 2 * F_PITCH;
     static_assert(BM / 64 < WAVES, "one scale piece per 64 rows and one for the columns, a wave each");
-    static_assert(MT % 2 == 0 && NT % 2 == 0 && NT % (MT / 2) == 0 && A_DMA * 16 * WAVES == BM && B_DMA * 8 * WAVES == BN, "whole pieces");
+    static_assert(MT % 2 == 0 && NT % 2 == 0 && MT % WIN == 0 && LEAD < MT / 2 + 1 && A_DMA * 16 * WAVES == BM && B_DMA * 8 * WAVES == BN, "whole pieces");
     static_assert(LDS_BYTES <= 160 * 1024, "LDS");
 };
 
+// Epilogues with at most a bias per column and a FastGelu: every wave turns one row block at a time into whole lines through a
+// piece of LDS of its own, so that neither the slots nor a barrier are needed and the next tile's loads run underneath.
+// (N and ldc multiples of 8, C 16-byte aligned: whole 16-byte pieces; pieces past M or N fall out of the buffer resource.)
+enum F8F8Out { F8F8_F16, F8F8_BF16_TRUNC, F8F8_BF16_RTN };
+
+template <class T, F8F8Out OUTK>
+__device__ __forceinline__ void f8f8_stream_rows(const f4_t (&acc)[T::NT][T::MT], uint8_t* st, const __amdgpu_buffer_rsrc_t& rsrc, uint32_t voff,
+                                                 uint32_t row_bytes, int lane)
+{
+    constexpr int CH = T::NT * 2, RPI = 64 / CH; // 16-byte pieces of a row, rows per store instruction
+    uint8_t* w       = st + (lane & 15) * T::ST_PITCH + (lane >> 4) * 8;
+    const uint8_t* r = st + lane / CH * T::ST_PITCH + lane % CH * 16;
+#pragma unroll
+    for(int mt = 0; mt < T::MT; ++mt)
+    {
+#pragma unroll
+        for(int nt = 0; nt < T::NT; ++nt)
+        {
+            f4_t v = acc[nt][mt];
+            if constexpr(OUTK == F8F8_BF16_RTN)
+                v = f4_t{convert_bf16_rtn_bits(v[0]), convert_bf16_rtn_bits(v[1]), convert_bf16_rtn_bits(v[2]), convert_bf16_rtn_bits(v[3])};
+            *(u2_t*)(w + nt * 32) = pack_out4<OUTK != F8F8_F16>(v);
+        }
+        // (a wave's LDS operations are executed in order: no barrier between its own writes, reads and the next block's writes)
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for(int i = 0; i < 16 / RPI; ++i)
+        {
+            const u4_t v = *(const u4_t*)(r + i * RPI * T::ST_PITCH);
+            __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, voff, (uint32_t)(mt * 16 + i * RPI) * row_bytes, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 template <class T>
-__device__ __forceinline__ void f8f8_epilogue(const F8F8Params& p, const f4_t (&acc)[T::NT][T::MT], uint8_t* lds, int m0, int n0, int wave,
-                                              int lane)
+__device__ __forceinline__ void f8f8_epilogue_stream(const F8F8Params& p, f4_t (&acc)[T::NT][T::MT], uint8_t* lds, int m0, int n0, int wave,
+                                                     int lane)
 {
     constexpr int MT = T::MT, NT = T::NT;
-    const int fr = lane & 15, fq = lane >> 4, row = wave / T::WC * (MT * 16) + fr, col = wave % T::WC * (NT * 16) + fq * 4;
+    const int mw = m0 + wave / T::WC * (MT * 16), nw = n0 + wave % T::WC * (NT * 16);
     const int kind = p.epi.kind;
-    if(!p.partial && (kind == 0 || kind == 14))
+    if(kind == 6 || kind == 7)
     {
-        // no operand to fetch: converted on the way into LDS, out in 16-byte pieces, whole rows of the tile at a time
-        const bool bf = p.epi.c_dtype == 1 /*WQ_BF16*/, rtn = bf && (p.bf16_rtn || kind == 14);
+#pragma unroll
+        for(int nt = 0; nt < NT; ++nt)
+        {
+            f4_t d;
+#pragma unroll
+            for(int j = 0; j < 4; ++j)
+                d[j] = load_d_as_f32(p.epi.d0, min(nw + nt * 16 + (lane >> 4) * 4 + j, p.N - 1), p.epi.c_dtype);
+#pragma unroll
+            for(int mt = 0; mt < MT; ++mt)
+                acc[nt][mt] = acc[nt][mt] + d;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    if(kind == 1 || kind == 7)
+    {
 #pragma unroll
         for(int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for(int mt = 0; mt < MT; ++mt)
             {
-                f4_t v = acc[nt][mt];
-                if(rtn)
-                    v = f4_t{convert_bf16_rtn_bits(v[0]), convert_bf16_rtn_bits(v[1]), convert_bf16_rtn_bits(v[2]), convert_bf16_rtn_bits(v[3])};
-                *(u2_t*)(lds + (row + mt * 16) * T::C_PITCH + (col + nt * 16) * 2) = bf ? pack_out4<true>(v) : pack_out4<false>(v);
+                const f4_t v = acc[nt][mt];
+                acc[nt][mt]  = f4_t{fast_gelu(v[0]), fast_gelu(v[1]), fast_gelu(v[2]), fast_gelu(v[3])};
+                __builtin_amdgcn_sched_barrier(0);
             }
-        __syncthreads();
-        constexpr int CH = T::BN / 8; // 16-byte pieces of a row
-        uint16_t* c      = (uint16_t*)p.c + (size_t)m0 * (size_t)p.ldc + n0;
-        const bool wide  = p.ldc % 8 == 0 && (uintptr_t)p.c % 16 == 0;
-#pragma unroll 4
-        for(int i = threadIdx.x; i < T::BM * CH; i += T::THREADS)
-        {
-            const int r = i / CH, n = (i % CH) * 8;
-            const u4_t v = *(const u4_t*)(lds + r * T::C_PITCH + n * 2);
-            if(m0 + r >= p.M)
-                break;
-            uint16_t* d = c + (size_t)r * (size_t)p.ldc + n;
-            if(wide && n0 + n + 8 <= p.N)
-                *(u4_t*)d = v;
-            else
-            {
-#pragma unroll
-                for(int j = 0; j < 8; ++j)
-                    if(n0 + n + j < p.N)
-                        d[j] = (uint16_t)(v[j >> 1] >> (16 * (j & 1)));
-            }
-        }
-        return;
     }
-    // half of every wave's rows at a time as fp32; the epilogue and the edges in one rolled loop
-    const int row_h = wave / T::WC * (MT * 8) + fr;
+    if(mw >= p.M || nw >= p.N)
+        return;
+    constexpr int CH = NT * 2;
+    const uint32_t row_bytes = (uint32_t)p.ldc * 2;
+    const long bytes         = ((long)(p.M - mw - 1) * p.ldc + (p.N - nw)) * 2;
+    const __amdgpu_buffer_rsrc_t rsrc =
+        __builtin_amdgcn_make_buffer_rsrc((uint16_t*)p.c + (size_t)mw * (size_t)p.ldc + nw, 0, (int)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF), 0x00020000);
+    const uint32_t voff = nw + lane % CH * 8 < p.N ? (uint32_t)(lane / CH) * row_bytes + lane % CH * 16 : 0x80000000u;
+    uint8_t* st         = lds + T::ST_OFF + wave * (16 * T::ST_PITCH);
+    if(p.epi.c_dtype != 1 /*WQ_BF16*/)
+        f8f8_stream_rows<T, F8F8_F16>(acc, st, rsrc, voff, row_bytes, lane);
+    else if(p.bf16_rtn || kind == 14)
+        f8f8_stream_rows<T, F8F8_BF16_RTN>(acc, st, rsrc, voff, row_bytes, lane);
+    else
+        f8f8_stream_rows<T, F8F8_BF16_TRUNC>(acc, st, rsrc, voff, row_bytes, lane);
+}
+
+// Every epilogue, and fp32 slabs: half of every wave's rows at a time as fp32 through the slots, epilogue and edges in one rolled loop.
+template <class T>
+__device__ __forceinline__ void f8f8_epilogue_any(const F8F8Params& p, const f4_t (&acc)[T::NT][T::MT], uint8_t* lds, int m0, int n0, int z,
+                                                  int wave, int lane)
+{
+    constexpr int MT = T::MT, NT = T::NT;
+    const int fr = lane & 15, fq = lane >> 4, col = wave % T::WC * (NT * 16) + fq * 4, row = wave / T::WC * (MT * 8) + fr;
 #pragma unroll
     for(int ph = 0; ph < 2; ++ph)
     {
@@ -290,14 +338,14 @@ __device__ __forceinline__ void f8f8_epilogue(const F8F8Params& p, const f4_t (&
         for(int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for(int mi = 0; mi < MT / 2; ++mi)
-                *(f4_t*)(lds + (row_h + mi * 16) * T::F_PITCH + (col + nt * 16) * 4) = acc[nt][ph * (MT / 2) + mi];
+                *(f4_t*)(lds + (row + mi * 16) * T::F_PITCH + (col + nt * 16) * 4) = acc[nt][ph * (MT / 2) + mi];
         __syncthreads();
 #pragma unroll 2
         for(int i = threadIdx.x; i < T::BM / 2 * (T::BN / 4); i += T::THREADS)
         {
             const int r = i / (T::BN / 4), n = (i % (T::BN / 4)) * 4;
             const int m = r / (MT * 8) * (MT * 16) + ph * (MT * 8) + r % (MT * 8);
-            f8f8_store4(p, *(const f4_t*)(lds + r * T::F_PITCH + n * 4), m0 + m, n0 + n);
+            f8f8_store4(p, *(const f4_t*)(lds + r * T::F_PITCH + n * 4), m0 + m, n0 + n, z);
         }
     }
 }
@@ -308,44 +356,18 @@ __device__ __forceinline__ void for_each_constant(F& f, std::integer_sequence<in
     (f(std::integral_constant<int, I>{}), ...);
 }
 
-template <class T, bool TAIL>
+template <class T, bool TAIL, bool STREAM>
 __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
 {
-    constexpr int MT = T::MT, NT = T::NT, MH = MT / 2;
-    using std::integral_constant;
+    constexpr int MT = T::MT, NT = T::NT, MH = MT / 2, LEAD = T::LEAD, WIN = T::WIN;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave / T::WC, wc = wave % T::WC;
     const int fr = lane & 15, fq = lane >> 4;
-    int tm, tn;
-    tile_coords(xcd_remap(blockIdx.x, p.tiles_m * p.tiles_n), p.tiles_m, p.tiles_n, p.group_m, tm, tn);
-    const int m0 = tm * T::BM, n0 = tn * T::BN;
-    const int k0 = p.k_begin + blockIdx.z * p.k_per_z, k1 = min(p.k_end, k0 + p.k_per_z);
-    const int ntiles = (k1 - k0 + T::BK - 1) / T::BK;
-
-    f4_t acc[NT][MT];
-    auto clear_acc = [&]() __attribute__((always_inline)) {
-#pragma unroll
-        for(int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for(int mt = 0; mt < MT; ++mt)
-                acc[nt][mt] = f4_t{0.f, 0.f, 0.f, 0.f};
-    };
-    if(ntiles <= 0)
-    {
-        clear_acc();
-        f8f8_epilogue<T>(p, acc, lds, m0, n0, wave, lane);
-        return;
-    }
-
-    // Resources start at the tile's first row / column (the distance from there fits 32 bits: lda, ldb <= 2^22 is checked on
-    // the host) and end with the last byte of the last one: what lies past M or N reads as zeros.
     auto resource = [](const void* base, long bytes) __attribute__((always_inline)) {
         return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF), 0x00020000);
     };
-    const __amdgpu_buffer_rsrc_t a_rsrc = resource(p.a + (size_t)m0 * (size_t)p.lda, (long)(p.M - m0 - 1) * p.lda + p.K);
-    const __amdgpu_buffer_rsrc_t b_rsrc = resource(p.b + (size_t)n0 * (size_t)p.ldb, (long)(p.N - n0 - 1) * p.ldb + p.K);
     const __amdgpu_buffer_rsrc_t null_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)p.a, 0, 0, 0x00020000);
     constexpr uint32_t OUT = 0x80000000u; // an offset past every resource
 
@@ -354,20 +376,52 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
     const int chunk       = ((lane & 7) ^ f8_a_swz(lane >> 3)) << 4;
     const uint32_t a_lane = (uint32_t)(lane >> 3) * (uint32_t)p.lda + chunk;
     const uint32_t b_lane = (uint32_t)(lane >> 3) * (uint32_t)p.ldb + chunk;
-    const bool past       = chunk >= k1 - k0 - (ntiles - 1) * T::BK; // this lane's chunk of the last K tile lies past its end
     auto a_row = [&](int h, int i) __attribute__((always_inline)) {
         const int q = wave * T::A_DMA + i;
         return q / MT * (MT * 16) + h * (MT * 8) + q % MT * 8;
     };
-    uint32_t a_run[2][T::A_DMA], b_run[T::B_DMA];
+    // Scale pieces: waves 0 .. BM / 64 - 1 fetch the scales of 64 rows each, the others all the same piece with the column
+    // blocks' (one lane per 32 columns); four consecutive K tiles per lane, 16 bytes from a 4-byte aligned address.
+    const bool s_is_row = wave < T::BM / 64;
+    const int kblocks   = (p.K + T::BK - 1) / T::BK;
+
+    // ---- the unit of work at hand: a tile, or a K slice of one ----
+    const int tiles = p.tiles_m * p.tiles_n, units = tiles * p.slices;
+    int m0, n0, z, ntiles, kt0, s_end;
+    __amdgpu_buffer_rsrc_t a_rsrc, b_rsrc, s_rsrc;
+    uint32_t a_run[2][T::A_DMA], b_run[T::B_DMA], s_lane;
+    bool past;
+    auto set_unit = [&](int unit) __attribute__((always_inline)) {
+        int tm, tn;
+        z = unit / tiles;
+        tile_coords(xcd_remap(unit - z * tiles, tiles), p.tiles_m, p.tiles_n, p.group_m, tm, tn);
+        m0 = tm * T::BM, n0 = tn * T::BN;
+        const int k0 = p.k_begin + z * p.k_per_z, k1 = min(p.k_end, k0 + p.k_per_z);
+        ntiles = max(0, (k1 - k0 + T::BK - 1) / T::BK);
+        kt0    = k0 / T::BK;
+        s_end  = kblocks - kt0 - 4;
+        past   = chunk >= k1 - k0 - (ntiles - 1) * T::BK; // this lane's chunk of the last K tile lies past its end
+        // Resources start at the tile's first row / column (the distance from there fits 32 bits: lda, ldb <= 2^22 is checked
+        // on the host) and end with the last byte of the last one: what lies past M or N reads as zeros.
+        a_rsrc = resource(p.a + (size_t)m0 * (size_t)p.lda, (long)(p.M - m0 - 1) * p.lda + p.K);
+        b_rsrc = resource(p.b + (size_t)n0 * (size_t)p.ldb, (long)(p.N - n0 - 1) * p.ldb + p.K);
 #pragma unroll
-    for(int i = 0; i < T::A_DMA; ++i)
+        for(int i = 0; i < T::A_DMA; ++i)
 #pragma unroll
-        for(int h = 0; h < 2; ++h)
-            a_run[h][i] = (uint32_t)a_row(h, i) * (uint32_t)p.lda + k0;
+            for(int h = 0; h < 2; ++h)
+                a_run[h][i] = (uint32_t)a_row(h, i) * (uint32_t)p.lda + k0;
 #pragma unroll
-    for(int i = 0; i < T::B_DMA; ++i)
-        b_run[i] = (uint32_t)((wave * T::B_DMA + i) * 8) * (uint32_t)p.ldb + k0;
+        for(int i = 0; i < T::B_DMA; ++i)
+            b_run[i] = (uint32_t)((wave * T::B_DMA + i) * 8) * (uint32_t)p.ldb + k0;
+        // (scale tables relative to the tile's first table row; rows past M repeat the last one, columns past N the last block)
+        const int ra = m0 / p.bm, ra_last = (p.M - 1) / p.bm, rb = n0 / p.bn, rb_last = (p.N - 1) / p.bn;
+        const __amdgpu_buffer_rsrc_t sa = resource(p.sa + (size_t)ra * (size_t)p.ld_sa, ((long)(ra_last - ra) * p.ld_sa + kblocks) * 4);
+        const __amdgpu_buffer_rsrc_t sb = resource(p.sb + (size_t)rb * (size_t)p.ld_sb, ((long)(rb_last - rb) * p.ld_sb + kblocks) * 4);
+        s_rsrc = s_is_row ? sa : sb;
+        const int row = min(m0 + (s_is_row ? wave : 0) * 64 + lane, p.M - 1) / p.bm - ra;
+        const int blk = min(n0 + lane * 32, p.N - 1) / p.bn - rb;
+        s_lane = s_is_row ? (uint32_t)row * (uint32_t)p.ld_sa * 4u : lane < T::BN / 32 ? (uint32_t)blk * (uint32_t)p.ld_sb * 4u : OUT;
+    };
     auto lds_at = [&](int at) __attribute__((always_inline)) { return (__attribute__((address_space(3))) void*)(lds + at); };
     auto dma_a = [&](const __amdgpu_buffer_rsrc_t& rsrc, int slot, int h, int i, bool last) __attribute__((always_inline)) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, lds_at(slot * T::SLOT + a_row(h, i) * 128), 16, TAIL && last && past ? OUT : a_lane,
@@ -379,26 +433,7 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
                                                  TAIL && last && past ? OUT : b_lane, b_run[i], 0, 0);
         b_run[i] += T::BK;
     };
-
-    // Scale pieces: waves 0 .. BM / 64 - 1 fetch the scales of 64 rows each, the others all the same piece with the column
-    // blocks' (one lane per 32 columns); four consecutive K tiles per lane, 16 bytes from a 4-byte aligned address.
-    const bool s_is_row = wave < T::BM / 64;
-    __amdgpu_buffer_rsrc_t s_rsrc;
-    uint32_t s_lane;
-    const int kt0 = k0 / T::BK;
-    {
-        // (relative to the tile's first table row; rows past M repeat the last one, columns past N the last block)
-        const int kblocks = (p.K + T::BK - 1) / T::BK;
-        const int ra = m0 / p.bm, ra_last = (p.M - 1) / p.bm, rb = n0 / p.bn, rb_last = (p.N - 1) / p.bn;
-        const __amdgpu_buffer_rsrc_t sa = resource(p.sa + (size_t)ra * (size_t)p.ld_sa, ((long)(ra_last - ra) * p.ld_sa + kblocks) * 4);
-        const __amdgpu_buffer_rsrc_t sb = resource(p.sb + (size_t)rb * (size_t)p.ld_sb, ((long)(rb_last - rb) * p.ld_sb + kblocks) * 4);
-        s_rsrc = s_is_row ? sa : sb;
-        const int row = min(m0 + (s_is_row ? wave : 0) * 64 + lane, p.M - 1) / p.bm - ra;
-        const int blk = min(n0 + lane * 32, p.N - 1) / p.bn - rb;
-        s_lane = s_is_row ? (uint32_t)row * (uint32_t)p.ld_sa * 4u : lane < T::BN / 32 ? (uint32_t)blk * (uint32_t)p.ld_sb * 4u : OUT;
-    }
     // the four scales of tile `tile`'s group: from 4 (tile / 4), or the last four of the table row
-    const int s_end = (p.K + T::BK - 1) / T::BK - kt0 - 4;
     auto s_first = [&](int tile) __attribute__((always_inline)) { return min(tile & ~3, s_end); };
     // (not due: a piece of zeros into a place nobody reads, so that every tile issues the same number of pieces)
     auto dma_s = [&](int tile, bool due) __attribute__((always_inline)) {
@@ -406,56 +441,53 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(due ? s_rsrc : null_rsrc, lds_at(at), 16, s_lane, (uint32_t)(kt0 + s_first(tile)) * 4u, 0, 0);
     };
 
-    // this lane's two 16-byte chunks of row fr of a 16-row block (swizzled position inside the 128-byte row)
+    // This lane's two 16-byte chunks of row fr of a 16-row block (swizzled position inside the 128-byte row): LDS addresses of the
+    // wave's first row block and first column block, in the slot that is read next (they change slots by an exclusive or).
     const int f_lo = fr * 128 + (((2 * fq) ^ f8_a_swz(fr)) << 4), f_hi = fr * 128 + (((2 * fq + 1) ^ f8_a_swz(fr)) << 4);
-    i8v_t af[2], bf[2][NT]; // fragments of row blocks mt, mt + 1; weights of tiles t, t + 1 (by tile parity)
-    auto read_frag = [&](const uint8_t* block) __attribute__((always_inline)) { return f8f8_frag(*(const u4_t*)(block + f_lo), *(const u4_t*)(block + f_hi)); };
-    auto read_a = [&](int slot, int mt) __attribute__((always_inline)) { return read_frag(lds + slot * T::SLOT + (wr * MT + mt) * 2048); };
-    auto read_b = [&](int slot, int nt) __attribute__((always_inline)) { return read_frag(lds + slot * T::SLOT + T::A_TILE + (wc * NT + nt) * 2048); };
-    auto group0 = [&](int tile, bool s_due, int slot) __attribute__((always_inline)) {
-        const __amdgpu_buffer_rsrc_t ra = tile < ntiles ? a_rsrc : null_rsrc, rb = tile < ntiles ? b_rsrc : null_rsrc;
-        dma_s(tile, s_due && tile < ntiles);
-#pragma unroll
-        for(int i = 0; i < T::A_DMA; ++i)
-            dma_a(ra, slot, 0, i, tile == ntiles - 1);
-#pragma unroll
-        for(int i = 0; i < T::B_DMA; ++i)
-            dma_b(rb, slot, i, tile == ntiles - 1);
+    static_assert((T::SLOT & (T::SLOT - 1)) == 0, "slots change by an exclusive or");
+    uint32_t a_lo, a_hi, b_lo, b_hi;
+    i8v_t af[WIN], bf[NT]; // fragments of row blocks mt .. mt + LEAD; weights of the tile
+    auto read_frag = [&](uint32_t lo, uint32_t hi, int block) __attribute__((always_inline)) {
+        return f8f8_frag(*(const u4_t*)(lds + lo + block * 2048), *(const u4_t*)(lds + hi + block * 2048));
     };
-    auto group1 = [&](int tile, int slot) __attribute__((always_inline)) {
+    // pieces [first, last) of a tile's group 0 (scales, first half of A, B) and group 1 (second half of A)
+    auto group0 = [&](int tile, bool s_due, int slot, int first, int last) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t ra = tile < ntiles ? a_rsrc : null_rsrc, rb = tile < ntiles ? b_rsrc : null_rsrc;
+#pragma unroll
+        for(int i = first; i < last; ++i)
+            if(i == 0)
+                dma_s(tile, s_due && tile < ntiles);
+            else if(i <= T::A_DMA)
+                dma_a(ra, slot, 0, i - 1, tile == ntiles - 1);
+            else
+                dma_b(rb, slot, i - 1 - T::A_DMA, tile == ntiles - 1);
+    };
+    auto group1 = [&](int tile, int slot, int first, int last) __attribute__((always_inline)) {
         const __amdgpu_buffer_rsrc_t ra = tile < ntiles ? a_rsrc : null_rsrc;
 #pragma unroll
-        for(int i = 0; i < T::A_DMA; ++i)
+        for(int i = first; i < last; ++i)
             dma_a(ra, slot, 1, i, tile == ntiles - 1);
     };
     constexpr int G0 = 1 + T::A_DMA + T::B_DMA, G1 = T::A_DMA;
 
-    group0(0, true, 0);
-    __builtin_amdgcn_sched_barrier(0); // (issue order is part of the vmcnt arithmetic)
-    group1(0, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    group0(1, false, 1);
-    __builtin_amdgcn_sched_barrier(0);
-    group1(1, 1);
-    __builtin_amdgcn_sched_barrier(0);
-    clear_acc();
-    wait_vmcnt<G0 + 2 * G1>(); // group (0, 0) done
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for(int nt = 0; nt < NT; ++nt)
-        bf[0][nt] = read_b(0, nt);
-    af[0] = read_a(0, 0);
-    __builtin_amdgcn_sched_barrier(0);
+    auto prologue = [&]() __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_barrier(0); // (issue order is part of the vmcnt arithmetic)
+        group0(0, true, 0, 0, G0);
+        __builtin_amdgcn_sched_barrier(0);
+        group1(0, 0, 0, G1);
+        __builtin_amdgcn_sched_barrier(0);
+        group0(1, false, 1, 0, G0);
+        __builtin_amdgcn_sched_barrier(0);
+        group1(1, 1, 0, G1);
+        __builtin_amdgcn_sched_barrier(0);
+    };
 
+    f4_t acc[NT][MT];
     f4_t pend[NT];        // block sums not yet folded in: of the previous row block
     float s_fold[NT / 2]; // and their factors, per 32 columns
-#pragma unroll
-    for(int nt = 0; nt < NT; ++nt)
-        pend[nt] = f4_t{0.f, 0.f, 0.f, 0.f}, s_fold[nt / 2] = 0.f;
-    int t = 0;
-    auto tile_body = [&](auto parity) __attribute__((always_inline)) {
-        constexpr int slot = decltype(parity)::value;
+    int t;
+    auto tile_body = [&]() __attribute__((always_inline)) {
+        const int slot    = t & 1;
         const uint8_t* sp = lds + T::S_OFF + ((t >> 2) & 1) * T::S_SLOT + (t - s_first(t)) * 4;
         const float* row_s = (const float*)(sp + (wr * MT * 16 + fr) * 16); // row 16 mt + fr at [64 mt]
         float sb[NT / 2];
@@ -466,79 +498,146 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
 
         auto row_block = [&](auto mt_c) __attribute__((always_inline)) {
             constexpr int mt = decltype(mt_c)::value, prev = (mt + MT - 1) % MT;
-            if constexpr(mt == MH - 1 || mt == MT - 1)
+            if constexpr(mt == MH - LEAD || mt == MT - LEAD)
             {
-                if constexpr(mt == MH - 1)
-                    wait_vmcnt<G1>();
+                wait_vmcnt<G0 + G1>();
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if constexpr(mt + 1 < MT)
-                af[(mt + 1) & 1] = read_a(slot, mt + 1);
-            else
-                af[0] = read_a(slot ^ 1, 0);
+            if constexpr(mt == MT - LEAD)
+                a_lo ^= T::SLOT, a_hi ^= T::SLOT; // (from here on the next tile's)
+            af[(mt + LEAD) % WIN] = read_frag(a_lo, a_hi, (mt + LEAD) % MT);
             float s_now[NT / 2];
 #pragma unroll
             for(int h = 0; h < NT / 2; ++h)
                 s_now[h] = s_row * sb[h];
             if constexpr(mt + 1 < MT)
                 s_row = row_s[64 * (mt + 1)];
-            constexpr int BPER = mt >= MH - 1 && mt < MT - 1 ? NT / MH : 0;
-#pragma unroll
-            for(int i = 0; i < BPER; ++i)
-                bf[slot ^ 1][(mt - (MH - 1)) * BPER + i] = read_b(slot ^ 1, (mt - (MH - 1)) * BPER + i);
-            if constexpr(mt == MH - 1)
-                group0(t + 2, (t & 3) == 2, slot); // (scale slot: of tiles t - 6 .. t - 3)
-            if constexpr(mt == MT - 1)
-                group1(t + 2, slot);
+            // (a piece or two per row block: issued at once they hold the wave up behind everybody else's)
+            if constexpr(mt >= MH - LEAD && mt < MT - LEAD)
+            {
+                constexpr int PER = (G0 + MH - 1) / MH, i = (mt - (MH - LEAD)) * PER;
+                group0(t + 2, (t & 3) == 2, slot, i, i + PER < G0 ? i + PER : G0); // (scale slot: of tiles t - 6 .. t - 3)
+            }
+            if constexpr(mt >= MT - LEAD)
+            {
+                constexpr int PER = (G1 + LEAD - 1) / LEAD, i = (mt - (MT - LEAD)) * PER;
+                group1(t + 2, slot, i, i + PER < G1 ? i + PER : G1);
+            }
             const f4_t zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for(int nt = 0; nt < NT; ++nt)
             {
                 const float f  = s_fold[nt / 2];
                 acc[nt][prev] = __builtin_elementwise_fma(pend[nt], f4_t{f, f, f, f}, acc[nt][prev]);
-                pend[nt]      = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[slot][nt], af[mt & 1], zero, 0, 0, 0, 0, 0, 0);
+                pend[nt]      = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[nt], af[mt % WIN], zero, 0, 0, 0, 0, 0, 0);
+                if constexpr(mt == MT - 1)
+                    bf[nt] = read_frag(b_lo, b_hi, nt);
             }
 #pragma unroll
             for(int h = 0; h < NT / 2; ++h)
                 s_fold[h] = s_now[h];
+            // order: a fold and an MFMA in turn, the fragment reads behind the first MFMA (as early as they can hide behind one)
+            __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, mt == MT - 1 ? 5 : 3, 0);
+            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
 #pragma unroll
-            for(int nt = 0; nt < NT; ++nt)
+            for(int nt = 1; nt < NT; ++nt)
             {
                 __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1 + BPER, 0);
+                if constexpr(mt == MT - 1)
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
         };
         for_each_constant(row_block, std::make_integer_sequence<int, MT>{});
-        ++t;
+        b_lo ^= T::SLOT, b_hi ^= T::SLOT;
     };
-    for(;;)
-    {
-        tile_body(integral_constant<int, 0>{});
-        if(t == ntiles)
-            break;
-        tile_body(integral_constant<int, 1>{});
-        if(t == ntiles)
-            break;
-    }
+    auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for(int nt = 0; nt < NT; ++nt)
+        for(int nt = 0; nt < NT; ++nt)
+        {
+            pend[nt] = f4_t{0.f, 0.f, 0.f, 0.f}, s_fold[nt / 2] = 0.f;
+#pragma unroll
+            for(int mt = 0; mt < MT; ++mt)
+                acc[nt][mt] = f4_t{0.f, 0.f, 0.f, 0.f};
+        }
+    };
+    // the K loop of the unit whose first loads are in flight (ntiles > 0); every wave is done with the slots at its end
+    auto multiply = [&]() __attribute__((always_inline)) {
+        wait_vmcnt<G0 + 2 * G1>(); // group (0, 0) done (the stores of the tile before are younger: they only add to the wait)
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        a_lo = f_lo + wr * (MT * 2048), a_hi = f_hi + wr * (MT * 2048);
+        b_lo = f_lo + T::A_TILE + wc * (NT * 2048), b_hi = f_hi + T::A_TILE + wc * (NT * 2048);
+#pragma unroll
+        for(int nt = 0; nt < NT; ++nt)
+            bf[nt] = read_frag(b_lo, b_hi, nt);
+#pragma unroll
+        for(int i = 0; i < LEAD; ++i)
+            af[i] = read_frag(a_lo, a_hi, i);
+        b_lo ^= T::SLOT, b_hi ^= T::SLOT;
+        __builtin_amdgcn_sched_barrier(0);
+        t = 0;
+        do
+            tile_body();
+        while(++t < ntiles);
+#pragma unroll
+        for(int nt = 0; nt < NT; ++nt)
+        {
+            const float f   = s_fold[nt / 2];
+            acc[nt][MT - 1] = __builtin_elementwise_fma(pend[nt], f4_t{f, f, f, f}, acc[nt][MT - 1]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+    };
+
+    int unit = blockIdx.x;
+    set_unit(unit);
+    if constexpr(STREAM)
     {
-        const float f   = s_fold[nt / 2];
-        acc[nt][MT - 1] = __builtin_elementwise_fma(pend[nt], f4_t{f, f, f, f}, acc[nt][MT - 1]);
+        prologue();
+        for(;;)
+        {
+            clear();
+            multiply();
+            const int m = m0, n = n0;
+            unit += gridDim.x;
+            if(unit < units)
+            {
+                set_unit(unit);
+                prologue(); // (the next tile's first loads fly while this one leaves)
+            }
+            f8f8_epilogue_stream<T>(p, acc, lds, m, n, wave, lane);
+            if(unit >= units)
+                break;
+        }
+        wait_vmcnt<0>();
     }
-    wait_vmcnt<0>(); // (null-resource loads of tiles past the end still count)
-    __syncthreads(); // every wave is done with the slots before they become the C tile image
-    f8f8_epilogue<T>(p, acc, lds, m0, n0, wave, lane);
+    else
+    {
+        clear();
+        if(ntiles > 0)
+        {
+            prologue();
+            multiply();
+            wait_vmcnt<0>(); // (null-resource pieces of tiles past the end write zeros into the slots)
+            __syncthreads();
+        }
+        f8f8_epilogue_any<T>(p, acc, lds, m0, n0, z, wave, lane);
+    }
 }
 
-template <bool TAIL>
-__global__ __launch_bounds__(512, 2) void wq_gemm_f8f8_256(const F8F8Params p) { f8f8_tile_body<F8F8Tile<8, 4, 2, 4>, TAIL>(p); }
-template <bool TAIL>
-__global__ __launch_bounds__(256, 2) void wq_gemm_f8f8_128(const F8F8Params p) { f8f8_tile_body<F8F8Tile<4, 4, 2, 2>, TAIL>(p); }
+using F8F8Tile256 = F8F8Tile<8, 4, 2, 4, 3>;
+using F8F8Tile128 = F8F8Tile<4, 4, 2, 2, 1>;
+template <bool TAIL, bool STREAM>
+__global__ __launch_bounds__(512, 2) void wq_gemm_f8f8_256(const F8F8Params p) { f8f8_tile_body<F8F8Tile256, TAIL, STREAM>(p); }
+template <bool TAIL, bool STREAM>
+__global__ __launch_bounds__(256, 2) void wq_gemm_f8f8_128(const F8F8Params p) { f8f8_tile_body<F8F8Tile128, TAIL, STREAM>(p); }
 
 // Split-K: out[m, n] = epilogue(sum_z slab[z][m][n]), z ascending, for any N (ld_part is N rounded up to 4).
 __global__ __launch_bounds__(256) void wq_reduce_f8f8(const float* __restrict__ slabs, int k_batch, int ld_part, F8F8Params p)
@@ -551,7 +650,7 @@ __global__ __launch_bounds__(256) void wq_reduce_f8f8(const float* __restrict__ 
         f4_t s = *(const f4_t*)(slabs + (size_t)m * ld_part + n);
         for(int z = 1; z < k_batch; ++z)
             s += *(const f4_t*)(slabs + ((size_t)z * p.M + m) * (size_t)ld_part + n);
-        f8f8_store4(p, s, m, n);
+        f8f8_store4(p, s, m, n, 0);
     }
 }
 

@@ -1,5 +1,6 @@
 // Translation unit of the fp8 x fp8 kernels with block-wise scales (wq_gemm_f8f8.h).
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include <atomic>
 
 #include "wqgemm.h"
@@ -11,7 +12,7 @@ namespace {
 
 // more than 64 KiB of dynamic LDS must be opted into once per device
 template <class T, void (*kernel)(const F8F8Params)>
-int launch_tile(const F8F8Params& p, dim3 grid, hipStream_t s)
+int launch_tile(const F8F8Params& p, long grid, hipStream_t s)
 {
     static std::atomic<bool> opted_in[64];
     int dev = 0;
@@ -24,23 +25,36 @@ int launch_tile(const F8F8Params& p, dim3 grid, hipStream_t s)
         if(dev >= 0 && dev < 64)
             opted_in[dev] = true;
     }
-    hipLaunchKernelGGL(kernel, grid, dim3(T::THREADS), T::LDS_BYTES, s, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(T::THREADS), T::LDS_BYTES, s, p);
     return WQ_OK;
 }
 
 } // namespace
 
-int launch_f8f8(int kernel, const F8F8Params& p, int k_batch, hipStream_t s)
+int launch_f8f8(int kernel, const F8F8Params& p, hipStream_t s)
 {
-    const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)k_batch);
     const bool tail = (p.k_end - p.k_begin) % 128 != 0; // (slices between are whole K tiles)
+    const int kind  = p.epi.kind;
+    const bool stream = !p.partial && p.N % 8 == 0 && p.ldc % 8 == 0 && p.ldc <= 1 << 22 && (uintptr_t)p.c % 16 == 0 &&
+                        (kind == WQ_EPI_PASSTHROUGH || kind == WQ_EPI_FASTGELU || kind == WQ_EPI_CONVERT_BF16_RTN ||
+                         ((kind == WQ_EPI_ADD || kind == WQ_EPI_ADD_FASTGELU) && p.epi.ldd0 == 0));
+    // (streaming workgroups walk the tiles: one resident grid on the 256 CUs)
+    const long units = (long)p.tiles_m * p.tiles_n * p.slices;
     switch(kernel)
     {
     case F8F8_256:
-        return tail ? launch_tile<F8F8Tile<8, 4, 2, 4>, wq_gemm_f8f8_256<true>>(p, grid, s) : launch_tile<F8F8Tile<8, 4, 2, 4>, wq_gemm_f8f8_256<false>>(p, grid, s);
+        return stream ? tail ? launch_tile<F8F8Tile256, wq_gemm_f8f8_256<true, true>>(p, std::min(units, 256L), s)
+                             : launch_tile<F8F8Tile256, wq_gemm_f8f8_256<false, true>>(p, std::min(units, 256L), s)
+               : tail ? launch_tile<F8F8Tile256, wq_gemm_f8f8_256<true, false>>(p, units, s)
+                      : launch_tile<F8F8Tile256, wq_gemm_f8f8_256<false, false>>(p, units, s);
     case F8F8_128:
-        return tail ? launch_tile<F8F8Tile<4, 4, 2, 2>, wq_gemm_f8f8_128<true>>(p, grid, s) : launch_tile<F8F8Tile<4, 4, 2, 2>, wq_gemm_f8f8_128<false>>(p, grid, s);
-    default: hipLaunchKernelGGL(wq_gemm_f8f8_any, grid, dim3(256), 0, s, p); return WQ_OK;
+        return stream ? tail ? launch_tile<F8F8Tile128, wq_gemm_f8f8_128<true, true>>(p, std::min(units, 512L), s)
+                             : launch_tile<F8F8Tile128, wq_gemm_f8f8_128<false, true>>(p, std::min(units, 512L), s)
+               : tail ? launch_tile<F8F8Tile128, wq_gemm_f8f8_128<true, false>>(p, units, s)
+                      : launch_tile<F8F8Tile128, wq_gemm_f8f8_128<false, false>>(p, units, s);
+    default:
+        hipLaunchKernelGGL(wq_gemm_f8f8_any, dim3((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.slices), dim3(256), 0, s, p);
+        return WQ_OK;
     }
 }
 

@@ -988,6 +988,7 @@ int launch_main(const wqgemm_problem* p, const Plan& plan, void* workspace, hipS
         wq::F8F8Params gp = f8f8_params(p);
         gp.k_begin = plan.k_begin, gp.k_end = plan.k_end, gp.k_per_z = plan.k_per_z;
         gp.partial = plan.partial ? 1 : 0;
+        gp.slices  = plan.k_batch;
         gp.c       = out;
         if(plan.partial && !plan.to_c)
             gp.ldc = f8f8_ld_part(p);
@@ -1002,7 +1003,7 @@ int launch_main(const wqgemm_problem* p, const Plan& plan, void* workspace, hipS
             if(!best || cost <= best)
                 best = cost, gp.group_m = g;
         }
-        if(wq::launch_f8f8(plan.f8f8, gp, plan.k_batch, s) != WQ_OK)
+        if(wq::launch_f8f8(plan.f8f8, gp, s) != WQ_OK)
             return fail(WQ_ERR_HIP, "fp8 x fp8 kernel launch failed: %s", hipGetErrorString(hipGetLastError()));
     }
     else

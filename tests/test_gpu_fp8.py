@@ -110,7 +110,8 @@ def check_exact(got, P):
 
 SIZES = [(1, 128, 128), (1, 4096, 4096), (2, 1, 1), (5, 33, 17), (1, 257, 1001), (15, 64, 2048), (16, 256, 4112), (17, 300, 640), (33, 100, 384),
          (64, 1024, 1024), (65, 130, 272), (96, 512, 2816), (127, 129, 1100), (128, 128, 128), (129, 256, 256), (200, 1000, 528), (256, 256, 144),
-         (300, 700, 1040), (513, 384, 512), (777, 520, 400), (1024, 1024, 384), (2048, 2304, 256)]
+         (300, 700, 1040), (513, 384, 512), (777, 520, 400), (1024, 1024, 384), (2048, 2304, 256),
+         (4352, 4608, 512), (4300, 4616, 656)]  # (the last two: more tiles than resident workgroups)
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
