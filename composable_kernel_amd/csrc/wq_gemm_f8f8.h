@@ -639,6 +639,259 @@ __global__ __launch_bounds__(512, 2) void wq_gemm_f8f8_256(const F8F8Params p) {
 template <bool TAIL, bool STREAM>
 __global__ __launch_bounds__(256, 2) void wq_gemm_f8f8_128(const F8F8Params p) { f8f8_tile_body<F8F8Tile128, TAIL, STREAM>(p); }
 
+// ---------------------------------------------------------------------------------------------
+// Few rows (M <= 16 MT): one pass over the weights, bound by their stream.  A workgroup owns 16 NB columns; its waves deal the K
+// tiles among themselves (tile i WAVES + wave: the workgroup reads runs of WAVES cache lines of every column) and add their sums
+// through LDS at the end, in the order of the waves: no second kernel, no workspace.  Rows past M and columns past N lie outside
+// the resources and read as zeros without memory accesses, and so does what lies past the end of the last K tile (K a multiple of
+// 16).  Two forms:
+//   * _direct: operands straight to the registers of the MFMA, P tiles at a time.  The vector cache takes such fragment-shaped
+//     loads at one access of 16 bytes per lane: 16 bytes a cycle and CU, 8.6 TB/s on the chip, more than HBM delivers, but
+//     activations of 16 rows double the accesses.  Least latency: 4096 x 4096 at M = 1 6.5 us (7.2 through LDS), 28672 x 8192
+//     37.9 us = 6.2 TB/s (50.7);
+//   * through LDS: LDS-DMA takes 64 bytes an access; every wave fills a ring of its own, D tiles ahead, so there is no barrier in
+//     the loop.  4096 x 4096 at M = 16 8.0 us (direct 8.4), 4096 x 11008 15.1 (17.0), 28672 x 8192, 64 columns a
+//     workgroup, 45.7 (69.0).
+// ---------------------------------------------------------------------------------------------
+template <int MT, int NB, int WAVES, int P>
+__global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny_direct(const F8F8Params p)
+{
+    __shared__ __attribute__((aligned(16))) f4_t sums[WAVES][MT * NB][64];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int fr = lane & 15, fq = lane >> 4;
+    const int n0 = blockIdx.x * (NB * 16), z = blockIdx.y;
+    const int k0 = p.k_begin + z * p.k_per_z, k1 = min(p.k_end, k0 + p.k_per_z);
+    const int ntiles = (k1 - k0 + 127) >> 7; // (empty slices: <= 0)
+    constexpr uint32_t OUT = 0x80000000u;
+
+    const long a_bytes = (long)(p.M - 1) * p.lda + p.K, b_bytes = (long)(p.N - n0 - 1) * p.ldb + p.K;
+    const __amdgpu_buffer_rsrc_t a_rsrc =
+        __builtin_amdgcn_make_buffer_rsrc((void*)p.a, 0, (int)(a_bytes < 0x7FFFFFFF ? a_bytes : 0x7FFFFFFF), 0x00020000);
+    const __amdgpu_buffer_rsrc_t b_rsrc =
+        __builtin_amdgcn_make_buffer_rsrc((void*)(p.b + (size_t)n0 * (size_t)p.ldb), 0, (int)(b_bytes < 0x7FFFFFFF ? b_bytes : 0x7FFFFFFF), 0x00020000);
+    const uint32_t a_lane = (uint32_t)fr * (uint32_t)p.lda + fq * 32, b_lane = (uint32_t)fr * (uint32_t)p.ldb + fq * 32;
+    const int k_last      = k1 - k0 - (ntiles - 1) * 128;
+    const uint32_t bad_lo = fq * 32 < k_last ? 0u : OUT, bad_hi = fq * 32 + 16 < k_last ? 0u : OUT;
+    const int kt0 = k0 >> 7;
+    const float* sa[MT]; // (rows past M repeat the last one: their results are not stored)
+    const float* sb[NB];
+#pragma unroll
+    for(int mt = 0; mt < MT; ++mt)
+        sa[mt] = p.sa + (size_t)(min(mt * 16 + fr, p.M - 1) / p.bm) * (size_t)p.ld_sa + kt0;
+#pragma unroll
+    for(int nb = 0; nb < NB; ++nb)
+        sb[nb] = p.sb + (size_t)(min(n0 + nb * 16, p.N - 1) / p.bn) * (size_t)p.ld_sb + kt0;
+
+    f4_t acc[MT][NB];
+#pragma unroll
+    for(int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for(int nb = 0; nb < NB; ++nb)
+            acc[mt][nb] = f4_t{0.f, 0.f, 0.f, 0.f};
+
+    auto load = [&](const __amdgpu_buffer_rsrc_t& rsrc, uint32_t off, uint32_t row_block, int tile) __attribute__((always_inline)) {
+        const bool last     = tile == ntiles - 1;
+        const uint32_t soff = row_block + k0 + tile * 128;
+        const u4_t lo = __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, last ? off | bad_lo : off, soff, 0));
+        const u4_t hi = __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, last ? off | bad_hi : off, soff + 16, 0));
+        return f8f8_frag(lo, hi);
+    };
+    auto step = [&](int first, int tiles) __attribute__((always_inline)) {
+        i8v_t w[P][NB], a[P][MT];
+        float ra[P][MT];
+#pragma unroll
+        for(int i = 0; i < P; ++i)
+            if(i < tiles)
+            {
+                const int tile = first + i * WAVES;
+#pragma unroll
+                for(int nb = 0; nb < NB; ++nb)
+                    w[i][nb] = load(b_rsrc, b_lane, (uint32_t)(nb * 16) * (uint32_t)p.ldb, tile);
+#pragma unroll
+                for(int mt = 0; mt < MT; ++mt)
+                {
+                    a[i][mt]  = load(a_rsrc, a_lane, (uint32_t)(mt * 16) * (uint32_t)p.lda, tile);
+                    ra[i][mt] = sa[mt][tile];
+                }
+            }
+#pragma unroll
+        for(int i = 0; i < P; ++i)
+            if(i < tiles)
+            {
+                const int tile = first + i * WAVES;
+#pragma unroll
+                for(int nb = 0; nb < NB; ++nb)
+                {
+                    const float cs = sb[nb][tile] * p.fnuz;
+#pragma unroll
+                    for(int mt = 0; mt < MT; ++mt)
+                    {
+                        const float s   = ra[i][mt] * cs;
+                        const f4_t zero = {0.f, 0.f, 0.f, 0.f};
+                        const f4_t sum  = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i][nb], a[i][mt], zero, 0, 0, 0, 0, 0, 0);
+                        acc[mt][nb]     = __builtin_elementwise_fma(sum, f4_t{s, s, s, s}, acc[mt][nb]);
+                    }
+                }
+            }
+    };
+    int tile = wave;
+    for(; tile + (P - 1) * WAVES < ntiles; tile += P * WAVES)
+        step(tile, P);
+    for(; tile < ntiles; tile += WAVES)
+        step(tile, 1);
+
+#pragma unroll
+    for(int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for(int nb = 0; nb < NB; ++nb)
+            sums[wave][mt * NB + nb][lane] = acc[mt][nb];
+    __syncthreads();
+    for(int u = threadIdx.x; u < MT * NB * 64; u += WAVES * 64)
+    {
+        const int block = u >> 6, l = u & 63;
+        f4_t v = sums[0][block][l];
+#pragma unroll
+        for(int w = 1; w < WAVES; ++w)
+            v += sums[w][block][l];
+        f8f8_store4(p, v, block / NB * 16 + (l & 15), n0 + block % NB * 16 + (l >> 4) * 4, z);
+    }
+}
+
+// One wave's ring: D tiles of 16 NB columns' weights and 16 MT rows of activations, in LDS-DMA pieces of 8 rows.  OPS: what a tile
+// adds to vmcnt, its pieces and its row scales.
+template <int MT, int NB, int WAVES, int D>
+struct F8F8Skinny
+{
+    static constexpr int THREADS = WAVES * 64, SLOT = (NB + MT) * 2048, LDS_BYTES = WAVES * D * SLOT, OPS = 2 * (NB + MT) + MT;
+    static_assert(LDS_BYTES >= WAVES * MT * NB * 1024 && LDS_BYTES <= 160 * 1024, "the sums reuse the ring");
+};
+
+template <int MT, int NB, int WAVES, int D>
+__global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny(const F8F8Params p)
+{
+    using T = F8F8Skinny<MT, NB, WAVES, D>;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int fr = lane & 15, fq = lane >> 4;
+    const int n0 = blockIdx.x * (NB * 16), z = blockIdx.y;
+    const int k0 = p.k_begin + z * p.k_per_z, k1 = min(p.k_end, k0 + p.k_per_z);
+    const int ntiles = (k1 - k0 + 127) >> 7; // (empty slices: <= 0)
+    const int mine   = ntiles > wave ? (ntiles - wave + WAVES - 1) / WAVES : 0;
+    constexpr uint32_t OUT = 0x80000000u;
+
+    auto resource = [](const void* base, long bytes) __attribute__((always_inline)) {
+        return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF), 0x00020000);
+    };
+    const __amdgpu_buffer_rsrc_t a_rsrc    = resource(p.a, (long)(p.M - 1) * p.lda + p.K);
+    const __amdgpu_buffer_rsrc_t b_rsrc    = resource(p.b + (size_t)n0 * (size_t)p.ldb, (long)(p.N - n0 - 1) * p.ldb + p.K);
+    const __amdgpu_buffer_rsrc_t null_rsrc = resource(p.a, 0);
+    const int chunk       = ((lane & 7) ^ f8_a_swz(lane >> 3)) << 4;
+    const uint32_t a_lane = (uint32_t)(lane >> 3) * (uint32_t)p.lda + chunk, b_lane = (uint32_t)(lane >> 3) * (uint32_t)p.ldb + chunk;
+    const bool past       = chunk >= k1 - k0 - (ntiles - 1) * 128;
+    const int kt0 = k0 >> 7;
+    const float* sa[MT]; // (rows past M repeat the last one: their results are not stored)
+    const float* sb[NB];
+#pragma unroll
+    for(int mt = 0; mt < MT; ++mt)
+        sa[mt] = p.sa + (size_t)(min(mt * 16 + fr, p.M - 1) / p.bm) * (size_t)p.ld_sa + kt0;
+#pragma unroll
+    for(int nb = 0; nb < NB; ++nb)
+        sb[nb] = p.sb + (size_t)(min(n0 + nb * 16, p.N - 1) / p.bn) * (size_t)p.ld_sb + kt0;
+
+    f4_t acc[MT][NB];
+#pragma unroll
+    for(int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for(int nb = 0; nb < NB; ++nb)
+            acc[mt][nb] = f4_t{0.f, 0.f, 0.f, 0.f};
+    float ra[D][MT];
+    uint8_t* ring = lds + wave * (D * T::SLOT);
+    // (tiles past the wave's last one: scales of its last, pieces of zeros without a memory access)
+    auto fetch = [&](int i, int j) __attribute__((always_inline)) {
+        const int tile = wave + j * WAVES, known = min(tile, max(ntiles - 1, 0));
+#pragma unroll
+        for(int mt = 0; mt < MT; ++mt)
+            ra[i][mt] = sa[mt][known];
+        __builtin_amdgcn_sched_barrier(0); // (issue order is part of the vmcnt arithmetic)
+        const bool last = tile == ntiles - 1, there = tile < ntiles;
+        const __amdgpu_buffer_rsrc_t wr = there ? b_rsrc : null_rsrc, ar = there ? a_rsrc : null_rsrc;
+        const uint32_t w_off = last && past ? OUT : b_lane, x_off = last && past ? OUT : a_lane, soff = (uint32_t)(k0 + tile * 128);
+#pragma unroll
+        for(int h = 0; h < 2 * NB; ++h)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void*)(ring + i * T::SLOT + h * 1024), 16, w_off,
+                                                     soff + (uint32_t)(h * 8) * (uint32_t)p.ldb, 0, 0);
+#pragma unroll
+        for(int h = 0; h < 2 * MT; ++h)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ar, (__attribute__((address_space(3))) void*)(ring + i * T::SLOT + (2 * NB + h) * 1024), 16,
+                                                     x_off, soff + (uint32_t)(h * 8) * (uint32_t)p.lda, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const int f_lo = fr * 128 + (((2 * fq) ^ f8_a_swz(fr)) << 4), f_hi = fr * 128 + (((2 * fq + 1) ^ f8_a_swz(fr)) << 4);
+
+#pragma unroll
+    for(int i = 0; i < D; ++i)
+        fetch(i, i);
+    for(int j = 0; j < mine; j += D)
+    {
+#pragma unroll
+        for(int i = 0; i < D; ++i)
+            if(j + i < mine)
+            {
+                const int tile = wave + (j + i) * WAVES;
+                wait_vmcnt<(D - 1) * T::OPS>();
+                __builtin_amdgcn_sched_barrier(0);
+                i8v_t w[NB], a[MT];
+                float s[MT];
+                const uint8_t* st = ring + i * T::SLOT;
+#pragma unroll
+                for(int nb = 0; nb < NB; ++nb)
+                    w[nb] = f8f8_frag(*(const u4_t*)(st + nb * 2048 + f_lo), *(const u4_t*)(st + nb * 2048 + f_hi));
+#pragma unroll
+                for(int mt = 0; mt < MT; ++mt)
+                {
+                    a[mt] = f8f8_frag(*(const u4_t*)(st + (NB + mt) * 2048 + f_lo), *(const u4_t*)(st + (NB + mt) * 2048 + f_hi));
+                    s[mt] = ra[i][mt];
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // read: the slot may be filled again
+                __builtin_amdgcn_sched_barrier(0);
+                fetch(i, j + i + D);
+#pragma unroll
+                for(int nb = 0; nb < NB; ++nb)
+                {
+                    const float cs = sb[nb][tile] * p.fnuz;
+#pragma unroll
+                    for(int mt = 0; mt < MT; ++mt)
+                    {
+                        const float f   = s[mt] * cs;
+                        const f4_t zero = {0.f, 0.f, 0.f, 0.f};
+                        const f4_t sum  = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[nb], a[mt], zero, 0, 0, 0, 0, 0, 0);
+                        acc[mt][nb]     = __builtin_elementwise_fma(sum, f4_t{f, f, f, f}, acc[mt][nb]);
+                    }
+                }
+            }
+    }
+    wait_vmcnt<0>(); // (pieces of zeros still write)
+    __syncthreads();
+    f4_t* sums = (f4_t*)lds;
+#pragma unroll
+    for(int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for(int nb = 0; nb < NB; ++nb)
+            sums[(wave * (MT * NB) + mt * NB + nb) * 64 + lane] = acc[mt][nb];
+    __syncthreads();
+    for(int u = threadIdx.x; u < MT * NB * 64; u += WAVES * 64)
+    {
+        const int block = u >> 6, l = u & 63;
+        f4_t v = sums[u];
+#pragma unroll
+        for(int w = 1; w < WAVES; ++w)
+            v += sums[w * (MT * NB * 64) + u];
+        f8f8_store4(p, v, block / NB * 16 + (l & 15), n0 + block % NB * 16 + (l >> 4) * 4, z);
+    }
+}
+
 // Split-K: out[m, n] = epilogue(sum_z slab[z][m][n]), z ascending, for any N (ld_part is N rounded up to 4).
 __global__ __launch_bounds__(256) void wq_reduce_f8f8(const float* __restrict__ slabs, int k_batch, int ld_part, F8F8Params p)
 {

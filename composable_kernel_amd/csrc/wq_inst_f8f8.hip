@@ -12,7 +12,7 @@ namespace {
 
 // more than 64 KiB of dynamic LDS must be opted into once per device
 template <class T, void (*kernel)(const F8F8Params)>
-int launch_tile(const F8F8Params& p, long grid, hipStream_t s)
+int launch_tile(const F8F8Params& p, dim3 grid, hipStream_t s)
 {
     static std::atomic<bool> opted_in[64];
     int dev = 0;
@@ -25,7 +25,7 @@ int launch_tile(const F8F8Params& p, long grid, hipStream_t s)
         if(dev >= 0 && dev < 64)
             opted_in[dev] = true;
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(T::THREADS), T::LDS_BYTES, s, p);
+    hipLaunchKernelGGL(kernel, grid, dim3(T::THREADS), T::LDS_BYTES, s, p);
     return WQ_OK;
 }
 
@@ -40,18 +40,23 @@ int launch_f8f8(int kernel, const F8F8Params& p, hipStream_t s)
                          ((kind == WQ_EPI_ADD || kind == WQ_EPI_ADD_FASTGELU) && p.epi.ldd0 == 0));
     // (streaming workgroups walk the tiles: one resident grid on the 256 CUs)
     const long units = (long)p.tiles_m * p.tiles_n * p.slices;
+    const dim3 strips((unsigned)p.tiles_n, (unsigned)p.slices); // small-M kernels: strips of columns
     switch(kernel)
     {
     case F8F8_256:
-        return stream ? tail ? launch_tile<F8F8Tile256, wq_gemm_f8f8_256<true, true>>(p, std::min(units, 256L), s)
-                             : launch_tile<F8F8Tile256, wq_gemm_f8f8_256<false, true>>(p, std::min(units, 256L), s)
-               : tail ? launch_tile<F8F8Tile256, wq_gemm_f8f8_256<true, false>>(p, units, s)
-                      : launch_tile<F8F8Tile256, wq_gemm_f8f8_256<false, false>>(p, units, s);
+        return stream ? tail ? launch_tile<F8F8Tile256, wq_gemm_f8f8_256<true, true>>(p, dim3((unsigned)std::min(units, 256L)), s)
+                             : launch_tile<F8F8Tile256, wq_gemm_f8f8_256<false, true>>(p, dim3((unsigned)std::min(units, 256L)), s)
+               : tail ? launch_tile<F8F8Tile256, wq_gemm_f8f8_256<true, false>>(p, dim3((unsigned)units), s)
+                      : launch_tile<F8F8Tile256, wq_gemm_f8f8_256<false, false>>(p, dim3((unsigned)units), s);
     case F8F8_128:
-        return stream ? tail ? launch_tile<F8F8Tile128, wq_gemm_f8f8_128<true, true>>(p, std::min(units, 512L), s)
-                             : launch_tile<F8F8Tile128, wq_gemm_f8f8_128<false, true>>(p, std::min(units, 512L), s)
-               : tail ? launch_tile<F8F8Tile128, wq_gemm_f8f8_128<true, false>>(p, units, s)
-                      : launch_tile<F8F8Tile128, wq_gemm_f8f8_128<false, false>>(p, units, s);
+        return stream ? tail ? launch_tile<F8F8Tile128, wq_gemm_f8f8_128<true, true>>(p, dim3((unsigned)std::min(units, 512L)), s)
+                             : launch_tile<F8F8Tile128, wq_gemm_f8f8_128<false, true>>(p, dim3((unsigned)std::min(units, 512L)), s)
+               : tail ? launch_tile<F8F8Tile128, wq_gemm_f8f8_128<true, false>>(p, dim3((unsigned)units), s)
+                      : launch_tile<F8F8Tile128, wq_gemm_f8f8_128<false, false>>(p, dim3((unsigned)units), s);
+    case F8F8_SKINNY_DIRECT: hipLaunchKernelGGL((wq_gemm_f8f8_skinny_direct<1, 1, 16, 2>), strips, dim3(1024), 0, s, p); return WQ_OK;
+    case F8F8_SKINNY_16: return launch_tile<F8F8Skinny<1, 1, 8, 2>, wq_gemm_f8f8_skinny<1, 1, 8, 2>>(p, strips, s);
+    case F8F8_SKINNY_16X64: return launch_tile<F8F8Skinny<1, 4, 4, 2>, wq_gemm_f8f8_skinny<1, 4, 4, 2>>(p, strips, s);
+    case F8F8_SKINNY_32: return launch_tile<F8F8Skinny<2, 1, 8, 1>, wq_gemm_f8f8_skinny<2, 1, 8, 1>>(p, strips, s);
     default:
         hipLaunchKernelGGL(wq_gemm_f8f8_any, dim3((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.slices), dim3(256), 0, s, p);
         return WQ_OK;

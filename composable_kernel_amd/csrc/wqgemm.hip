@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -158,7 +159,7 @@ int check_block_scales(const wqgemm_problem* p)
 }
 
 // fp8 weights: called by make_plan once sizes, layouts and the K slice are validated.
-int make_plan_f8f8(const wqgemm_problem* p, Plan& plan)
+int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
 {
     const bool slice = plan.to_c;
     if(!is_f8(p->a_dtype) || !has_block_scales(p))
@@ -194,16 +195,52 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan)
         return fail(WQ_ERR_UNSUPPORTED, "too many tiles for one launch");
     // The kernels that load 16 bytes at a time: aligned rows, slices that end on whole pieces, distances inside a tile in 32 bits.
     const int ld_sa = std::max(p->ld_a_scale, (p->K - 1) / 128 + 1), ld_sb = std::max(p->ld_b_scale, (p->K - 1) / 128 + 1);
-    const bool wide = p->lda % 16 == 0 && p->ldb % 16 == 0 && (uintptr_t)p->a % 16 == 0 && (uintptr_t)p->b % 16 == 0 &&
-                      plan.k_end % 16 == 0 && p->lda <= 1 << 22 && p->ldb <= 1 << 22 && ld_sa <= 1 << 20 && ld_sb <= 1 << 20 && p->K > 384;
-    const long tiles256 = (long)((p->M + 255) / 256) * ((p->N + 255) / 256);
-    plan.f8f8           = !wide ? wq::F8F8_ANY : tiles256 * plan.k_batch >= 128 ? wq::F8F8_256 : wq::F8F8_128;
-    if(wide && (p->flags & WQ_FLAG_TILE_256))
-        plan.f8f8 = wq::F8F8_256;
-    else if(wide && (p->flags & WQ_FLAG_TILE_128))
-        plan.f8f8 = wq::F8F8_128;
-    else if(p->flags & (WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256))
+    const bool rows16 = p->lda % 16 == 0 && p->ldb % 16 == 0 && (uintptr_t)p->a % 16 == 0 && (uintptr_t)p->b % 16 == 0 &&
+                        plan.k_end % 16 == 0 && p->lda <= 1 << 22 && p->ldb <= 1 << 22 && p->K <= 1 << 26;
+    const bool tiles = rows16 && ld_sa <= 1 << 20 && ld_sb <= 1 << 20 && p->K > 384;
+    const int pinned = p->flags & (WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256);
+    if(pinned && !tiles)
         return fail(WQ_ERR_UNSUPPORTED, "fp8 weights: WQ_FLAG_TILE_* needs 16-byte aligned rows and K a multiple of 16 above 384");
+    // Few rows: one pass over the weights, K dealt to the waves of a workgroup.  Up to 4 rows straight to registers; through LDS
+    // beyond, 64 columns a workgroup once that leaves more than a hundred of them (the activations are read once per workgroup).
+    // With 17 .. 32 rows the tile kernel is as fast from 8192 columns up (11008 x 4096: 17.8 against 17.9 us; 28672 x 8192: 42 against
+    // 60), and from 33 rows everywhere once it splits K (64 rows, 4096 x 11008: 19 against 27; 4096 x 4096: 15 against 13).
+    if(rows16 && !pinned && p->M <= (p->N <= 8192 ? 32 : 16))
+    {
+        plan.f8f8  = p->M <= 4 ? wq::F8F8_SKINNY_DIRECT : p->M > 16 ? wq::F8F8_SKINNY_32 : p->N <= 8192 ? wq::F8F8_SKINNY_16 : wq::F8F8_SKINNY_16X64;
+        plan.route = ROUTE_F8F8;
+        return WQ_OK;
+    }
+    // Tile kernels: the kernel and the number of K slices with the shortest estimate, in microseconds, fitted to 4 weight shapes x 13
+    // row counts x up to 5 slice counts of each kernel (the chosen one is within 10 % of the best measured at all of them): per
+    // workgroup a fixed part, then a time per K tile on the busiest CU (the 256-tile kernel's grows as the chip fills and the
+    // clock falls); slices write and re-read fp32 slabs and need a second kernel.
+    const int klen = plan.k_end - plan.k_begin, ktiles = (klen + 127) / 128;
+    double best    = 1e30;
+    int slices     = plan.k_batch;
+    for(int kernel : {(int)wq::F8F8_ANY, (int)wq::F8F8_128, (int)wq::F8F8_256})
+    {
+        if((kernel == wq::F8F8_ANY) == tiles || (pinned && pinned != (kernel == wq::F8F8_256 ? WQ_FLAG_TILE_256 : WQ_FLAG_TILE_128)))
+            continue;
+        const double grid = (double)((p->M - 1) / wq::f8f8_bm(kernel) + 1) * ((p->N - 1) / wq::f8f8_bn(kernel) + 1);
+        const bool may_split = !plan.partial && !pinned && have_workspace;
+        for(int c = plan.k_batch; c <= (may_split ? 16 : plan.k_batch) && (c == plan.k_batch || ktiles / c >= 2); ++c)
+        {
+            const double wgs = grid * c, chain = std::ceil(wgs / 256) * ((ktiles + c - 1) / c);
+            double t = kernel == wq::F8F8_256 ? 8 + chain * (1.25 + 0.45 * std::min(1.0, wgs / 256)) : 5 + chain * (kernel == wq::F8F8_128 ? 0.62 : 1.6);
+            if(c > 1)
+                t += 3.5 + c * (double)p->M * p->N * 8 / 6e6;
+            if(t < best)
+                best = t, plan.f8f8 = kernel, slices = c;
+        }
+    }
+    if(!plan.partial && slices > 1)
+    {
+        const int per = wqgemm_splitk_kread(klen, slices, 128);
+        const int kb  = (klen + per - 1) / per;
+        if(kb > 1)
+            plan.auto_split = true, plan.partial = true, plan.k_batch = kb, plan.k_per_z = per;
+    }
     plan.route = ROUTE_F8F8;
     return WQ_OK;
 }
@@ -261,7 +298,7 @@ int make_plan(const wqgemm_problem* p, Plan& plan, bool have_workspace = true)
 
     // ---- fp8 x fp8 with block-wise scales of both operands --------------------------------------
     if(is_f8(p->b_dtype))
-        return make_plan_f8f8(p, plan);
+        return make_plan_f8f8(p, plan, have_workspace);
 
     // ---- int8 x int8 requantised GEMM (example/14, client_example/09) ------------------------
     if(p->a_dtype == WQ_I8 && has_block_scales(p))
@@ -739,7 +776,11 @@ void f16_image_of_a(const wqgemm_problem* p, void* workspace, hipStream_t s, wq:
 // Columns of a split-K slab of the fp8 x fp8 kernels: whole groups of four, so that odd N splits like any other.
 int f8f8_ld_part(const wqgemm_problem* p) { return (p->N + 3) & ~3; }
 
-const char* const kF8F8Names[] = {"wq_gemm_f8f8_any", "wq_gemm_f8f8_128", "wq_gemm_f8f8_256"};
+const char* const kF8F8Names[] = {"wq_gemm_f8f8_any",           "wq_gemm_f8f8_128",    "wq_gemm_f8f8_256",   "wq_gemm_f8f8_skinny_direct",
+                                  "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny"};
+const char* const kF8F8Instances[] = {"256, 128, 128, 128, AnyAlignment", "256, 128, 128, 128, LdsDma", "512, 256, 256, 128, LdsDma",
+                                      "1024, 16, 16, 128, WavesSplitK, Direct", "512, 16, 16, 128, WavesSplitK, LdsDma",
+                                      "256, 16, 64, 128, WavesSplitK, LdsDma", "512, 32, 16, 128, WavesSplitK, LdsDma"};
 
 wq::F8F8Params f8f8_params(const wqgemm_problem* p)
 {
@@ -993,7 +1034,7 @@ int launch_main(const wqgemm_problem* p, const Plan& plan, void* workspace, hipS
         if(plan.partial && !plan.to_c)
             gp.ldc = f8f8_ld_part(p);
         const int bm = wq::f8f8_bm(plan.f8f8), bn = wq::f8f8_bn(plan.f8f8);
-        gp.tiles_m = (p->M + bm - 1) / bm, gp.tiles_n = (p->N + bn - 1) / bn;
+        gp.tiles_m = (p->M - 1) / bm + 1, gp.tiles_n = (p->N - 1) / bn + 1;
         // (group_m as for the other tile kernels: g rows of A plus run / g columns of B per XCD)
         const int run = (gp.tiles_m * gp.tiles_n + 7) / 8;
         long best     = 0;
@@ -1416,9 +1457,7 @@ int wqgemm_type_string(const wqgemm_problem* p, char* buf, size_t n)
                  !has_block_scales(p) ? "" : p->scale_block_m % 128 == 0 ? ", ABScalePer128K" : ", ABScalePer128K_RowScaleA");
     else if(plan.route == ROUTE_F8F8)
         snprintf(buf, n, "DeviceGemmMultiD_ABScale_Mfma_gfx950<%s, 16x16x128_f8f6f4, %s, %s, %s, KBatch%d>",
-                 plan.f8f8 == wq::F8F8_256   ? "512, 256, 256, 128, LdsDma"
-                 : plan.f8f8 == wq::F8F8_128 ? "256, 128, 128, 128, LdsDma"
-                                             : "256, 128, 128, 128, AnyAlignment",
+                 kF8F8Instances[plan.f8f8],
                  dt_name(p->a_dtype), dt_name(p->b_dtype), dt_name(p->c_dtype), plan.k_batch);
     else if(plan.route == ROUTE_SKINNY_WS)
         snprintf(buf, n, "DeviceFpAintBGemm_SmallM_gfx950<256, 16, 16, 16x16x32, %s, %s, %s, StreamB, WavesSplitK>",
