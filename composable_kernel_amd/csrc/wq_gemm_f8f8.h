@@ -219,7 +219,8 @@ struct F8F8Tile
 {
     static constexpr int MT = MT_, NT = NT_, WR = WR_, WC = WC_, WAVES = WR * WC, LEAD = LEAD_, WIN = LEAD + 1;
     static constexpr int BM = WR * MT * 16, BN = WC * NT * 16, BK = 128, THREADS = WAVES * 64;
-    static constexpr int A_TILE  = BM * BK, B_TILE = BN * BK, SLOT = A_TILE + B_TILE;
+    static constexpr int A_TILE  = BM * BK, B_TILE = BN * BK;
+    static constexpr int SLOT    = A_TILE + B_TILE <= 32768 ? 32768 : 65536; // (a power of two: slots change by an exclusive or)
     static constexpr int A_DMA   = BM / 16 / WAVES; // pieces per wave and half of A
     static constexpr int B_DMA   = BN / 8 / WAVES;
     static constexpr int S_ROWS  = BM * 16;       // four K tiles of row scales
@@ -444,7 +445,7 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
     // This lane's two 16-byte chunks of row fr of a 16-row block (swizzled position inside the 128-byte row): LDS addresses of the
     // wave's first row block and first column block, in the slot that is read next (they change slots by an exclusive or).
     const int f_lo = fr * 128 + (((2 * fq) ^ f8_a_swz(fr)) << 4), f_hi = fr * 128 + (((2 * fq + 1) ^ f8_a_swz(fr)) << 4);
-    static_assert((T::SLOT & (T::SLOT - 1)) == 0, "slots change by an exclusive or");
+    static_assert((T::SLOT & (T::SLOT - 1)) == 0 && T::A_TILE + T::B_TILE <= T::SLOT, "slots change by an exclusive or");
     uint32_t a_lo, a_hi, b_lo, b_hi;
     i8v_t af[WIN], bf[NT]; // fragments of row blocks mt .. mt + LEAD; weights of the tile
     auto read_frag = [&](uint32_t lo, uint32_t hi, int block) __attribute__((always_inline)) {
@@ -634,8 +635,11 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
 
 using F8F8Tile256 = F8F8Tile<8, 4, 2, 4, 3>;
 using F8F8Tile128 = F8F8Tile<4, 4, 2, 2, 1>;
+using F8F8Tile128x256 = F8F8Tile<4, 4, 2, 4, 1>;
 template <bool TAIL, bool STREAM>
 __global__ __launch_bounds__(512, 2) void wq_gemm_f8f8_256(const F8F8Params p) { f8f8_tile_body<F8F8Tile256, TAIL, STREAM>(p); }
+template <bool TAIL, bool STREAM>
+__global__ __launch_bounds__(512, 2) void wq_gemm_f8f8_128x256(const F8F8Params p) { f8f8_tile_body<F8F8Tile128x256, TAIL, STREAM>(p); }
 template <bool TAIL, bool STREAM>
 __global__ __launch_bounds__(256, 2) void wq_gemm_f8f8_128(const F8F8Params p) { f8f8_tile_body<F8F8Tile128, TAIL, STREAM>(p); }
 

@@ -48,6 +48,11 @@ int launch_f8f8(int kernel, const F8F8Params& p, hipStream_t s)
                              : launch_tile<F8F8Tile256, wq_gemm_f8f8_256<false, true>>(p, dim3((unsigned)std::min(units, 256L)), s)
                : tail ? launch_tile<F8F8Tile256, wq_gemm_f8f8_256<true, false>>(p, dim3((unsigned)units), s)
                       : launch_tile<F8F8Tile256, wq_gemm_f8f8_256<false, false>>(p, dim3((unsigned)units), s);
+    case F8F8_128X256:
+        return stream ? tail ? launch_tile<F8F8Tile128x256, wq_gemm_f8f8_128x256<true, true>>(p, dim3((unsigned)std::min(units, 256L)), s)
+                             : launch_tile<F8F8Tile128x256, wq_gemm_f8f8_128x256<false, true>>(p, dim3((unsigned)std::min(units, 256L)), s)
+               : tail ? launch_tile<F8F8Tile128x256, wq_gemm_f8f8_128x256<true, false>>(p, dim3((unsigned)units), s)
+                      : launch_tile<F8F8Tile128x256, wq_gemm_f8f8_128x256<false, false>>(p, dim3((unsigned)units), s);
     case F8F8_128:
         return stream ? tail ? launch_tile<F8F8Tile128, wq_gemm_f8f8_128<true, true>>(p, dim3((unsigned)std::min(units, 512L)), s)
                              : launch_tile<F8F8Tile128, wq_gemm_f8f8_128<false, true>>(p, dim3((unsigned)std::min(units, 512L)), s)

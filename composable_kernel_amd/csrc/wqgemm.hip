@@ -218,16 +218,19 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
     const int klen = plan.k_end - plan.k_begin, ktiles = (klen + 127) / 128;
     double best    = 1e30;
     int slices     = plan.k_batch;
-    for(int kernel : {(int)wq::F8F8_ANY, (int)wq::F8F8_128, (int)wq::F8F8_256})
+    for(int kernel : {(int)wq::F8F8_ANY, (int)wq::F8F8_128, (int)wq::F8F8_128X256, (int)wq::F8F8_256})
     {
-        if((kernel == wq::F8F8_ANY) == tiles || (pinned && pinned != (kernel == wq::F8F8_256 ? WQ_FLAG_TILE_256 : WQ_FLAG_TILE_128)))
+        if((kernel == wq::F8F8_ANY) == tiles || (pinned && pinned != (kernel == wq::F8F8_256 ? WQ_FLAG_TILE_256 : kernel == wq::F8F8_128 ? WQ_FLAG_TILE_128 : WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256)))
             continue;
         const double grid = (double)((p->M - 1) / wq::f8f8_bm(kernel) + 1) * ((p->N - 1) / wq::f8f8_bn(kernel) + 1);
         const bool may_split = !plan.partial && !pinned && have_workspace;
         for(int c = plan.k_batch; c <= (may_split ? 16 : plan.k_batch) && (c == plan.k_batch || ktiles / c >= 2); ++c)
         {
             const double wgs = grid * c, chain = std::ceil(wgs / 256) * ((ktiles + c - 1) / c);
-            double t = kernel == wq::F8F8_256 ? 8 + chain * (1.25 + 0.45 * std::min(1.0, wgs / 256)) : 5 + chain * (kernel == wq::F8F8_128 ? 0.62 : 1.6);
+            double t = kernel == wq::F8F8_256       ? 8 + chain * (1.25 + 0.35 * std::min(1.0, wgs / 256))
+                       : kernel == wq::F8F8_128X256 ? 6 + chain * (0.75 + 0.2 * std::min(1.0, wgs / 256))
+                       : kernel == wq::F8F8_128     ? 5 + chain * (wgs > 256 ? 0.55 : 0.62)
+                                                    : 5 + chain * 1.6;
             if(c > 1)
                 t += 3.5 + c * (double)p->M * p->N * 8 / 6e6;
             if(t < best)
@@ -776,9 +779,9 @@ void f16_image_of_a(const wqgemm_problem* p, void* workspace, hipStream_t s, wq:
 // Columns of a split-K slab of the fp8 x fp8 kernels: whole groups of four, so that odd N splits like any other.
 int f8f8_ld_part(const wqgemm_problem* p) { return (p->N + 3) & ~3; }
 
-const char* const kF8F8Names[] = {"wq_gemm_f8f8_any",           "wq_gemm_f8f8_128",    "wq_gemm_f8f8_256",   "wq_gemm_f8f8_skinny_direct",
-                                  "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny"};
-const char* const kF8F8Instances[] = {"256, 128, 128, 128, AnyAlignment", "256, 128, 128, 128, LdsDma", "512, 256, 256, 128, LdsDma",
+const char* const kF8F8Names[] = {"wq_gemm_f8f8_any",    "wq_gemm_f8f8_128",           "wq_gemm_f8f8_128x256", "wq_gemm_f8f8_256",
+                                  "wq_gemm_f8f8_skinny_direct", "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny"};
+const char* const kF8F8Instances[] = {"256, 128, 128, 128, AnyAlignment", "256, 128, 128, 128, LdsDma", "512, 128, 256, 128, LdsDma", "512, 256, 256, 128, LdsDma",
                                       "1024, 16, 16, 128, WavesSplitK, Direct", "512, 16, 16, 128, WavesSplitK, LdsDma",
                                       "256, 16, 64, 128, WavesSplitK, LdsDma", "512, 32, 16, 128, WavesSplitK, LdsDma"};
 
