@@ -40,23 +40,39 @@ struct QuantParams
 constexpr float kF8Max     = 448.f;  // largest finite e4m3fn
 constexpr float kAmaxFloor = 1e-12f; // keeps 448 / amax finite for groups of zeros
 
-// 8 consecutive 16-bit values -> fp32; elements at and past `valid` read as zero
+// 8 consecutive 16-bit values; elements at and past `valid` read as zero
 template <bool BF16>
-__device__ __forceinline__ void quant_load8(const void* base, long at, int valid, float (&v)[8])
+__device__ __forceinline__ u4_t quant_load16(const void* base, long at, int valid)
 {
     const uint16_t* p = (const uint16_t*)base + at;
-    uint16_t b[8];
+    u4_t v            = {0, 0, 0, 0};
     if(valid >= 8)
-        __builtin_memcpy(b, p, 16);
+        __builtin_memcpy(&v, p, 16);
     else
     {
 #pragma unroll
         for(int j = 0; j < 8; ++j)
-            b[j] = j < valid ? p[j] : (uint16_t)0;
+            if(j < valid)
+                v[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
     }
+    return v;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void widen8(u4_t b, float (&v)[8])
+{
 #pragma unroll
     for(int j = 0; j < 8; ++j)
-        v[j] = BF16 ? bf16_to_f32(b[j]) : (float)__builtin_bit_cast(_Float16, b[j]);
+    {
+        const uint16_t h = (uint16_t)(b[j >> 1] >> (16 * (j & 1)));
+        v[j]             = BF16 ? bf16_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+    }
+}
+
+template <bool BF16>
+__device__ __forceinline__ void quant_load8(const void* base, long at, int valid, float (&v)[8])
+{
+    widen8<BF16>(quant_load16<BF16>(base, at, valid), v);
 }
 
 __device__ __forceinline__ void quant_load8_f32(const float* p, int valid, float (&v)[8])
@@ -133,17 +149,29 @@ __device__ __forceinline__ uint32_t row16_max(uint32_t m)
     return m;
 }
 
-// scale of a group from the bits of its largest magnitude, and its reciprocal (a NaN passes through both)
-__device__ __forceinline__ void scale_of(uint32_t bits, float& s, float& inv)
+// Scale of a group from the bits of its largest magnitude, and what the quotients are made with: the reciprocal, and the scale
+// again for the correction (0 if it is infinite: the finite values of such a group become 0, not NaN).
+struct GroupScale
 {
-    float a = __builtin_bit_cast(float, bits);
-    a       = a < kAmaxFloor ? kAmaxFloor : a;
-    s       = a / kF8Max;
-    inv     = kF8Max / a;
-    inv     = __builtin_isinf(a) ? 1.f / a : inv;
-}
+    float s, inv, fix;
+    __device__ __forceinline__ explicit GroupScale(uint32_t bits)
+    {
+        float a = __builtin_bit_cast(float, bits);
+        a       = a < kAmaxFloor ? kAmaxFloor : a; // (a NaN passes through)
+        s       = a / kF8Max;
+        inv     = 1.f / s;
+        fix     = __builtin_isinf(s) ? 0.f : s;
+    }
+    // y / s as a division gives it: the product with the reciprocal, corrected by what it leaves over.  (The product alone rounds
+    // exact ties of the 8-bit format, frequent with 16-bit inputs, either way.)
+    __device__ __forceinline__ float quotient(float y) const
+    {
+        const float q = y * inv;
+        return __builtin_fmaf(__builtin_fmaf(-q, fix, y), inv, q);
+    }
+};
 
-__device__ __forceinline__ float silu(float g) { return g / (1.f + __expf(-g)); }
+__device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
 
 template <bool BF16>
 __device__ __forceinline__ void gated8(const QuantParams& p, long row, int k, int valid, float (&y)[8])
@@ -175,14 +203,13 @@ __global__ __launch_bounds__(256) void wq_quantize_groups(const QuantParams p, i
             gated8<BF16>(p, row, k, valid, y);
         else
             quant_load8<BF16>(p.x, row * p.ldx + k, valid, y);
-        float s, inv;
-        scale_of(row16_max(amax8(y)), s, inv);
+        const GroupScale g(row16_max(amax8(y)));
 #pragma unroll
         for(int j = 0; j < 8; ++j)
-            y[j] *= inv;
+            y[j] = g.quotient(y[j]);
         quant_store8_f8(p.q + row * p.ldq + k, valid, y);
         if((lane & 15) == 0 && valid > 0)
-            p.scale[row * p.ld_scale + (k >> 7)] = s;
+            p.scale[row * p.ld_scale + (k >> 7)] = g.s;
     }
 }
 
@@ -234,6 +261,7 @@ __global__ void wq_quantize_row(const QuantParams p)
     const int waves = T >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     constexpr int RR = R > 0 ? R : 1;
     float y[RR][8];
+    u4_t w16[RR];
 
     float rinv = 1.f;
     if constexpr(OP == 1)
@@ -247,6 +275,14 @@ __global__ void wq_quantize_row(const QuantParams p)
                 const int k = (r * T + (int)threadIdx.x) * 8;
                 row_value8<OP, BF16>(p, row, k, min(p.K - k, 8), y[r]);
             }
+            // (the weights' loads fly while the row's sum is made)
+            if(!p.weight_f32)
+#pragma unroll
+                for(int r = 0; r < RR; ++r)
+                {
+                    const int k = (r * T + (int)threadIdx.x) * 8;
+                    w16[r]      = quant_load16<BF16>(p.weight, k, min(p.K - k, 8));
+                }
 #pragma unroll
             for(int r = 0; r < RR; ++r)
 #pragma unroll
@@ -281,7 +317,7 @@ __global__ void wq_quantize_row(const QuantParams p)
     }
 
     // the final values of piece r (k, valid): the norm's factor and weight, and h written out on the way
-    auto finish = [&](float (&v)[8], int k, int valid, bool write_h) __attribute__((always_inline)) {
+    auto finish = [&](float (&v)[8], int k, int valid, bool write_h, int r = -1) __attribute__((always_inline)) {
         if constexpr(OP == 1)
         {
             if(write_h && p.residual_out && valid > 0)
@@ -290,16 +326,16 @@ __global__ void wq_quantize_row(const QuantParams p)
             if(p.weight_f32)
                 quant_load8_f32((const float*)p.weight + k, valid, w);
             else
-                quant_load8<BF16>(p.weight, k, valid, w);
+                widen8<BF16>(r >= 0 ? w16[r] : quant_load16<BF16>(p.weight, k, valid), w);
 #pragma unroll
             for(int j = 0; j < 8; ++j)
                 v[j] = v[j] * rinv * w[j];
         }
     };
-    auto emit = [&](float (&v)[8], int k, int valid, float inv) __attribute__((always_inline)) {
+    auto emit = [&](float (&v)[8], int k, int valid, const GroupScale& g) __attribute__((always_inline)) {
 #pragma unroll
         for(int j = 0; j < 8; ++j)
-            v[j] *= inv;
+            v[j] = g.quotient(v[j]);
         if(valid > 0)
             quant_store8_f8(p.q + row * p.ldq + k, valid, v);
     };
@@ -307,27 +343,26 @@ __global__ void wq_quantize_row(const QuantParams p)
     if constexpr(GROUPED)
     {
         // (16 lanes hold one group; lanes past the row's end hold zeros)
-        auto one = [&](float (&v)[8], int k) __attribute__((always_inline)) {
+        auto one = [&](float (&v)[8], int k, int r) __attribute__((always_inline)) {
             const int valid = min(p.K - k, 8);
-            finish(v, k, valid, true);
-            float s, inv;
-            scale_of(row16_max(amax8(v)), s, inv);
-            emit(v, k, valid, inv);
+            finish(v, k, valid, true, r);
+            const GroupScale g(row16_max(amax8(v)));
+            emit(v, k, valid, g);
             if((lane & 15) == 0 && valid > 0)
-                p.scale[row * p.ld_scale + (k >> 7)] = s;
+                p.scale[row * p.ld_scale + (k >> 7)] = g.s;
         };
         if constexpr(R > 0)
         {
 #pragma unroll
             for(int r = 0; r < RR; ++r)
-                one(y[r], (r * T + (int)threadIdx.x) * 8);
+                one(y[r], (r * T + (int)threadIdx.x) * 8, r);
         }
         else
             for(int k0 = 0; k0 < p.K; k0 += T * 8)
             {
                 const int k = k0 + threadIdx.x * 8;
                 row_value8<OP, BF16>(p, row, k, min(p.K - k, 8), y[0]);
-                one(y[0], k);
+                one(y[0], k, -1);
             }
     }
     else
@@ -339,7 +374,7 @@ __global__ void wq_quantize_row(const QuantParams p)
             for(int r = 0; r < RR; ++r)
             {
                 const int k = (r * T + (int)threadIdx.x) * 8;
-                finish(y[r], k, min(p.K - k, 8), true);
+                finish(y[r], k, min(p.K - k, 8), true, r);
                 m = max(m, amax8(y[r]));
             }
         }
@@ -357,17 +392,16 @@ __global__ void wq_quantize_row(const QuantParams p)
         m = 0;
         for(int w = 0; w < waves; ++w)
             m = max(m, partm[w]);
-        float s, inv;
-        scale_of(m, s, inv);
+        const GroupScale g(m);
         if(threadIdx.x == 0)
-            p.scale[row * p.ld_scale] = s;
+            p.scale[row * p.ld_scale] = g.s;
         if constexpr(R > 0)
         {
 #pragma unroll
             for(int r = 0; r < RR; ++r)
             {
                 const int k = (r * T + (int)threadIdx.x) * 8;
-                emit(y[r], k, min(p.K - k, 8), inv);
+                emit(y[r], k, min(p.K - k, 8), g);
             }
         }
         else
@@ -376,7 +410,7 @@ __global__ void wq_quantize_row(const QuantParams p)
                 const int valid = min(p.K - k, 8);
                 row_value8<OP, BF16>(p, row, k, valid, y[0]);
                 finish(y[0], k, valid, true);
-                emit(y[0], k, valid, inv);
+                emit(y[0], k, valid, g);
             }
     }
 }

@@ -118,9 +118,13 @@ _ACTIVATIONS = {"silu": capi.ACT_SILU, "fastgelu": capi.ACT_FASTGELU}
 _INT_MAX = 2 ** 31 - 1
 
 
-def _inference_only(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} is inference-only: call it under torch.no_grad() or with tensors that need no gradient")
+# (small calls are bound by the host: what follows asks each tensor as little as it can.  The raw stream handle takes 0.07 us
+# where torch.cuda.current_stream(...).cuda_stream takes 1.8)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _needs_gradients(name):
+    raise RuntimeError(f"{name} is inference-only: call it under torch.no_grad() or with tensors that need no gradient")
 
 
 def _same_device(name, x, **others):
@@ -136,21 +140,25 @@ def _rows(t, cols):
     if t.dim() != 2:
         t = t.reshape(-1, cols)
     m = t.shape[0]
-    ld = t.stride(0) if m > 1 else cols
-    if (t.stride(1) != 1 and cols > 1) or ld < cols:
-        t, ld = t.contiguous(), cols
+    if t.is_contiguous():
+        ld = cols
+    else:
+        ld = t.stride(0) if m > 1 else cols
+        if (t.stride(1) != 1 and cols > 1) or ld < cols:
+            t, ld = t.contiguous(), cols
     if m > _INT_MAX or ld > _INT_MAX:
         raise ValueError("at most 2^31 - 1 rows, columns and elements between rows")
     return t, m, ld
 
 
-def _launch_on(device, call, *args):
-    """call(*args, stream) with `device` current: the library launches on the current device."""
-    if torch.cuda.current_device() == device.index:
-        call(*args, torch.cuda.current_stream(device).cuda_stream)
+def _launch_on(x, call, *args):
+    """call(*args, stream) with x's device current: the library launches on the current device."""
+    index = x.get_device()
+    if torch.cuda.current_device() == index:
+        call(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            call(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            call(*args, _raw_stream(index))
 
 
 def _fp8_linear(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype):
@@ -165,12 +173,13 @@ def _fp8_linear(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype):
         raise ValueError(f"unknown epilogue {epilogue!r}")
     if (bias is None) != (epilogue in ("none", "fastgelu")):
         raise ValueError("bias goes with the add / add_fastgelu epilogues only")
-    if x.dim() < 1 or weight.dim() != 2:
+    shape, w_shape = x.shape, weight.shape
+    if not shape or len(w_shape) != 2:
         raise ValueError("x must be (..., K) and weight (N, K)")
-    N, K = weight.shape
-    lead = x.shape[:-1]
-    if x.shape[-1] != K or K == 0 or N == 0:
-        raise ValueError(f"x {tuple(x.shape)} does not go with a weight of shape {(N, K)}")
+    N, K = w_shape
+    lead = shape[:-1]
+    if shape[-1] != K or K == 0 or N == 0:
+        raise ValueError(f"x {tuple(shape)} does not go with a weight of shape {(N, K)}")
     kb = (K + 127) >> 7
     if x_scale.shape != (*lead, kb):
         raise ValueError(f"x_scale must have shape {(*lead, kb)}, got {tuple(x_scale.shape)}")
@@ -180,10 +189,10 @@ def _fp8_linear(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype):
         if bias.shape != (N,) or bias.dtype != out_dtype:
             raise ValueError(f"bias must have shape {(N,)} and the output's dtype {out_dtype}, got {tuple(bias.shape)} {bias.dtype}")
         bias = bias.contiguous()
-    y = torch.empty((*lead, N), dtype=out_dtype, device=x.device)
-    if y.numel() == 0:
-        return y
+    y = x.new_empty((*lead, N), dtype=out_dtype)
     x, M, lda = _rows(x, K)
+    if M == 0:
+        return y
     x_scale, _, ld_a_scale = _rows(x_scale, kb)
     weight, _, ldb = _rows(weight, K)
     weight_scale, _, ld_b_scale = _rows(weight_scale, kb)
@@ -192,81 +201,71 @@ def _fp8_linear(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype):
                         epilogue=_EPILOGUES[epilogue], d0=bias.data_ptr() if bias is not None else None,
                         flags=capi.FLAG_BF16_RTN)
     nbytes = capi.workspace_bytes(p)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    _launch_on(x.device, capi.launch, p, ws.data_ptr() if nbytes else None)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch_on(x, capi.launch, p, ws.data_ptr() if nbytes else None)
     return y
 
 
-def _quantized_outputs(x, K, group_k):
-    if group_k not in (0, 128):
-        raise ValueError(f"group_k must be 128, or 0 for one scale per row, got {group_k}")
-    groups = (K + 127) >> 7 if group_k else 1
-    return torch.empty(x.shape, dtype=_F8, device=x.device), torch.empty((*x.shape[:-1], groups), dtype=torch.float32, device=x.device), groups
-
-
-def _quant_rows_input(name, x):
-    if x.dtype not in _DT:
+def _quantized_rows(name, op, x, x2, weight, activation, eps, group_k, keep):
+    """The common part of the quantisers, their operands' shapes and dtypes checked but for x's; keep: h is stored too."""
+    dtype = _DT.get(x.dtype)
+    if dtype is None:
         raise TypeError(f"{name}: inputs must be float16 or bfloat16, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] == 0:
+    shape = x.shape
+    if not shape or shape[-1] == 0:
         raise ValueError(f"{name}: inputs must be (..., K) with K > 0")
-    return x.shape[-1]
-
-
-def _quantize(op, x, x2, weight, activation, eps, group_k, q, scale, groups, residual_out):
-    K = x.shape[-1]
+    if group_k != 128 and group_k != 0:
+        raise ValueError(f"group_k must be 128, or 0 for one scale per row, got {group_k}")
+    K = shape[-1]
+    groups = (K + 127) >> 7 if group_k else 1
+    if x.is_contiguous():
+        q, out = torch.empty_like(x, dtype=_F8), torch.empty_like(x) if keep else None
+    else:
+        q, out = x.new_empty(shape, dtype=_F8), x.new_empty(shape) if keep else None
+    scale = x.new_empty((*shape[:-1], groups), dtype=torch.float32)
+    x, M, ldx = _rows(x, K)
+    if M == 0:
+        return q, scale, out
     d = capi.Quant()
-    x, M, d.ldx = _rows(x, K)
-    d.op, d.dtype, d.M, d.K, d.group_k, d.ldq, d.ld_scale = op, _DT[x.dtype], M, K, group_k, K, groups
+    d.op, d.dtype, d.M, d.K, d.group_k, d.ldx, d.ldq, d.ld_scale = op, dtype, M, K, group_k, ldx, K, groups
     d.x, d.q, d.scale = x.data_ptr(), q.data_ptr(), scale.data_ptr()
     if x2 is not None:
         x2, _, d.ldx2 = _rows(x2, K)
         d.x2 = x2.data_ptr()
-    if op == capi.QUANT_RMSNORM:
-        d.weight, d.eps = weight.data_ptr(), eps
-        d.weight_dtype = capi.F32 if weight.dtype == torch.float32 else d.dtype
-        if residual_out is not None:
-            d.residual_out, d.ld_residual_out = residual_out.data_ptr(), K
-    elif op == capi.QUANT_GATED:
-        d.activation = activation
-    _launch_on(x.device, capi.quantize, d)
+    if weight is not None:
+        weight = weight.contiguous()
+        d.weight, d.eps, d.weight_dtype = weight.data_ptr(), eps, capi.F32 if weight.dtype == torch.float32 else dtype
+        if keep:
+            d.residual_out, d.ld_residual_out = out.data_ptr(), K
+    d.activation = activation
+    _launch_on(x, capi.quantize, d)
+    return q, scale, out
 
 
 def _quantize_fp8(x, group_k):
-    _same_device("quantize_fp8", x)
-    K = _quant_rows_input("quantize_fp8", x)
-    q, scale, groups = _quantized_outputs(x, K, group_k)
-    if q.numel():
-        _quantize(capi.QUANT_ROWS, x, None, None, 0, 0.0, group_k, q, scale, groups, None)
-    return q, scale
+    if not x.is_cuda:
+        _same_device("quantize_fp8", x)
+    return _quantized_rows("quantize_fp8", capi.QUANT_ROWS, x, None, None, 0, 0.0, group_k, False)[:2]
 
 
 def _gated_fp8(gate, up, activation, group_k):
     _same_device("gated_fp8", gate, up=up)
-    K = _quant_rows_input("gated_fp8", gate)
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}")
     if up.shape != gate.shape or up.dtype != gate.dtype:
         raise ValueError(f"gate and up must have one shape and dtype, got {tuple(gate.shape)} {gate.dtype} and {tuple(up.shape)} {up.dtype}")
-    q, scale, groups = _quantized_outputs(gate, K, group_k)
-    if q.numel():
-        _quantize(capi.QUANT_GATED, gate, up, None, _ACTIVATIONS[activation], 0.0, group_k, q, scale, groups, None)
-    return q, scale
+    return _quantized_rows("gated_fp8", capi.QUANT_GATED, gate, up, None, _ACTIVATIONS[activation], 0.0, group_k, False)[:2]
 
 
 def _rmsnorm_fp8(x, weight, residual, eps, group_k):
     _same_device("rmsnorm_fp8", x, weight=weight, residual=residual)
-    K = _quant_rows_input("rmsnorm_fp8", x)
-    if weight.shape != (K,) or weight.dtype not in (x.dtype, torch.float32):
-        raise ValueError(f"weight must have shape {(K,)} and dtype {x.dtype} or float32, got {tuple(weight.shape)} {weight.dtype}")
+    if weight.shape != x.shape[-1:] or weight.dim() != 1 or weight.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"weight must have shape {tuple(x.shape[-1:])} and dtype {x.dtype} or float32, got {tuple(weight.shape)} {weight.dtype}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"residual must have x's shape and dtype, got {tuple(residual.shape)} {residual.dtype}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    q, scale, groups = _quantized_outputs(x, K, group_k)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
-    if q.numel():
-        _quantize(capi.QUANT_RMSNORM, x, residual, weight.contiguous(), 0, eps, group_k, q, scale, groups, out)
-    return q, scale, out
+    return _quantized_rows("rmsnorm_fp8", capi.QUANT_RMSNORM, x, residual, weight, 0, eps, group_k, residual is not None)
 
 
 @torch.library.custom_op("wqgemm::fp8_linear", mutates_args=())
@@ -325,7 +324,9 @@ def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
     float32; bias (N,) of out_dtype, with the "add" / "add_fastgelu" epilogues ("none" and "fastgelu" go without).  Sums in
     fp32, one rounding to nearest even into out_dtype (float16 or bfloat16).  Any N and K; fastest where K is a multiple of 16
     and the rows are 16-byte aligned."""
-    _inference_only("fp8_linear", x, x_scale, weight, weight_scale, bias)
+    if torch.is_grad_enabled() and (x.requires_grad or x_scale.requires_grad or weight.requires_grad or weight_scale.requires_grad or
+                                    (bias is not None and bias.requires_grad)):
+        _needs_gradients("fp8_linear")
     if torch.compiler.is_compiling():
         return _fp8_linear_op(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype)
     return _fp8_linear(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype)
@@ -335,7 +336,8 @@ def quantize_fp8(x: torch.Tensor, group_k: int = 128) -> tuple[torch.Tensor, tor
     """x (..., K) float16 / bfloat16 -> (q, scale) with x ~ q * scale: q float8_e4m3fn of x's shape, scale float32 of shape
     (..., ceil(K / 128)), one per 128 consecutive values, or (..., 1) for group_k = 0.  scale = max|x| / 448 of its group
     (groups below 1e-12: as if the maximum were that); a NaN makes its whole group NaN."""
-    _inference_only("quantize_fp8", x)
+    if torch.is_grad_enabled() and x.requires_grad:
+        _needs_gradients("quantize_fp8")
     return _quantize_fp8_op(x, group_k) if torch.compiler.is_compiling() else _quantize_fp8(x, group_k)
 
 
@@ -343,7 +345,8 @@ def gated_fp8(gate: torch.Tensor, up: torch.Tensor, activation: str = "silu",
               group_k: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
     """quantize_fp8 of activation(gate) * up, evaluated in fp32 (activation "silu" or "fastgelu").  gate and up may be the
     two halves of one projection's output (row-strided views are read in place)."""
-    _inference_only("gated_fp8", gate, up)
+    if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
+        _needs_gradients("gated_fp8")
     return (_gated_fp8_op if torch.compiler.is_compiling() else _gated_fp8)(gate, up, activation, group_k)
 
 
@@ -351,7 +354,8 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
                 group_k: int = 128) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
     """h = x + residual; returns (q, scale) = quantize_fp8 of h / sqrt(mean(h^2) + eps) * weight, and h rounded to x's dtype
     (None without a residual).  The norm sees h unrounded; weight (K,) has x's dtype or float32."""
-    _inference_only("rmsnorm_fp8", x, weight, residual)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        _needs_gradients("rmsnorm_fp8")
     if torch.compiler.is_compiling():
         q, scale, out = _rmsnorm_fp8_op(x, weight, residual, eps, group_k)
         return q, scale, out if residual is not None else None
