@@ -20,8 +20,21 @@ void launch_groups(const QuantParams& p, hipStream_t s)
 }
 
 template <int OP, bool BF16, bool GROUPED>
-void launch_row(const QuantParams& p, hipStream_t s)
+void launch_row(QuantParams p, hipStream_t s)
 {
+    // (a launch holds fewer than 2^32 work items: more rows than that go in several)
+    constexpr int MOST = 1 << 21;
+    for(; p.M > MOST; p.M -= MOST)
+    {
+        QuantParams part = p;
+        part.M           = MOST;
+        launch_row<OP, BF16, GROUPED>(part, s);
+        p.x     = (const uint16_t*)p.x + MOST * p.ldx;
+        p.x2    = p.x2 ? (const uint16_t*)p.x2 + MOST * p.ldx2 : nullptr;
+        p.q     = p.q + MOST * p.ldq;
+        p.scale = p.scale + MOST * p.ld_scale;
+        p.residual_out = p.residual_out ? (uint16_t*)p.residual_out + MOST * p.ld_res : nullptr;
+    }
     // Threads: 512 with up to two pieces each in registers (norm of 4096 x 8192: 51.8 us = 4.5 TB/s; 256 threads 60, 1024 54), 1024
     // for longer rows, and while there are few rows, where the latency of one counts (64 x 8192: 4.1 us, 512 threads 4.8).
     const long pieces = ((long)p.K + 7) / 8;

@@ -191,7 +191,9 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
         plan.route = ROUTE_GENERIC;
         return WQ_OK;
     }
-    if(p->M > 0x7FFFFF00 || p->N > 0x7FFFFF00 || (long)((p->M + 127) / 128) * ((p->N + 127) / 128) > 0x7FFFFFFFL)
+    // (a launch holds fewer than 2^32 work items along x, of which a 128 x 128 tile takes 256, and 65535 slices along y or z)
+    if(p->M > 0x7FFFFF00 || p->N > 0x7FFFFF00 || plan.k_batch > 65535 ||
+       (long)((p->M + 127) / 128) * ((p->N + 127) / 128) * plan.k_batch >= 1L << 24)
         return fail(WQ_ERR_UNSUPPORTED, "too many tiles for one launch");
     // The kernels that load 16 bytes at a time: aligned rows, slices that end on whole pieces, distances inside a tile in 32 bits.
     const int ld_sa = std::max(p->ld_a_scale, (p->K - 1) / 128 + 1), ld_sb = std::max(p->ld_b_scale, (p->K - 1) / 128 + 1);
@@ -205,7 +207,7 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
     // beyond, 64 columns a workgroup once that leaves more than a hundred of them (the activations are read once per workgroup).
     // With 17 .. 32 rows the tile kernel is as fast from 8192 columns up (11008 x 4096: 17.8 against 17.9 us; 28672 x 8192: 42 against
     // 60), and from 33 rows everywhere once it splits K (64 rows, 4096 x 11008: 19 against 27; 4096 x 4096: 15 against 13).
-    if(rows16 && !pinned && p->M <= (p->N <= 8192 ? 32 : 16))
+    if(rows16 && !pinned && p->M <= (p->N <= 8192 ? 32 : 16) && p->N <= 1 << 25) // (64 work items per column: as above)
     {
         plan.f8f8  = p->M <= 4 ? wq::F8F8_SKINNY_DIRECT : p->M > 16 ? wq::F8F8_SKINNY_32 : p->N <= 8192 ? wq::F8F8_SKINNY_16 : wq::F8F8_SKINNY_16X64;
         plan.route = ROUTE_F8F8;
@@ -223,7 +225,7 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
         if((kernel == wq::F8F8_ANY) == tiles || (pinned && pinned != (kernel == wq::F8F8_256 ? WQ_FLAG_TILE_256 : kernel == wq::F8F8_128 ? WQ_FLAG_TILE_128 : WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256)))
             continue;
         const double grid = (double)((p->M - 1) / wq::f8f8_bm(kernel) + 1) * ((p->N - 1) / wq::f8f8_bn(kernel) + 1);
-        const bool may_split = !plan.partial && !pinned && have_workspace;
+        const bool may_split = !plan.partial && !pinned && have_workspace && grid < 1 << 16; // (work items along x)
         for(int c = plan.k_batch; c <= (may_split ? 16 : plan.k_batch) && (c == plan.k_batch || ktiles / c >= 2); ++c)
         {
             const double wgs = grid * c, chain = std::ceil(wgs / 256) * ((ktiles + c - 1) / c);
@@ -1518,6 +1520,8 @@ int wqgemm_quantize(const wqgemm_quant* q, void* stream)
         return fail(WQ_ERR_INVALID, "quantize: unknown op %d", q->op);
     if(q->M <= 0 || q->K <= 0)
         return fail(WQ_ERR_INVALID, "quantize: M and K must be positive (got %d, %d)", q->M, q->K);
+    if(q->K > 1 << 30) // (positions inside a row are 32 bits, and run a workgroup's step past its end)
+        return fail(WQ_ERR_UNSUPPORTED, "quantize: rows of at most 2^30 elements (K = %d)", q->K);
     if(!is16(q->dtype))
         return fail(WQ_ERR_UNSUPPORTED, "quantize: inputs must be fp16 or bf16");
     if(q->group_k != 0 && q->group_k != 128)

@@ -203,7 +203,10 @@ int wqgemm_is_supported(const wqgemm_problem* p);
  *    matrix-core kernel runs);
  *  - K*N for tile-aligned row-major (K x N) 8-bit weights (optional: holds the K-contiguous transpose the
  *    matrix-core kernels read);
+ *  - kb*M*roundup(N, 4)*4 for fp8 weights, k_batch > 1 or the planner's own split (optional: without it one slice);
  *  - else 0.
+ * The answer is for *p as it stands: strides and the alignment of its pointers choose the kernel, so ask with the problem that
+ * will be launched.
  * Without an optional workspace the launch uses the general kernel, which gives the same results far slower.
  * Replaces BaseOperator::GetWorkSpaceSize
  * (device_base.hpp:60; impl/device_gemm_xdl_cshuffle_v3r1.hpp:686-694). */
@@ -285,7 +288,7 @@ int wqgemm_pack_int4_host(const int8_t* q, int32_t ldq, int32_t K, int32_t N, ui
  * its scale and all its bytes NaN; an infinity makes the scale infinite and its own bytes NaN.
  * All strides count elements of their tensor and no alignment beyond an element's own is required (16-byte aligned rows
  * are fastest).  residual_out may be x or x2 themselves (same pointer and stride); no other outputs may overlap an input.
- * Rows are independent: a row's result does not depend on M. */
+ * Rows are independent: a row's result does not depend on M.  K up to 2^30. */
 typedef enum wq_quant_op
 {
     WQ_QUANT_ROWS    = 0,

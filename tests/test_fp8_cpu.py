@@ -100,6 +100,33 @@ def test_quantize_refusals(kw):
     assert "quantize" in str(e.value)
 
 
+@pytest.mark.parametrize("kw", [dict(K=2 ** 30 + 1), dict(K=2 ** 31 - 1), dict(op=capi.QUANT_RMSNORM, weight=FAKE, K=2 ** 30 + 1),
+                                dict(group_k=0, K=2 ** 31 - 1)])
+def test_rows_too_long_for_32_bit_positions_are_refused(kw):
+    d = quant(ldx=2 ** 31 - 1, ldq=2 ** 31 - 1, ld_scale=2 ** 31 - 1, **kw)
+    with pytest.raises(capi.WqError) as e:
+        capi.quantize(d)
+    assert e.value.status == capi.ERR_UNSUPPORTED and "2^30" in str(e.value)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(M=2 ** 19, N=2 ** 19), dict(M=2 ** 31 - 1), dict(N=2 ** 31 - 1, ldc=2 ** 31 - 1), dict(k_batch=65536),
+    dict(M=2 ** 15, N=2 ** 13, k_batch=1024),
+])
+def test_more_tiles_than_a_launch_holds_are_refused(kw):
+    # a launch holds fewer than 2^32 work items along x (a tile takes 256 per 128 x 128 outputs) and 65535 slices
+    kw.setdefault("ldc", kw.get("N", 512))
+    p = f8(**kw)
+    assert not capi.is_supported(p)
+    assert "too many tiles" in capi.lib.wqgemm_last_error().decode()
+
+
+def test_strips_of_columns_stay_within_a_launch():
+    # 16 columns take 1024 work items in the kernel for few rows: 2^32 are reached at 2^26 columns, where tiles take over
+    assert capi.kernel_name(f8(M=1, N=2 ** 25, ldc=2 ** 25)) == "wq_gemm_f8f8_skinny_direct"
+    assert "skinny" not in capi.kernel_name(f8(M=1, N=2 ** 26, ldc=2 ** 26))
+
+
 def test_null_descriptor():
     assert capi.lib.wqgemm_quantize(None, None) == capi.ERR_INVALID
 

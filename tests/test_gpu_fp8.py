@@ -1,5 +1,8 @@
 """The fp8 x fp8 product with block-wise scales and the quantisers of its activations on the GPU, against 64-bit references."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -275,6 +278,39 @@ def test_operands_beyond_32_bits():
     check(launch(Q, torch.float16), Q, torch.float16)
 
 
+def test_outputs_beyond_32_bits():
+    """C and the weights past 4 GiB in the tile kernels: the last rows, and the last columns, of both."""
+    m, n, k = 40000, 65536, 512
+    P = problem(m, n, k, 5)
+    got = launch(P, torch.bfloat16)
+    tail = dict(P, m=200, a_bits=P["a_bits"][-200:], sa=P["sa"][-200:])
+    check(got[-200:], tail, torch.bfloat16)
+    del got
+    ldb = 1 << 22
+    b = torch.empty(1300 * ldb, dtype=torch.uint8, device="cuda")
+    Q = problem(300, 1300, k, 6)
+    b.as_strided((1300, k), (ldb, 1)).copy_(Q["b_bits"])
+    Q["b_ptr"], Q["ldb"], Q["keep"] = b.data_ptr(), ldb, b
+    check(launch(Q, torch.float16), Q, torch.float16)
+    R = dict(Q, m=16, a_bits=Q["a_bits"][:16], sa=Q["sa"][:16])
+    check(launch(R, torch.float16), R, torch.float16)
+
+
+@pytest.mark.parametrize("m", [1, 10, 137])
+@pytest.mark.parametrize("flags", [0, capi.FLAG_TILE_128, capi.FLAG_TILE_256, capi.FLAG_TILE_128 | capi.FLAG_TILE_256])
+def test_nothing_behind_the_last_row(m, flags):
+    """A C of many more rows than the product: all of a tile's rows past M, and those of the tile behind it, stay as they were."""
+    n, k = 264, 640
+    P = problem(m, n, k, m)
+    c = torch.full((m + 600, n), -77.0, dtype=torch.float16, device="cuda")
+    p = capi.f8_problem(P["a_ptr"], P["sa"].data_ptr(), P["b_ptr"], P["sb"].data_ptr(), c.data_ptr(), m, n, k, c_dtype=capi.F16,
+                        scale_block=P["block"], flags=flags)
+    capi.launch(p, None, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    check(c[:m], P, torch.float16)
+    assert bool((c[m:] == -77).all())
+
+
 # ---- quantisers ----
 
 def rows(m, k, seed, dtype):
@@ -407,6 +443,38 @@ def test_strided_rows_in_place_and_guards(op, group, k, ld):
         assert bool(torch.isnan(outside).all()) and bool(torch.isnan(t[:3]).all())
 
 
+@pytest.mark.parametrize("op", ["rows", "norm", "gated"])
+@pytest.mark.parametrize("group", [128, 0])
+def test_quantisers_beyond_32_bits(op, group):
+    """More than 2^31 elements: the rows at the end are those of a small call."""
+    m, k, last, dtype = 70000, 40000, 5, torch.bfloat16
+    x = torch.empty(m, k, dtype=dtype, device="cuda")
+    x.view(-1, 8 * k)[:] = rows(8, k, 3, dtype).view(-1)
+    x[-last:] = rows(last, k, 4, dtype)
+    w = torch.randn(k, device="cuda", generator=gen(2)).to(dtype)
+    call = {"rows": lambda v: torch_ops.quantize_fp8(v, group), "norm": lambda v: torch_ops.rmsnorm_fp8(v, w, v, 1e-6, group),
+            "gated": lambda v: torch_ops.gated_fp8(v, v, "silu", group)}[op]
+    for big, small in zip(call(x), call(x[-last:].clone())):
+        if small is not None:
+            assert torch.equal(big[-last:].view(torch.uint8), small.view(torch.uint8))
+
+
+@pytest.mark.parametrize("op", ["rows", "norm"])
+def test_more_rows_than_a_launch_holds(op):
+    """One workgroup per row: 2^26 rows of 64 threads are 2^32 work items, more than one launch takes."""
+    m, k, dtype = 2 ** 26 + 5, 3, torch.float16
+    part = rows(1021, k, 8, dtype)
+    x = part.repeat(m // 1021 + 1, 1)[:m]
+    w = torch.ones(k, device="cuda", dtype=dtype)
+    call = (lambda v: torch_ops.quantize_fp8(v, 0)) if op == "rows" else (lambda v: torch_ops.rmsnorm_fp8(v, w, v, 1e-6, 0))
+    small = call(part)
+    at = torch.arange(m, device="cuda") % 1021
+    for got, want in zip(call(x), small):
+        if want is not None:
+            got, want = got.view(torch.uint8), want.view(torch.uint8)
+            assert all(torch.equal(got[i:i + 2 ** 24], want[at[i:i + 2 ** 24]]) for i in range(0, m, 2 ** 24))
+
+
 # ---- the torch front end, and the operators together ----
 
 def test_linear_module_and_leading_dimensions():
@@ -525,6 +593,26 @@ def test_block_captured_and_replayed(m):
             torch.cuda.synchronize()
             want, want_res = block(x.clone(), r.clone())
             assert torch.equal(y, want) and torch.equal(res, want_res)
+
+
+def test_first_call_of_a_process_is_captured():
+    """Nothing that a first call sets up (code objects, shared memory above 64 KiB) disturbs a capture."""
+    code = """
+import torch
+from composable_kernel_amd import torch_ops
+x, g = torch.randn(600, 1024, device="cuda").bfloat16(), torch.cuda.CUDAGraph()
+w, ws = torch.randn(512, 1024, device="cuda").to(torch.float8_e4m3fn), torch.rand(4, 8, device="cuda")
+torch.cuda.synchronize()
+with torch.cuda.graph(g):
+    y = [torch_ops.fp8_linear(*torch_ops.quantize_fp8(x[:m]), w, ws) for m in (1, 12, 20, 300, 600)]
+g.replay(), torch.cuda.synchronize()
+for m, v in zip((1, 12, 20, 300, 600), y):
+    assert torch.equal(v, torch_ops.fp8_linear(*torch_ops.quantize_fp8(x[:m]), w, ws)), m
+print("same")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True,
+                       text=True, timeout=100)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
 
 
 def test_two_streams_at_once():
