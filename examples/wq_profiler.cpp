@@ -8,7 +8,9 @@
 //   gemm_quantization        the int8 row of profile_gemm.cpp:20-27 with example/14's requantisation epilogue
 // The data-type enums are extended for the weight-quantized forms this engine adds (listed in each usage text).
 // A stride of -1 (script/profile_mixed_gemm.sh:17-51) selects the packed default.
+#include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <functional>
 #include <iomanip>
 #include <iostream>
@@ -421,42 +423,60 @@ int profile_gemm_multiply_multiply(int argc, char* argv[])
     return run_mm<ck::wq_f8_e4m3fn_t, false>(c, sa, sb, se, n_warmup, n_iter, rotating);
 }
 
-// ---- fp8 activations x int4 weights, fp32 scales per 128 x 128 block of both operands ------------------------------------
-template <typename ADataType, typename EDataType, bool NoSpecials>
-int run_ab_scale(const Common& c, ck::index_t sa, ck::index_t sb, ck::index_t se, int n_warmup, int n_iter, uint64_t rotating)
+// ---- fp8 activations x int4 or fp8 weights, fp32 scales per 128 x 128 block of both operands -----------------------------
+// bytes of fp8 operands: -2 .. 2 (init 1: the reference's GeneratorTensor_2{-2, 2}), else eight binades around one
+template <typename F8>
+void fill_f8(Tensor<F8>& t, int init, std::mt19937& gen)
 {
-    constexpr ck::index_t BM = 128, BN = 128, BK = 128;
-    using Op = dev::DeviceGemmMultiD_ABScale_WeightQuant_gfx950<Row, Col, Row, ADataType, ck::wq_int4x2_t, EDataType, BM, BN, BK, NoSpecials>;
-    const auto m = static_cast<std::size_t>(c.M), n = static_cast<std::size_t>(c.N), k = static_cast<std::size_t>(c.K);
-    const std::size_t mb = (m + BM - 1) / BM, nb = (n + BN - 1) / BN, kb = (k + BK - 1) / BK;
-    Tensor<ADataType> a0(HostTensorDescriptor({m, k}, {static_cast<std::size_t>(sa), 1}));
-    Tensor<float> a1(HostTensorDescriptor({mb, kb}, {kb, 1}));
-    Tensor<int8_t> q(HostTensorDescriptor({k, n}, {1, static_cast<std::size_t>(sb)}));
-    Tensor<float> b1(HostTensorDescriptor({kb, nb}, {1, kb}));
-    Tensor<EDataType> e_dev(HostTensorDescriptor({m, n}, {static_cast<std::size_t>(se), 1})), e_host(e_dev.mDesc);
-    std::mt19937 gen(11939);
-    const uint8_t one = std::is_same_v<ADataType, ck::wq_f8_e4m3fn_t> ? 0x38 : 0x40; // 1.0 in E4M3FN / FNUZ
-    auto* bytes       = reinterpret_cast<uint8_t*>(a0.mData.data());
-    for(std::size_t i = 0; i < a0.mData.size(); ++i)
+    const uint8_t one = std::is_same_v<F8, ck::wq_f8_e4m3fn_t> ? 0x38 : 0x40; // 1.0 in E4M3FN / FNUZ
+    auto* bytes       = reinterpret_cast<uint8_t*>(t.mData.data());
+    for(std::size_t i = 0; i < t.mData.size(); ++i)
     {
         const uint32_t r = gen();
-        if(c.init == 1)
+        if(init == 1)
         {
-            const int v = static_cast<int>(r % 5) - 2; // -2 .. 2, as the reference's GeneratorTensor_2{-2, 2}
+            const int v = static_cast<int>(r % 5) - 2;
             bytes[i]    = v == 0 ? 0 : static_cast<uint8_t>((v < 0 ? 0x80 : 0) | (one + (std::abs(v) == 2 ? 8 : 0)));
         }
         else
             bytes[i] = static_cast<uint8_t>((r & 0x80) | ((one - 32 + ((r >> 8) % 64)) & 0x7F));
     }
-    q.GenerateTensorValue(GeneratorTensor_2<int8_t>{-8, 8});
+}
+
+// BDataType: ck::wq_int4x2_t, or the fp8 type of the activations
+template <typename ADataType, typename BDataType, typename EDataType, bool NoSpecials>
+int run_ab_scale(const Common& c, ck::index_t sa, ck::index_t sb, ck::index_t se, int n_warmup, int n_iter, uint64_t rotating)
+{
+    constexpr ck::index_t BM = 128, BN = 128, BK = 128;
+    constexpr bool int4      = std::is_same_v<BDataType, ck::wq_int4x2_t>;
+    using BValue             = std::conditional_t<int4, int8_t, BDataType>; // host tensor: one value per byte
+    using Op = dev::DeviceGemmMultiD_ABScale_WeightQuant_gfx950<Row, Col, Row, ADataType, BDataType, EDataType, BM, BN, BK, NoSpecials>;
+    const auto m = static_cast<std::size_t>(c.M), n = static_cast<std::size_t>(c.N), k = static_cast<std::size_t>(c.K);
+    const std::size_t mb = (m + BM - 1) / BM, nb = (n + BN - 1) / BN, kb = (k + BK - 1) / BK;
+    Tensor<ADataType> a0(HostTensorDescriptor({m, k}, {static_cast<std::size_t>(sa), 1}));
+    Tensor<float> a1(HostTensorDescriptor({mb, kb}, {kb, 1}));
+    Tensor<BValue> q(HostTensorDescriptor({k, n}, {1, static_cast<std::size_t>(sb)}));
+    Tensor<float> b1(HostTensorDescriptor({kb, nb}, {1, kb}));
+    Tensor<EDataType> e_dev(HostTensorDescriptor({m, n}, {static_cast<std::size_t>(se), 1})), e_host(e_dev.mDesc);
+    std::mt19937 gen(11939);
+    fill_f8(a0, c.init, gen);
+    if constexpr(int4)
+        q.GenerateTensorValue(GeneratorTensor_2<int8_t>{-8, 8});
+    else
+        fill_f8(q, c.init, gen);
     a1.GenerateTensorValue(GeneratorTensor_3<float>{0, 1.0}); // (profile_gemm_ab_scale_impl.hpp:104-117)
     b1.GenerateTensorValue(GeneratorTensor_3<float>{0, 1.0});
-    std::vector<uint8_t> packed(static_cast<std::size_t>(sb) / 2 * n);
-    if(wqgemm_pack_int4_host(q.mData.data(), sb, c.K, c.N, packed.data(), sb / 2) != WQ_OK)
+    std::vector<uint8_t> packed(static_cast<std::size_t>(sb) / (int4 ? 2 : 1) * n);
+    if constexpr(int4)
     {
-        std::cerr << wqgemm_last_error() << std::endl;
-        return 1;
+        if(wqgemm_pack_int4_host(q.mData.data(), sb, c.K, c.N, packed.data(), sb / 2) != WQ_OK)
+        {
+            std::cerr << wqgemm_last_error() << std::endl;
+            return 1;
+        }
     }
+    else
+        std::memcpy(packed.data(), q.mData.data(), std::min(packed.size(), q.mData.size()));
     DeviceMem a0_buf(a0.mData.size()), a1_buf(4 * a1.mData.size()), b0_buf(packed.size()), b1_buf(4 * b1.mData.size()),
         e_buf(sizeof(EDataType) * e_dev.mData.size());
     a0_buf.ToDevice(a0.mData.data());
@@ -466,6 +486,10 @@ int run_ab_scale(const Common& c, ck::index_t sa, ck::index_t sb, ck::index_t se
     auto op  = Op{};
     auto arg = op.MakeArgument(a0_buf.GetDeviceBuffer(), b0_buf.GetDeviceBuffer(), {}, e_buf.GetDeviceBuffer(), c.M, c.N, c.K, sa, sb, {},
                                se, a1_buf.GetDeviceBuffer(), b1_buf.GetDeviceBuffer(), PassThrough{}, PassThrough{}, PassThrough{});
+    const std::size_t ws_bytes = op.GetWorkSpaceSize(&arg);
+    DeviceMem ws_buf(ws_bytes ? ws_bytes : 1);
+    if(ws_bytes)
+        op.SetWorkSpacePointer(&arg, ws_buf.GetDeviceBuffer());
     const std::string name = dev::wq_detail::type_string(arg.prob);
     if(!op.IsSupportedArgument(arg))
     {
@@ -487,7 +511,7 @@ int run_ab_scale(const Common& c, ck::index_t sa, ck::index_t sb, ck::index_t se
                 a_f(i, kk) = ck::type_convert<float>(a0(i, kk)) * a1(i / BM, kk / BK);
         for(std::size_t j = 0; j < n; ++j)
             for(std::size_t kk = 0; kk < k; ++kk)
-                b_f(kk, j) = static_cast<float>(q(kk, j)) * b1(kk / BK, j / BN);
+                b_f(kk, j) = ck::type_convert<float>(q(kk, j)) * b1(kk / BK, j / BN);
         using Ref = ck::tensor_operation::host::ReferenceGemm<float, float, float, float, PassThrough, PassThrough, PassThrough>;
         auto ref  = Ref{};
         ref.MakeInvoker().Run(ref.MakeArgument(a_f, b_f, acc, PassThrough{}, PassThrough{}, PassThrough{}));
@@ -499,7 +523,7 @@ int run_ab_scale(const Common& c, ck::index_t sa, ck::index_t sb, ck::index_t se
     }
     if(c.time)
         report(std::is_same_v<EDataType, ck::bhalf_t> ? "bf16" : "f16", c.M, c.N, c.K, sa, sb, se, ms,
-               m * k + k * n / 2 + sizeof(EDataType) * m * n, name);
+               m * k + k * n / (int4 ? 2 : 1) + sizeof(EDataType) * m * n, name);
     return pass ? 0 : 1;
 }
 
@@ -518,13 +542,13 @@ int profile_gemm_ab_scale(int argc, char* argv[])
         c.log       = std::stoi(argv[7]);
         c.time      = std::stoi(argv[8]);
         c.M = std::stoi(argv[9]), c.N = std::stoi(argv[10]), c.K = std::stoi(argv[11]);
-        ok = c.layout == 1 && std::stoi(argv[4]) == 0 && c.data_type >= 8 && c.data_type <= 11;
+        ok = c.layout == 1 && std::stoi(argv[4]) == 0 && c.data_type >= 8 && c.data_type <= 14;
     }
     if(!ok)
     {
         std::cout << "arg1: tensor operation (gemm_ab_scale: GEMM_AB_Scale)\n"
                   << "arg2: data type (8: f8 FNUZ@int4 -> f16, no 0x7F/0xFF/0x80 bytes; 9: the same -> bf16; 10: f8 E4M3FN@int4 -> f16; "
-                     "11: -> bf16)\n"
+                     "11: -> bf16; 12: f8 E4M3FN@f8 E4M3FN -> f16; 13: -> bf16; 14: f8 FNUZ@f8 FNUZ -> bf16, no 0x7F/0xFF/0x80 bytes)\n"
                   << "arg3: matrix layout (1: A[m, k] * B[n, k] = C[m, n])\n"
                   << "arg4: scale block tile (0: ScaleBlockM/N/K = [128, 128, 128])\n"
                   << "arg5: verification (0: no; 1: yes)\narg6: initialization (0: no init; 1: integer value; 2: decimal value)\n"
@@ -540,10 +564,13 @@ int profile_gemm_ab_scale(int argc, char* argv[])
     const uint64_t rotating = argc == 18 ? std::stoull(argv[17]) * 1024 * 1024 : 0;
     switch(c.data_type)
     {
-    case 8: return run_ab_scale<ck::f8_t, ck::half_t, true>(c, sa, sb, se, n_warmup, n_iter, rotating);
-    case 9: return run_ab_scale<ck::f8_t, ck::bhalf_t, true>(c, sa, sb, se, n_warmup, n_iter, rotating);
-    case 10: return run_ab_scale<ck::wq_f8_e4m3fn_t, ck::half_t, false>(c, sa, sb, se, n_warmup, n_iter, rotating);
-    default: return run_ab_scale<ck::wq_f8_e4m3fn_t, ck::bhalf_t, false>(c, sa, sb, se, n_warmup, n_iter, rotating);
+    case 8: return run_ab_scale<ck::f8_t, ck::wq_int4x2_t, ck::half_t, true>(c, sa, sb, se, n_warmup, n_iter, rotating);
+    case 9: return run_ab_scale<ck::f8_t, ck::wq_int4x2_t, ck::bhalf_t, true>(c, sa, sb, se, n_warmup, n_iter, rotating);
+    case 10: return run_ab_scale<ck::wq_f8_e4m3fn_t, ck::wq_int4x2_t, ck::half_t, false>(c, sa, sb, se, n_warmup, n_iter, rotating);
+    case 12: return run_ab_scale<ck::wq_f8_e4m3fn_t, ck::wq_f8_e4m3fn_t, ck::half_t, false>(c, sa, sb, se, n_warmup, n_iter, rotating);
+    case 13: return run_ab_scale<ck::wq_f8_e4m3fn_t, ck::wq_f8_e4m3fn_t, ck::bhalf_t, false>(c, sa, sb, se, n_warmup, n_iter, rotating);
+    case 14: return run_ab_scale<ck::f8_t, ck::f8_t, ck::bhalf_t, true>(c, sa, sb, se, n_warmup, n_iter, rotating);
+    default: return run_ab_scale<ck::wq_f8_e4m3fn_t, ck::wq_int4x2_t, ck::bhalf_t, false>(c, sa, sb, se, n_warmup, n_iter, rotating);
     }
 }
 
@@ -552,7 +579,7 @@ const Register r1("gemm_splitk", "Split-K GEMM with weight-only quantized B", pr
 const Register r2("gemm_quantization", "int8 GEMM + Activation_Mul_Clamp", profile_gemm_quantization);
 const Register r2g("gemm", "GEMM (data type 3: int8, requantised)", profile_gemm_quantization);
 const Register r3("gemm_multiply_multiply", "GEMM_Multiply_Multiply (fp8 x int4)", profile_gemm_multiply_multiply);
-const Register r4("gemm_ab_scale", "GEMM_AB_Scale (fp8 x int4, 128 x 128 x 128 block scales of both operands)", profile_gemm_ab_scale);
+const Register r4("gemm_ab_scale", "GEMM_AB_Scale (fp8 x int4 or fp8, 128 x 128 x 128 block scales of both operands)", profile_gemm_ab_scale);
 
 } // namespace
 

@@ -22,7 +22,7 @@
 //
 //   DeviceGemmMultiD_ABScale_WeightQuant_gfx950 : DeviceGemmMultipleD_ABScale (example/65 ..._fp8_ab_scale)
 //        stands where DeviceGemmMultiD_ABScale_Xdl_CShuffle_V3<f8, f32, f8, f32> does
-//        (impl/device_gemm_multiple_d_xdl_cshuffle_v3_ab_scale.hpp), with int4 / int8 weights in place of fp8 ones
+//        (impl/device_gemm_multiple_d_xdl_cshuffle_v3_ab_scale.hpp), with fp8 weights, or int4 / int8 ones in their place
 //
 //   DeviceGemmV2R1_WeightQuant_gfx950    : DeviceGemmV2R1          (example/35 gemm_xdl_splitk_reduce_bf16A_i8B)
 //        stands where DeviceGemm_Xdl_CShuffleV3R1<bf16, int8> does
@@ -966,12 +966,14 @@ struct DeviceGemmMultiplyMultiply_Int4Values_gfx950
 // ---------------------------------------------------------------------------------------------
 // E[M,N] = convert( sum_k (float(A[m,k]) * a_scale[m / ScaleBlockM][k / ScaleBlockK])
 //                        * (float(B[k,n]) * b_scale[k / ScaleBlockK][n / ScaleBlockN]) )
-// fp8 activations, int4 (packed / pre-shuffled) or int8 weights, fp32 block scales of BOTH operands -- the problem
-// of example/65_gemm_multiply_multiply/gemm_multiply_multiply_xdl_fp8_ab_scale.cpp:58-75,126-152,262-283 with
-// weight-quantized B.  a_scale is row-major (ceil(M/ScaleBlockM), ceil(K/ScaleBlockK)), b_scale column-major
+// fp8 activations, fp8, int4 (packed / pre-shuffled) or int8 weights, fp32 block scales of BOTH operands -- the problem
+// of example/65_gemm_multiply_multiply/gemm_multiply_multiply_xdl_fp8_ab_scale.cpp:58-75,126-152,262-283, and its
+// weight-quantized forms.  a_scale is row-major (ceil(M/ScaleBlockM), ceil(K/ScaleBlockK)), b_scale column-major
 // (ceil(K/ScaleBlockK), ceil(N/ScaleBlockN)), both densely packed (leading dimension ceil(K/ScaleBlockK), as the
 // example's Scale_Stride_AM / Scale_Stride_BN).  With 128-k blocks (ScaleBlockM a multiple of 128, ScaleBlockN of 32)
 // the fp8 matrix-core kernel scales each 128-k block sum in registers; other block shapes run on the general kernel.
+// fp8 weights take any ScaleBlockM there, and split K into a workspace (GetWorkSpaceSize / SetWorkSpacePointer) where the
+// grid is short; without one they run in one slice.
 // ---------------------------------------------------------------------------------------------
 template <typename ALayout, typename BLayout, typename ELayout, typename ADataType, typename BDataType,
           typename EDataType, index_t ScaleBlockM, index_t ScaleBlockN, index_t ScaleBlockK,
@@ -984,6 +986,7 @@ struct DeviceGemmMultiD_ABScale_WeightQuant_gfx950
     using Argument    = wq_detail::Argument;
     using Invoker     = wq_detail::Invoker;
     using PassThrough = element_wise::PassThrough;
+    static constexpr bool kF8Weights = std::is_same_v<BDataType, ck::wq_f8_e4m3fn_t> || std::is_same_v<BDataType, ck::f8_t>;
 
     static Argument MakeArgument(const void* p_a, const void* p_b, std::array<const void*, 0>, void* p_e, index_t M,
                                  index_t N, index_t K, index_t StrideA, index_t StrideB, std::array<index_t, 0>,
@@ -1027,11 +1030,15 @@ struct DeviceGemmMultiD_ABScale_WeightQuant_gfx950
                                                        p_a_scale, p_b_scale, a_op, b_op, cde_op));
     }
     std::unique_ptr<BaseInvoker> MakeInvokerPointer() override { return std::make_unique<Invoker>(MakeInvoker()); }
+    size_t GetWorkSpaceSize(const BaseArgument* p_arg) const override
+    {
+        return kF8Weights ? wqgemm_workspace_bytes(&dynamic_cast<const Argument*>(p_arg)->prob) : 0;
+    }
     std::string GetTypeString() const override
     {
         return std::string("DeviceGemmMultiD_ABScale_WeightQuant_gfx950<") +
                (std::is_same_v<ADataType, ck::wq_f8_e4m3fn_t> ? "F8_E4M3FN" : AssumeNoFnuzSpecials ? "F8_FNUZ_NoSpecials" : "F8_FNUZ") +
-               ", " + std::to_string(ScaleBlockM) + "x" + std::to_string(ScaleBlockN) + "x" + std::to_string(ScaleBlockK) + ">";
+               (kF8Weights ? ", fp8 weights, " : ", ") + std::to_string(ScaleBlockM) + "x" + std::to_string(ScaleBlockN) + "x" + std::to_string(ScaleBlockK) + ">";
     }
 };
 

@@ -663,3 +663,21 @@ def test_per_token_scales_feed_the_int4_path():
     ref, size = fp8_ref.linear(a, b)
     bound = (2 * k + 8) * U32 * size + fp8_ref.HALF_STEP[torch.float16] * ref.abs() * (1 + 2.0 ** -8) + fp8_ref.SMALLEST_HALF_STEP[torch.float16]
     assert bool(((y.double() - ref).abs() <= bound)[torch.isfinite(y)].all()) and bool((torch.isfinite(y) | (ref.abs() > 65000)).all())
+
+
+@pytest.mark.parametrize("args", [
+    ("gemm_ab_scale", 12, 1, 0, 1, 1, 0, 1, 256, 256, 384, -1, -1, -1),
+    ("gemm_ab_scale", 13, 1, 0, 1, 2, 0, 1, 300, 520, 1024, -1, -1, -1),
+    ("gemm_ab_scale", 13, 1, 0, 1, 2, 0, 1, 64, 256, 4096, -1, -1, -1),
+    ("gemm_ab_scale", 14, 1, 0, 1, 2, 0, 1, 16, 512, 640, 656, 672, 530),
+    ("gemm_ab_scale", 12, 1, 0, 1, 2, 0, 1, 40, 100, 333, -1, -1, -1, 2, 7, 16),
+])
+def test_profiler_command_with_fp8_weights(args):
+    """The command line's block-scaled operation with fp8 weights, through the C++ operator, verified on the host."""
+    exe = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "example_wq_profiler")
+    r = subprocess.run([exe, *map(str, args)], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert "verification: PASS" in r.stdout and "Best Perf for datatype" in r.stdout
+    assert "16x16x128_f8f6f4" in r.stdout and "DeviceGemmMultiD_ABScale_Mfma_gfx950" in r.stdout
+    if len(args) == 17:
+        assert "rotating count: 7" in r.stdout
