@@ -8,7 +8,10 @@ namespace wq {
 enum F8F8Kernel
 {
     F8F8_ANY = 0, // 128 x 128, any alignment and K
+    F8F8_64X64,   // 64 x 64, four waves, three workgroups per CU
+    F8F8_64,      // 64 x 128, four waves, two workgroups per CU
     F8F8_128,     // 128 x 128, four waves, two workgroups per CU
+    F8F8_128_W8,  // 128 x 128, eight waves, one workgroup per CU
     F8F8_128X256, // 128 x 256, eight waves
     F8F8_256,     // 256 x 256, eight waves
     F8F8_SKINNY_DIRECT, // M <= 16: 16 columns, sixteen waves, weights straight to registers
@@ -16,10 +19,10 @@ enum F8F8Kernel
     F8F8_SKINNY_16X64,  // M <= 16: 64 columns, four waves
     F8F8_SKINNY_32      // M <= 32: 16 columns, eight waves
 };
-constexpr int f8f8_bm(int kernel) { return kernel == F8F8_256 ? 256 : 128; }
+constexpr int f8f8_bm(int kernel) { return kernel == F8F8_256 ? 256 : kernel == F8F8_64 || kernel == F8F8_64X64 ? 64 : 128; }
 constexpr int f8f8_bn(int kernel)
 {
-    return kernel <= F8F8_128 ? 128 : kernel <= F8F8_256 ? 256 : kernel == F8F8_SKINNY_16X64 ? 64 : 16;
+    return kernel == F8F8_64X64 ? 64 : kernel <= F8F8_128_W8 ? 128 : kernel <= F8F8_256 ? 256 : kernel == F8F8_SKINNY_16X64 ? 64 : 16;
 }
 
 struct F8F8Params

@@ -220,7 +220,7 @@ struct F8F8Tile
     static constexpr int MT = MT_, NT = NT_, WR = WR_, WC = WC_, WAVES = WR * WC, LEAD = LEAD_, WIN = LEAD + 1;
     static constexpr int BM = WR * MT * 16, BN = WC * NT * 16, BK = 128, THREADS = WAVES * 64;
     static constexpr int A_TILE  = BM * BK, B_TILE = BN * BK;
-    static constexpr int SLOT    = A_TILE + B_TILE <= 32768 ? 32768 : 65536; // (a power of two: slots change by an exclusive or)
+    static constexpr int SLOT    = A_TILE + B_TILE <= 16384 ? 16384 : A_TILE + B_TILE <= 32768 ? 32768 : 65536; // (a power of two: slots change by an exclusive or)
     static constexpr int A_DMA   = BM / 16 / WAVES; // pieces per wave and half of A
     static constexpr int B_DMA   = BN / 8 / WAVES;
     static constexpr int S_ROWS  = BM * 16;       // four K tiles of row scales
@@ -633,8 +633,16 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
     }
 }
 
+// The smaller tiles are for grids that leave the chip empty: what a K tile costs is then the time from one barrier to the next, not
+// its bytes or MFMAs (a ring of four K tiles instead of two: 128 x 128 0.75 us a K tile against 0.62), and it shrinks with the tile:
+// 256 x 256 1.6 us, 128 x 256 0.98, 128 x 128 with eight waves 0.6, with four 0.55, 64 x 128 0.37, 64 x 64 0.3.  Eight waves on
+// 128 x 128 hide each other's waits where there is one workgroup per CU (777 x 4096 x 4096: 23.5 us against 24.8), two workgroups of
+// four waves do it better where there are two (512 x 11008 x 4096: 36.6 against 43.5).
 using F8F8Tile256 = F8F8Tile<8, 4, 2, 4, 3>;
 using F8F8Tile128 = F8F8Tile<4, 4, 2, 2, 1>;
+using F8F8Tile128W8 = F8F8Tile<4, 2, 2, 4, 1>;
+using F8F8Tile64 = F8F8Tile<2, 4, 2, 2, 1>;
+using F8F8Tile64x64 = F8F8Tile<2, 2, 2, 2, 1>;
 using F8F8Tile128x256 = F8F8Tile<4, 4, 2, 4, 1>;
 template <bool TAIL, bool STREAM>
 __global__ __launch_bounds__(512, 2) void wq_gemm_f8f8_256(const F8F8Params p) { f8f8_tile_body<F8F8Tile256, TAIL, STREAM>(p); }
@@ -642,6 +650,13 @@ template <bool TAIL, bool STREAM>
 __global__ __launch_bounds__(512, 2) void wq_gemm_f8f8_128x256(const F8F8Params p) { f8f8_tile_body<F8F8Tile128x256, TAIL, STREAM>(p); }
 template <bool TAIL, bool STREAM>
 __global__ __launch_bounds__(256, 2) void wq_gemm_f8f8_128(const F8F8Params p) { f8f8_tile_body<F8F8Tile128, TAIL, STREAM>(p); }
+
+template <bool TAIL, bool STREAM>
+__global__ __launch_bounds__(512, 2) void wq_gemm_f8f8_128_w8(const F8F8Params p) { f8f8_tile_body<F8F8Tile128W8, TAIL, STREAM>(p); }
+template <bool TAIL, bool STREAM>
+__global__ __launch_bounds__(256, 3) void wq_gemm_f8f8_64x64(const F8F8Params p) { f8f8_tile_body<F8F8Tile64x64, TAIL, STREAM>(p); }
+template <bool TAIL, bool STREAM>
+__global__ __launch_bounds__(256, 2) void wq_gemm_f8f8_64(const F8F8Params p) { f8f8_tile_body<F8F8Tile64, TAIL, STREAM>(p); }
 
 // ---------------------------------------------------------------------------------------------
 // Few rows (M <= 16 MT): one pass over the weights, bound by their stream.  A workgroup owns 16 NB columns; its waves deal the K

@@ -41,23 +41,22 @@ int launch_f8f8(int kernel, const F8F8Params& p, hipStream_t s)
     // (streaming workgroups walk the tiles: one resident grid on the 256 CUs)
     const long units = (long)p.tiles_m * p.tiles_n * p.slices;
     const dim3 strips((unsigned)p.tiles_n, (unsigned)p.slices); // small-M kernels: strips of columns
+    // (the last argument: workgroups that the chip holds at a time)
+#define F8F8_TILE_CASE(KIND, TILE, KERNEL, RESIDENT)                                                                             \
+    case KIND:                                                                                                                   \
+        return stream ? tail ? launch_tile<TILE, KERNEL<true, true>>(p, dim3((unsigned)std::min(units, (long)RESIDENT)), s)      \
+                             : launch_tile<TILE, KERNEL<false, true>>(p, dim3((unsigned)std::min(units, (long)RESIDENT)), s)     \
+               : tail ? launch_tile<TILE, KERNEL<true, false>>(p, dim3((unsigned)units), s)                                      \
+                      : launch_tile<TILE, KERNEL<false, false>>(p, dim3((unsigned)units), s);
     switch(kernel)
     {
-    case F8F8_256:
-        return stream ? tail ? launch_tile<F8F8Tile256, wq_gemm_f8f8_256<true, true>>(p, dim3((unsigned)std::min(units, 256L)), s)
-                             : launch_tile<F8F8Tile256, wq_gemm_f8f8_256<false, true>>(p, dim3((unsigned)std::min(units, 256L)), s)
-               : tail ? launch_tile<F8F8Tile256, wq_gemm_f8f8_256<true, false>>(p, dim3((unsigned)units), s)
-                      : launch_tile<F8F8Tile256, wq_gemm_f8f8_256<false, false>>(p, dim3((unsigned)units), s);
-    case F8F8_128X256:
-        return stream ? tail ? launch_tile<F8F8Tile128x256, wq_gemm_f8f8_128x256<true, true>>(p, dim3((unsigned)std::min(units, 256L)), s)
-                             : launch_tile<F8F8Tile128x256, wq_gemm_f8f8_128x256<false, true>>(p, dim3((unsigned)std::min(units, 256L)), s)
-               : tail ? launch_tile<F8F8Tile128x256, wq_gemm_f8f8_128x256<true, false>>(p, dim3((unsigned)units), s)
-                      : launch_tile<F8F8Tile128x256, wq_gemm_f8f8_128x256<false, false>>(p, dim3((unsigned)units), s);
-    case F8F8_128:
-        return stream ? tail ? launch_tile<F8F8Tile128, wq_gemm_f8f8_128<true, true>>(p, dim3((unsigned)std::min(units, 512L)), s)
-                             : launch_tile<F8F8Tile128, wq_gemm_f8f8_128<false, true>>(p, dim3((unsigned)std::min(units, 512L)), s)
-               : tail ? launch_tile<F8F8Tile128, wq_gemm_f8f8_128<true, false>>(p, dim3((unsigned)units), s)
-                      : launch_tile<F8F8Tile128, wq_gemm_f8f8_128<false, false>>(p, dim3((unsigned)units), s);
+        F8F8_TILE_CASE(F8F8_256, F8F8Tile256, wq_gemm_f8f8_256, 256)
+        F8F8_TILE_CASE(F8F8_128X256, F8F8Tile128x256, wq_gemm_f8f8_128x256, 256)
+        F8F8_TILE_CASE(F8F8_128, F8F8Tile128, wq_gemm_f8f8_128, 512)
+        F8F8_TILE_CASE(F8F8_128_W8, F8F8Tile128W8, wq_gemm_f8f8_128_w8, 256)
+        F8F8_TILE_CASE(F8F8_64, F8F8Tile64, wq_gemm_f8f8_64, 512)
+        F8F8_TILE_CASE(F8F8_64X64, F8F8Tile64x64, wq_gemm_f8f8_64x64, 768)
+#undef F8F8_TILE_CASE
     case F8F8_SKINNY_DIRECT: hipLaunchKernelGGL((wq_gemm_f8f8_skinny_direct<1, 1, 16, 2>), strips, dim3(1024), 0, s, p); return WQ_OK;
     case F8F8_SKINNY_16: return launch_tile<F8F8Skinny<1, 1, 8, 2>, wq_gemm_f8f8_skinny<1, 1, 8, 2>>(p, strips, s);
     case F8F8_SKINNY_16X64: return launch_tile<F8F8Skinny<1, 4, 4, 2>, wq_gemm_f8f8_skinny<1, 4, 4, 2>>(p, strips, s);

@@ -205,40 +205,65 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
         return fail(WQ_ERR_UNSUPPORTED, "fp8 weights: WQ_FLAG_TILE_* needs 16-byte aligned rows and K a multiple of 16 above 384");
     // Few rows: one pass over the weights, K dealt to the waves of a workgroup.  Up to 4 rows straight to registers; through LDS
     // beyond, 64 columns a workgroup once that leaves more than a hundred of them (the activations are read once per workgroup).
-    // With 17 .. 32 rows the tile kernel is as fast from 8192 columns up (11008 x 4096: 17.8 against 17.9 us; 28672 x 8192: 42 against
-    // 60), and from 33 rows everywhere once it splits K (64 rows, 4096 x 11008: 19 against 27; 4096 x 4096: 15 against 13).
+    // With 17 .. 32 rows up to 8192 columns (32 rows, 4096 x 4096: 7.0 us, the best tile kernel 10.2; 4096 x 11008: 12.2 against 15.6;
+    // 5000 x 4112: 10.2 against 11.0), beyond them the tile kernels (11008 x 4096: 15.5 against 14.0), and so from 33 rows (64 rows,
+    // 4096 x 11008: 27 against 16.2; 4096 x 4096: 13 against 11.3).
     if(rows16 && !pinned && p->M <= (p->N <= 8192 ? 32 : 16) && p->N <= 1 << 25) // (64 work items per column: as above)
     {
         plan.f8f8  = p->M <= 4 ? wq::F8F8_SKINNY_DIRECT : p->M > 16 ? wq::F8F8_SKINNY_32 : p->N <= 8192 ? wq::F8F8_SKINNY_16 : wq::F8F8_SKINNY_16X64;
         plan.route = ROUTE_F8F8;
         return WQ_OK;
     }
-    // Tile kernels: the kernel and the number of K slices with the shortest estimate, in microseconds, fitted to 4 weight shapes x 13
-    // row counts x up to 5 slice counts of each kernel (the chosen one is within 10 % of the best measured at all of them): per
-    // workgroup a fixed part, then a time per K tile on the busiest CU (the 256-tile kernel's grows as the chip fills and the
-    // clock falls); slices write and re-read fp32 slabs and need a second kernel.
+    // Tile kernels: the kernel and the number of K slices with the shortest estimate, in microseconds.  Fitted to 6 weight shapes
+    // (1024 x 8192 .. 28672 x 8192) x 15 row counts (20 .. 4096) x up to 8 slice counts of each kernel, 1500 timings: the choice is on
+    // average 1.4 % and at most 16 % behind the best of them.  A K tile takes first + fill * (the filled part of the 256 CUs) with one
+    // workgroup per CU, more[j] with j + 2; a launch takes whole rounds of the workgroups that the chip holds, and no less than its
+    // bytes do; slices write and re-read fp32 slabs and need a second kernel.
+    struct Cost
+    {
+        int kernel, resident;
+        double fixed, first, fill, more[2];
+    };
+    static const Cost costs[] = {{wq::F8F8_ANY, 1, 8, 1.5, 0.1, {}},
+                                 {wq::F8F8_64X64, 3, 5.64, 0.258, 0.044, {0.432, 0.661}},
+                                 {wq::F8F8_64, 2, 7.18, 0.345, 0.030, {0.657}},
+                                 {wq::F8F8_128, 2, 7.91, 0.497, 0.057, {0.984}},
+                                 {wq::F8F8_128_W8, 1, 7.67, 0.402, 0.203, {}},
+                                 {wq::F8F8_128X256, 1, 7.38, 0.710, 0.268, {}},
+                                 {wq::F8F8_256, 1, 7.57, 1.257, 0.358, {}}};
     const int klen = plan.k_end - plan.k_begin, ktiles = (klen + 127) / 128;
+    const double floor = 7.2 + ((double)p->N * klen + (double)p->M * klen + 2.0 * p->M * p->N) / 8.1e6;
     double best    = 1e30;
     int slices     = plan.k_batch;
-    for(int kernel : {(int)wq::F8F8_ANY, (int)wq::F8F8_128, (int)wq::F8F8_128X256, (int)wq::F8F8_256})
+    for(const Cost& k : costs)
     {
-        if((kernel == wq::F8F8_ANY) == tiles || (pinned && pinned != (kernel == wq::F8F8_256 ? WQ_FLAG_TILE_256 : kernel == wq::F8F8_128 ? WQ_FLAG_TILE_128 : WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256)))
+        const int flags = k.kernel == wq::F8F8_256       ? WQ_FLAG_TILE_256
+                          : k.kernel == wq::F8F8_128X256 ? WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256
+                          : k.kernel >= wq::F8F8_128     ? WQ_FLAG_TILE_128
+                                                         : 0;
+        if((k.kernel == wq::F8F8_ANY) == tiles || (pinned && pinned != flags))
             continue;
-        const double grid = (double)((p->M - 1) / wq::f8f8_bm(kernel) + 1) * ((p->N - 1) / wq::f8f8_bn(kernel) + 1);
-        const bool may_split = !plan.partial && !pinned && have_workspace && grid < 1 << 16; // (work items along x)
-        for(int c = plan.k_batch; c <= (may_split ? 16 : plan.k_batch) && (c == plan.k_batch || ktiles / c >= 2); ++c)
+        const double grid = (double)((p->M - 1) / wq::f8f8_bm(k.kernel) + 1) * ((p->N - 1) / wq::f8f8_bn(k.kernel) + 1);
+        if(grid * plan.k_batch >= 1 << 23) // (work items along x)
+            continue;
+        const bool may_split = !plan.partial && !pinned && have_workspace && grid < 1 << 16;
+        for(int c : {1, 2, 3, 4, 6, 8, 12, 16}) // (a factor of what the caller fixed)
         {
-            const double wgs = grid * c, chain = std::ceil(wgs / 256) * ((ktiles + c - 1) / c);
-            double t = kernel == wq::F8F8_256       ? 8 + chain * (1.25 + 0.35 * std::min(1.0, wgs / 256))
-                       : kernel == wq::F8F8_128X256 ? 6 + chain * (0.75 + 0.2 * std::min(1.0, wgs / 256))
-                       : kernel == wq::F8F8_128     ? 5 + chain * (wgs > 256 ? 0.55 : 0.62)
-                                                    : 5 + chain * 1.6;
+            if(c > 1 && (!may_split || ktiles / c < 2))
+                break;
+            const double units = grid * c * plan.k_batch, round = 256.0 * k.resident;
+            auto tile_time = [&](double n) { return n <= 256 ? k.first + k.fill * n / 256 : k.more[(int)std::ceil(n / 256) - 2]; };
+            const double rounds = std::floor(units / round), rest = units - rounds * round;
+            const double chain  = (ktiles + c * plan.k_batch - 1) / (c * plan.k_batch);
+            double t = std::max(floor, k.fixed + chain * (rounds * tile_time(round) + (rest > 0 ? tile_time(rest) : 0)));
             if(c > 1)
-                t += 3.5 + c * (double)p->M * p->N * 8 / 6e6;
+                t += 1.89 + c * (double)p->M * p->N * 1.31e-6;
             if(t < best)
-                best = t, plan.f8f8 = kernel, slices = c;
+                best = t, plan.f8f8 = k.kernel, slices = c * plan.k_batch;
         }
     }
+    if(best == 1e30)
+        return fail(WQ_ERR_UNSUPPORTED, "too many tiles for one launch");
     if(!plan.partial && slices > 1)
     {
         const int per = wqgemm_splitk_kread(klen, slices, 128);
@@ -781,9 +806,9 @@ void f16_image_of_a(const wqgemm_problem* p, void* workspace, hipStream_t s, wq:
 // Columns of a split-K slab of the fp8 x fp8 kernels: whole groups of four, so that odd N splits like any other.
 int f8f8_ld_part(const wqgemm_problem* p) { return (p->N + 3) & ~3; }
 
-const char* const kF8F8Names[] = {"wq_gemm_f8f8_any",    "wq_gemm_f8f8_128",           "wq_gemm_f8f8_128x256", "wq_gemm_f8f8_256",
+const char* const kF8F8Names[] = {"wq_gemm_f8f8_any", "wq_gemm_f8f8_64x64", "wq_gemm_f8f8_64", "wq_gemm_f8f8_128", "wq_gemm_f8f8_128_w8", "wq_gemm_f8f8_128x256", "wq_gemm_f8f8_256",
                                   "wq_gemm_f8f8_skinny_direct", "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny"};
-const char* const kF8F8Instances[] = {"256, 128, 128, 128, AnyAlignment", "256, 128, 128, 128, LdsDma", "512, 128, 256, 128, LdsDma", "512, 256, 256, 128, LdsDma",
+const char* const kF8F8Instances[] = {"256, 128, 128, 128, AnyAlignment", "256, 64, 64, 128, LdsDma", "256, 64, 128, 128, LdsDma", "256, 128, 128, 128, LdsDma", "512, 128, 128, 128, LdsDma", "512, 128, 256, 128, LdsDma", "512, 256, 256, 128, LdsDma",
                                       "1024, 16, 16, 128, WavesSplitK, Direct", "512, 16, 16, 128, WavesSplitK, LdsDma",
                                       "256, 16, 64, 128, WavesSplitK, LdsDma", "512, 32, 16, 128, WavesSplitK, LdsDma"};
 
