@@ -162,7 +162,10 @@ def _launch_on(x, call, *args):
 
 
 def _fp8_linear(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype):
-    _same_device("fp8_linear", x, x_scale=x_scale, weight=weight, weight_scale=weight_scale, bias=bias)
+    index = x.get_device()
+    if (index < 0 or x_scale.get_device() != index or weight.get_device() != index or weight_scale.get_device() != index or
+            (bias is not None and bias.get_device() != index)):
+        _same_device("fp8_linear", x, x_scale=x_scale, weight=weight, weight_scale=weight_scale, bias=bias)
     if x.dtype != _F8 or weight.dtype != _F8:
         raise TypeError(f"x and weight must be float8_e4m3fn, got {x.dtype} and {weight.dtype}")
     if x_scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
