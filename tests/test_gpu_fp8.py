@@ -126,6 +126,30 @@ def test_sizes(m, n, k, dtype):
     check_exact(launch(P, torch.bfloat16 if k > 4000 else dtype), P)  # (sums up to 64 * K would leave fp16's range)
 
 
+@pytest.mark.parametrize("kernel,m,n,k", [
+    ("64x64", 40, 520, 2048), ("64x64", 100, 1040, 656), ("64x64", 257, 514, 1040), ("64", 520, 6000, 656), ("64", 400, 8191, 656),
+    ("128_w8", 640, 5000, 1024), ("128_w8", 600, 4999, 1040), ("128", 400, 8192, 1024), ("128", 390, 8190, 1040), ("128x256", 512, 11008, 656),
+    ("128x256", 500, 11003, 656), ("256", 768, 11008, 656), ("256", 760, 11001, 1040)])
+def test_every_tile_kernel(kernel, m, n, k):
+    P = problem(m, n, k, m + n + k, exact=True)
+    p = capi.f8_problem(P["a_ptr"], P["sa"].data_ptr(), P["b_ptr"], P["sb"].data_ptr(), P["a_ptr"], m, n, k, scale_block=P["block"])
+    assert capi.kernel_name(p) == "wq_gemm_f8f8_" + kernel
+    check_exact(launch(P, torch.bfloat16), P)
+    P = problem(m, n, k, m + n)
+    check(launch(P, torch.float16), P, torch.float16)
+
+
+@pytest.mark.parametrize("flags", [capi.FLAG_TILE_128, capi.FLAG_TILE_256, capi.FLAG_TILE_128 | capi.FLAG_TILE_256])
+@pytest.mark.parametrize("m,n,k", [(5, 8, 400), (300, 700, 1040), (513, 1030, 528), (4300, 4616, 656)])
+@pytest.mark.parametrize("act", ["none", "add_fastgelu"])
+def test_chosen_tile_sizes(flags, m, n, k, act):
+    """The tile size fixed by the caller; the largest is more tiles than resident workgroups of every kernel."""
+    P = problem(m, n, k, m + k)
+    P["sa"] *= 0.05
+    bias = torch.randn(n, device="cuda", generator=gen(5)).bfloat16() if act != "none" else None
+    check(launch(P, torch.bfloat16, bias=bias, act=act, flags=flags | capi.FLAG_BF16_RTN), P, torch.bfloat16, bias, act)
+
+
 @pytest.mark.parametrize("m,n,k", [(3, 257, 384), (40, 512, 640), (150, 384, 272), (300, 515, 1024)])
 @pytest.mark.parametrize("act", ["fastgelu", "add", "add_fastgelu"])
 def test_epilogues(m, n, k, act):
