@@ -6,6 +6,8 @@ PyTorch supplies device memory and the stream; the arithmetic is the HIP kernels
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import capi
@@ -121,6 +123,15 @@ _INT_MAX = 2 ** 31 - 1
 # (small calls are bound by the host: what follows asks each tensor as little as it can.  The raw stream handle takes 0.07 us
 # where torch.cuda.current_stream(...).cuda_stream takes 1.8)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+# (a call with nothing to copy, convert or refuse goes the short way, in C++: csrc/torch_front.cpp.  It answers None to the others)
+try:
+    from . import _torch_front
+except ImportError as e:
+    raise ImportError(f"composable_kernel_amd/_torch_front.so cannot be loaded ({e}): build it with `make -C composable_kernel_amd/csrc`") from e
+_torch_front.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (capi.lib.wqgemm_quantize, capi.lib.wqgemm_launch,
+                                                                   capi.lib.wqgemm_workspace_bytes, capi.lib.wqgemm_last_error)), capi.WqError)
 
 
 def _needs_gradients(name):
@@ -327,6 +338,10 @@ def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
     float32; bias (N,) of out_dtype, with the "add" / "add_fastgelu" epilogues ("none" and "fastgelu" go without).  Sums in
     fp32, one rounding to nearest even into out_dtype (float16 or bfloat16).  Any N and K; fastest where K is a multiple of 16
     and the rows are 16-byte aligned."""
+    if not torch.compiler.is_compiling() and x.is_cuda and epilogue in _EPILOGUES:
+        y = _torch_front.linear(x, x_scale, weight, weight_scale, bias, _EPILOGUES[epilogue], out_dtype, _raw_stream(x.get_device()))
+        if y is not None:
+            return y
     if torch.is_grad_enabled() and (x.requires_grad or x_scale.requires_grad or weight.requires_grad or weight_scale.requires_grad or
                                     (bias is not None and bias.requires_grad)):
         _needs_gradients("fp8_linear")
@@ -339,6 +354,10 @@ def quantize_fp8(x: torch.Tensor, group_k: int = 128) -> tuple[torch.Tensor, tor
     """x (..., K) float16 / bfloat16 -> (q, scale) with x ~ q * scale: q float8_e4m3fn of x's shape, scale float32 of shape
     (..., ceil(K / 128)), one per 128 consecutive values, or (..., 1) for group_k = 0.  scale = max|x| / 448 of its group
     (groups below 1e-12: as if the maximum were that); a NaN makes its whole group NaN."""
+    if not torch.compiler.is_compiling() and x.is_cuda:
+        r = _torch_front.quantized(capi.QUANT_ROWS, x, None, None, 0, 0.0, group_k, _raw_stream(x.get_device()))
+        if r is not None:
+            return r[:2]
     if torch.is_grad_enabled() and x.requires_grad:
         _needs_gradients("quantize_fp8")
     return _quantize_fp8_op(x, group_k) if torch.compiler.is_compiling() else _quantize_fp8(x, group_k)
@@ -348,6 +367,10 @@ def gated_fp8(gate: torch.Tensor, up: torch.Tensor, activation: str = "silu",
               group_k: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
     """quantize_fp8 of activation(gate) * up, evaluated in fp32 (activation "silu" or "fastgelu").  gate and up may be the
     two halves of one projection's output (row-strided views are read in place)."""
+    if not torch.compiler.is_compiling() and gate.is_cuda and activation in _ACTIVATIONS:
+        r = _torch_front.quantized(capi.QUANT_GATED, gate, up, None, _ACTIVATIONS[activation], 0.0, group_k, _raw_stream(gate.get_device()))
+        if r is not None:
+            return r[:2]
     if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
         _needs_gradients("gated_fp8")
     return (_gated_fp8_op if torch.compiler.is_compiling() else _gated_fp8)(gate, up, activation, group_k)
@@ -357,6 +380,10 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
                 group_k: int = 128) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
     """h = x + residual; returns (q, scale) = quantize_fp8 of h / sqrt(mean(h^2) + eps) * weight, and h rounded to x's dtype
     (None without a residual).  The norm sees h unrounded; weight (K,) has x's dtype or float32."""
+    if not torch.compiler.is_compiling() and x.is_cuda:
+        r = _torch_front.quantized(capi.QUANT_RMSNORM, x, residual, weight, 0, eps, group_k, _raw_stream(x.get_device()))
+        if r is not None:
+            return r
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         _needs_gradients("rmsnorm_fp8")
     if torch.compiler.is_compiling():

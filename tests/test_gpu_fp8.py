@@ -3,6 +3,7 @@ import math
 import os
 import subprocess
 import sys
+import threading
 
 import numpy as np
 import pytest
@@ -536,6 +537,62 @@ def test_empty_batches_and_column_views():
     wt = layer.weight.t().contiguous().t()
     q, s = torch_ops.quantize_fp8(one)
     assert torch.equal(torch_ops.fp8_linear(q, s, wt, layer.weight_scale), layer((q, s)))
+
+
+@pytest.mark.parametrize("shape", [(1, 4096), (5, 300), (2, 3, 640), (700,)])
+@pytest.mark.parametrize("group", [128, 0])
+def test_both_ways_into_the_library(shape, group):
+    """What plain calls return (they go through C++) is what the long way returns, bit for bit; its dtypes, shapes and strides too."""
+    k = shape[-1]
+    x, r = (torch.randn(shape, device="cuda", generator=gen(s)).bfloat16() for s in (1, 2))
+    w = torch.rand(k, device="cuda", generator=gen(3))
+    wide = torch.cat([x, r], -1)
+    f8 = torch.float8_e4m3fn
+    for short, long in [(torch_ops.quantize_fp8(x, group), torch_ops._quantize_fp8(x, group)),
+                        (torch_ops.gated_fp8(x, r, "fastgelu", group), torch_ops._gated_fp8(x, r, "fastgelu", group)),
+                        (torch_ops.gated_fp8(wide[..., :k], wide[..., k:], "silu", group), torch_ops._gated_fp8(x, r, "silu", group)),
+                        (torch_ops.rmsnorm_fp8(x, w, r, 1e-5, group), torch_ops._rmsnorm_fp8(x, w, r, 1e-5, group)),
+                        (torch_ops.rmsnorm_fp8(x, w.bfloat16(), None, 0, group), torch_ops._rmsnorm_fp8(x, w.bfloat16(), None, 0, group))]:
+        assert len(short) == len(long)
+        for a, b in zip(short, long):
+            assert (a is None) == (b is None)
+            if a is not None:
+                assert a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride() and torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    q, s = torch_ops.quantize_fp8(x)
+    weight = torch.randn(200, k, device="cuda", generator=gen(4)).to(f8)
+    ws, bias = torch.rand(2, -(-k // 128), device="cuda", generator=gen(5)), torch.randn(200, device="cuda", generator=gen(6)).half()
+    for args in [(None, "none", torch.bfloat16), (None, "fastgelu", torch.float16), (bias, "add", torch.float16)]:
+        a, b = torch_ops.fp8_linear(q, s, weight, ws, *args), torch_ops._fp8_linear(q, s, weight, ws, *args)
+        assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
+
+
+def test_two_threads():
+    """Each on its own stream, with its own errors."""
+    x = torch.randn(300, 1024, device="cuda").bfloat16()
+    want = [t.clone() for t in torch_ops.quantize_fp8(x)]
+    bad = []
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(100):
+                q, s = torch_ops.quantize_fp8(x)
+                try:
+                    torch_ops.quantize_fp8(x, 64 + i)
+                    bad.append("accepted")
+                except ValueError as e:
+                    if str(64 + i) not in str(e):
+                        bad.append(str(e))
+            torch.cuda.current_stream().synchronize()
+            if not (torch.equal(q.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(s, want[1])):
+                bad.append("differs")
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad[:3]
 
 
 def test_refusals_of_the_front_end():
