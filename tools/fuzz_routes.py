@@ -316,20 +316,88 @@ def one_case_ab(rng) -> dict:
     return desc
 
 
+def one_case_f8f8(rng) -> dict:
+    """fp8 x fp8 with block-wise scales: any M, N, K, strides, alignment, block shape, epilogue, tile size and K split, whatever kernel
+    the dispatcher picks against the general kernel.  Small integers and power-of-two scales keep every sum exact."""
+    pick = lambda *v: int(rng.choice(v))  # noqa: E731
+    M = pick(1, 3, 4, 5, 16, 17, 32, 33, 64, 65, 100, 128, 200, 256, 257, 400, 600, 1024, 2048) if rng.integers(0, 3) else int(rng.integers(1, 1500))
+    N = pick(128, 256, 512, 1024, 2048, 4096) if rng.integers(0, 2) else int(rng.integers(1, 5000))
+    K = pick(128, 256, 384, 400, 512, 640, 1024, 2048, 4096) if rng.integers(0, 2) else int(rng.integers(1, 4200))
+    if rng.integers(0, 2):
+        K = -(-K // 16) * 16
+    fnuz = [bool(v) for v in rng.integers(0, 5, 2) == 0]
+    bf, rtn = bool(rng.integers(0, 2)), bool(rng.integers(0, 2))
+    bm, bn, bk = pick(1, 1, 128, 7, 64), pick(128, 128, 32, 96, 48), pick(128, 128, 128, 128, 64)
+    off = [pick(0, 0, 0, 1, 16), pick(0, 0, 0, 3, 32)]
+    lda, ldb, ldc = K + pick(0, 0, 16, 128, 5), K + pick(0, 0, 16, 64, 3), N + pick(0, 0, 8, 3)
+    epi = pick(capi.EPI_PASSTHROUGH, capi.EPI_PASSTHROUGH, capi.EPI_FASTGELU, capi.EPI_ADD, capi.EPI_ADD_FASTGELU)
+    k_batch = pick(2, 3, 5) if rng.integers(0, 5) == 0 and N % 4 == 0 and ldc % 4 == 0 else 1
+    pin = pick(0, 0, 0, capi.FLAG_TILE_128, capi.FLAG_TILE_256, capi.FLAG_TILE_128 | capi.FLAG_TILE_256)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(int(rng.integers(0, 1 << 30)))
+    ptr = []
+    keep = []
+    for rows, ld, o, z in ((M, lda, off[0], fnuz[0]), (N, ldb, off[1], fnuz[1])):
+        lut = torch.zeros(9, dtype=torch.uint8)
+        for v, code in (E4M3FNUZ if z else E4M3FN).items():
+            lut[v + 4] = code
+        t = torch.full((o + rows * ld + 64,), 0x7F, dtype=torch.uint8, device="cuda")
+        t[o:o + rows * ld].view(rows, ld)[:, :K] = lut.cuda()[torch.randint(0, 9, (rows, K), device="cuda", generator=g)]
+        keep.append(t)
+        ptr.append(t.data_ptr() + o)
+    kb = -(-K // bk)
+    ld_s = [kb + pick(0, 0, 3), kb + pick(0, 0, 5)]
+    sa = torch.exp2(torch.randint(-6, -2, (-(-M // bm), ld_s[0]), device="cuda", generator=g).float())
+    sb = torch.exp2(torch.randint(-5, 0, (-(-N // bn), ld_s[1]), device="cuda", generator=g).float())
+    dtype = torch.bfloat16 if bf else torch.float16
+    d0 = torch.randint(-8, 9, (N,), device="cuda", generator=g).to(dtype)
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def run(flags, split, workspace):
+        c = torch.full((M + 300, ldc), -77.0, dtype=dtype, device="cuda")
+        p = capi.f8_problem(ptr[0], sa.data_ptr(), ptr[1], sb.data_ptr(), c.data_ptr(), M, N, K, lda=lda, ldb=ldb, ldc=ldc,
+                            a_dtype=capi.F8_FNUZ if fnuz[0] else capi.F8_E4M3FN, b_dtype=capi.F8_FNUZ if fnuz[1] else capi.F8_E4M3FN,
+                            c_dtype=capi.BF16 if bf else capi.F16, epilogue=epi, d0=d0.data_ptr(), k_batch=split, scale_block=(bm, bn, bk),
+                            ld_a_scale=ld_s[0], ld_b_scale=ld_s[1], flags=flags | (capi.FLAG_BF16_RTN if rtn else 0) | capi.FLAG_F8_NO_SPECIALS)
+        if not capi.is_supported(p):
+            return None, capi.lib.wqgemm_last_error().decode(), 1
+        n = capi.workspace_bytes(p) if workspace else 0
+        ws = torch.full((n + 64,), 0xFF, dtype=torch.uint8, device="cuda")
+        text = capi.type_string(p) if workspace else "KBatch1>"
+        capi.launch(p, ws.data_ptr() if n else None, stream)
+        torch.cuda.synchronize()
+        assert bool((ws[n:] == 0xFF).all())
+        return c, capi.kernel_name(p).split("+")[0], int(text.rsplit("KBatch", 1)[1].rstrip(">")) if "KBatch" in text else 1
+
+    ref, _, _ = run(capi.FLAG_GENERIC, 1, False)
+    got, kernel, slices = run(pin, k_batch, k_batch > 1 or bool(rng.integers(0, 4)))
+    if got is None:
+        return {"skipped": kernel}
+    desc = dict(fmt="f8xf8", fnuz=fnuz, bf16=bf, rtn=rtn, M=M, N=N, K=K, lda=lda, ldb=ldb, ldc=ldc, offsets=off, block=[bm, bn, bk], ld_scales=ld_s,
+                epilogue=epi, k_batch=slices, pinned=pin, kernel=kernel)
+    desc["equal"] = bool(torch.equal(got[:M, :N], ref[:M, :N]))
+    desc["padding_untouched"] = bool((got[:M, N:] == -77).all() and (got[M:] == -77).all())
+    if not desc["equal"]:
+        bad = torch.nonzero(got[:M, :N] != ref[:M, :N])
+        desc["mismatches"], (i, j) = len(bad), bad[0].tolist() if len(bad) else (0, 0)
+        desc["first"] = [i, j, float(got[i, j]), float(ref[i, j])]
+    return desc
+
+
 def main() -> int:
     ap = argparse.ArgumentParser()
     ap.add_argument("--seconds", type=float, default=120)
     ap.add_argument("--seed", type=int, default=1)
     ap.add_argument("--out", default=None)
-    ap.add_argument("--family", choices=("fp", "i8", "f8", "ab"), default="fp",
+    ap.add_argument("--family", choices=("fp", "i8", "f8", "ab", "f8f8"), default="fp",
                     help="fp: fp16/bf16 x int4/int8; i8: int8 x int8 requantised; f8: fp8 x int4 MultiplyMultiply; "
-                         "ab: fp8 x int4/int8 with block-wise scales of both operands")
+                         "ab: fp8 x int4/int8 with block-wise scales of both operands; f8f8: fp8 x fp8 with them")
     args = ap.parse_args()
     rng = np.random.default_rng(args.seed)
     t0 = time.time()
     kernels, failures, skipped, n = {}, [], 0, 0
     while time.time() - t0 < args.seconds:
-        d = {"fp": one_case, "i8": one_case_i8, "f8": one_case_f8, "ab": one_case_ab}[args.family](rng)
+        d = {"fp": one_case, "i8": one_case_i8, "f8": one_case_f8, "ab": one_case_ab, "f8f8": one_case_f8f8}[args.family](rng)
         if "skipped" in d:
             skipped += 1
             continue
