@@ -14,15 +14,17 @@ enum F8F8Kernel
     F8F8_128_W8,  // 128 x 128, eight waves, one workgroup per CU
     F8F8_128X256, // 128 x 256, eight waves
     F8F8_256,     // 256 x 256, eight waves
-    F8F8_SKINNY_DIRECT, // M <= 16: 16 columns, sixteen waves, weights straight to registers
+    F8F8_SKINNY_DIRECT, // M <= 16 (used up to 4): 16 columns, sixteen waves, weights straight to registers
     F8F8_SKINNY_16,     // M <= 16: 16 columns, eight waves
+    F8F8_SKINNY_16X32,  // M <= 16: 32 columns, eight waves
     F8F8_SKINNY_16X64,  // M <= 16: 64 columns, four waves
-    F8F8_SKINNY_32      // M <= 32: 16 columns, eight waves
+    F8F8_SKINNY_32,     // M <= 32: 16 columns, eight waves
+    F8F8_SKINNY_32X32   // M <= 32: 32 columns, eight waves
 };
 constexpr int f8f8_bm(int kernel) { return kernel == F8F8_256 ? 256 : kernel == F8F8_64 || kernel == F8F8_64X64 ? 64 : 128; }
 constexpr int f8f8_bn(int kernel)
 {
-    return kernel == F8F8_64X64 ? 64 : kernel <= F8F8_128_W8 ? 128 : kernel <= F8F8_256 ? 256 : kernel == F8F8_SKINNY_16X64 ? 64 : 16;
+    return kernel == F8F8_64X64 ? 64 : kernel <= F8F8_128_W8 ? 128 : kernel <= F8F8_256 ? 256 : kernel == F8F8_SKINNY_16X64 ? 64 : kernel == F8F8_SKINNY_16X32 || kernel == F8F8_SKINNY_32X32 ? 32 : 16;
 }
 
 struct F8F8Params

@@ -665,17 +665,21 @@ __global__ __launch_bounds__(256, 2) void wq_gemm_f8f8_64(const F8F8Params p) { 
 // ---------------------------------------------------------------------------------------------
 // Few rows (M <= 16 MT): one pass over the weights, bound by their stream.  A workgroup owns 16 NB columns; its waves deal the K
 // tiles among themselves (tile i WAVES + wave: the workgroup reads runs of WAVES cache lines of every column) and add their sums
-// through LDS at the end, in the order of the waves: no second kernel, no workspace.  Rows past M and columns past N lie outside
-// the resources and read as zeros without memory accesses, and so does what lies past the end of the last K tile (K a multiple of
-// 16).  Two forms:
+// through LDS at the end, in the order of the waves: no second kernel, no workspace.  Workgroups start at different K tiles: all of
+// them at the same k of columns a power of two apart ask few of the memory's channels at a time (8192 x 8192 at M = 16 with 32
+// columns a workgroup 20.7 us, turned 14.8; 4096 x 11008 15.5 and 13.5).  Rows past M and columns past N lie outside the resources and
+// read as zeros without memory accesses, and so does what lies past the end of the last K tile (K a multiple of 16).  Two forms:
 //   * _direct: operands straight to the registers of the MFMA, P tiles at a time.  The vector cache takes such fragment-shaped
 //     loads at one access of 16 bytes per lane: 16 bytes a cycle and CU, 8.6 TB/s on the chip, more than HBM delivers, but
-//     activations of 16 rows double the accesses.  Least latency: 4096 x 4096 at M = 1 6.5 us (7.2 through LDS), 28672 x 8192
-//     37.9 us = 6.2 TB/s (50.7);
+//     activations of 16 rows double the accesses.  Least latency: 4096 x 4096 at M = 1 6.5 us (6.9 through LDS), 28672 x 8192
+//     38.3 us = 6.1 TB/s (43.1).  Turned only where a workgroup has a CU of its own (4096 x 11008 14.0 -> 11.8; 28672 x 8192
+//     would be 39.8);
 //   * through LDS: LDS-DMA takes 64 bytes an access; every wave fills a ring of its own, D tiles ahead, so there is no barrier in
-//     the loop.  4096 x 4096 at M = 16 8.0 us (direct 8.4), 4096 x 11008 15.1 (17.0), 28672 x 8192, 64 columns a
-//     workgroup, 45.7 (69.0).
+//     the loop.  At M = 16: 4096 x 4096 7.8 us (direct 8.4); 28672 x 8192, 64 columns a workgroup, 44.5 (68.7).
+// (Weights not in the last-level cache: several copies in turn.)
 // ---------------------------------------------------------------------------------------------
+constexpr unsigned kF8F8Turn = 11; // (3, 5, 13 and 21 within 3 % of it)
+
 template <int MT, int NB, int WAVES, int P>
 __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny_direct(const F8F8Params p)
 {
@@ -686,6 +690,8 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny_direct(const F
     const int n0 = blockIdx.x * (NB * 16), z = blockIdx.y;
     const int k0 = p.k_begin + z * p.k_per_z, k1 = min(p.k_end, k0 + p.k_per_z);
     const int ntiles = (k1 - k0 + 127) >> 7; // (empty slices: <= 0)
+    const int turn   = ntiles > 0 && gridDim.x <= 256 ? (int)(blockIdx.x * kF8F8Turn % (unsigned)ntiles) : 0;
+    auto turned      = [&](int tile) __attribute__((always_inline)) { return tile + turn < ntiles ? tile + turn : tile + turn - ntiles; };
     constexpr uint32_t OUT = 0x80000000u;
 
     const long a_bytes = (long)(p.M - 1) * p.lda + p.K, b_bytes = (long)(p.N - n0 - 1) * p.ldb + p.K;
@@ -727,7 +733,7 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny_direct(const F
         for(int i = 0; i < P; ++i)
             if(i < tiles)
             {
-                const int tile = first + i * WAVES;
+                const int tile = turned(first + i * WAVES);
 #pragma unroll
                 for(int nb = 0; nb < NB; ++nb)
                     w[i][nb] = load(b_rsrc, b_lane, (uint32_t)(nb * 16) * (uint32_t)p.ldb, tile);
@@ -742,7 +748,7 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny_direct(const F
         for(int i = 0; i < P; ++i)
             if(i < tiles)
             {
-                const int tile = first + i * WAVES;
+                const int tile = turned(first + i * WAVES);
 #pragma unroll
                 for(int nb = 0; nb < NB; ++nb)
                 {
@@ -802,6 +808,8 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny(const F8F8Para
     const int k0 = p.k_begin + z * p.k_per_z, k1 = min(p.k_end, k0 + p.k_per_z);
     const int ntiles = (k1 - k0 + 127) >> 7; // (empty slices: <= 0)
     const int mine   = ntiles > wave ? (ntiles - wave + WAVES - 1) / WAVES : 0;
+    const int turn   = ntiles > 0 ? (int)(blockIdx.x * kF8F8Turn % (unsigned)ntiles) : 0;
+    auto turned      = [&](int tile) __attribute__((always_inline)) { return tile + turn < ntiles ? tile + turn : tile + turn - ntiles; };
     constexpr uint32_t OUT = 0x80000000u;
 
     auto resource = [](const void* base, long bytes) __attribute__((always_inline)) {
@@ -833,12 +841,12 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny(const F8F8Para
     uint8_t* ring = lds + wave * (D * T::SLOT);
     // (tiles past the wave's last one: scales of its last, pieces of zeros without a memory access)
     auto fetch = [&](int i, int j) __attribute__((always_inline)) {
-        const int tile = wave + j * WAVES, known = min(tile, max(ntiles - 1, 0));
+        const int step = wave + j * WAVES, tile = turned(step), known = turned(min(step, max(ntiles - 1, 0)));
 #pragma unroll
         for(int mt = 0; mt < MT; ++mt)
             ra[i][mt] = sa[mt][known];
         __builtin_amdgcn_sched_barrier(0); // (issue order is part of the vmcnt arithmetic)
-        const bool last = tile == ntiles - 1, there = tile < ntiles;
+        const bool last = tile == ntiles - 1, there = step < ntiles;
         const __amdgpu_buffer_rsrc_t wr = there ? b_rsrc : null_rsrc, ar = there ? a_rsrc : null_rsrc;
         const uint32_t w_off = last && past ? OUT : b_lane, x_off = last && past ? OUT : a_lane, soff = (uint32_t)(k0 + tile * 128);
 #pragma unroll
@@ -862,7 +870,7 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny(const F8F8Para
         for(int i = 0; i < D; ++i)
             if(j + i < mine)
             {
-                const int tile = wave + (j + i) * WAVES;
+                const int tile = turned(wave + (j + i) * WAVES);
                 wait_vmcnt<(D - 1) * T::OPS>();
                 __builtin_amdgcn_sched_barrier(0);
                 i8v_t w[NB], a[MT];

@@ -60,6 +60,8 @@ int launch_f8f8(int kernel, const F8F8Params& p, hipStream_t s)
     case F8F8_SKINNY_DIRECT: hipLaunchKernelGGL((wq_gemm_f8f8_skinny_direct<1, 1, 16, 2>), strips, dim3(1024), 0, s, p); return WQ_OK;
     case F8F8_SKINNY_16: return launch_tile<F8F8Skinny<1, 1, 8, 2>, wq_gemm_f8f8_skinny<1, 1, 8, 2>>(p, strips, s);
     case F8F8_SKINNY_16X64: return launch_tile<F8F8Skinny<1, 4, 4, 2>, wq_gemm_f8f8_skinny<1, 4, 4, 2>>(p, strips, s);
+    case F8F8_SKINNY_16X32: return launch_tile<F8F8Skinny<1, 2, 8, 1>, wq_gemm_f8f8_skinny<1, 2, 8, 1>>(p, strips, s);
+    case F8F8_SKINNY_32X32: return launch_tile<F8F8Skinny<2, 2, 8, 1>, wq_gemm_f8f8_skinny<2, 2, 8, 1>>(p, strips, s);
     case F8F8_SKINNY_32: return launch_tile<F8F8Skinny<2, 1, 8, 1>, wq_gemm_f8f8_skinny<2, 1, 8, 1>>(p, strips, s);
     default:
         hipLaunchKernelGGL(wq_gemm_f8f8_any, dim3((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.slices), dim3(256), 0, s, p);

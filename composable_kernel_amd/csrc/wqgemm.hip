@@ -203,14 +203,18 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
     const int pinned = p->flags & (WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256);
     if(pinned && !tiles)
         return fail(WQ_ERR_UNSUPPORTED, "fp8 weights: WQ_FLAG_TILE_* needs 16-byte aligned rows and K a multiple of 16 above 384");
-    // Few rows: one pass over the weights, K dealt to the waves of a workgroup.  Up to 4 rows straight to registers; through LDS
-    // beyond, 64 columns a workgroup once that leaves more than a hundred of them (the activations are read once per workgroup).
-    // With 17 .. 32 rows up to 8192 columns (32 rows, 4096 x 4096: 7.0 us, the best tile kernel 10.2; 4096 x 11008: 12.2 against 15.6;
-    // 5000 x 4112: 10.2 against 11.0), beyond them the tile kernels (11008 x 4096: 15.5 against 14.0), and so from 33 rows (64 rows,
-    // 4096 x 11008: 27 against 16.2; 4096 x 4096: 13 against 11.3).
+    // Few rows: one pass over the weights, K dealt to the waves of a workgroup.  16 columns a workgroup as long as that is at most one
+    // per CU, 32 up to 8192 columns (the activations are read once per workgroup; 5000 x 4096 at M = 16: 8.5 us, 16 columns 10.9),
+    // 64 beyond (28672 x 8192: 44.5; 32 columns 47.4).  Straight to registers with up to 4 rows in the first range (4096 x 4096 at
+    // M = 1: 6.5, through LDS 6.9) and up to 2 in the last (28672 x 8192 at M = 1: 38.3 against 43.1, at M = 4: 45.6 against 43.2).
+    // With 17 .. 32 rows up to 8192 columns (32 rows, 4096 x 4096: 9.0, the best tile kernel 10.2; 5000 x 4096: 10.7), beyond them
+    // the tile kernels (28672 x 8192: 59 against 54), and so from 33 rows (64 rows, 4096 x 11008: 27 against 16.2).
     if(rows16 && !pinned && p->M <= (p->N <= 8192 ? 32 : 16) && p->N <= 1 << 25) // (64 work items per column: as above)
     {
-        plan.f8f8  = p->M <= 4 ? wq::F8F8_SKINNY_DIRECT : p->M > 16 ? wq::F8F8_SKINNY_32 : p->N <= 8192 ? wq::F8F8_SKINNY_16 : wq::F8F8_SKINNY_16X64;
+        const bool few = p->N <= 4096, many = p->N > 8192;
+        plan.f8f8      = (few && p->M <= 4) || (many && p->M <= 2) ? wq::F8F8_SKINNY_DIRECT
+                         : p->M > 16 ? (few ? wq::F8F8_SKINNY_32 : wq::F8F8_SKINNY_32X32)
+                         : few ? wq::F8F8_SKINNY_16 : many ? wq::F8F8_SKINNY_16X64 : wq::F8F8_SKINNY_16X32;
         plan.route = ROUTE_F8F8;
         return WQ_OK;
     }
@@ -807,10 +811,12 @@ void f16_image_of_a(const wqgemm_problem* p, void* workspace, hipStream_t s, wq:
 int f8f8_ld_part(const wqgemm_problem* p) { return (p->N + 3) & ~3; }
 
 const char* const kF8F8Names[] = {"wq_gemm_f8f8_any", "wq_gemm_f8f8_64x64", "wq_gemm_f8f8_64", "wq_gemm_f8f8_128", "wq_gemm_f8f8_128_w8", "wq_gemm_f8f8_128x256", "wq_gemm_f8f8_256",
-                                  "wq_gemm_f8f8_skinny_direct", "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny"};
+                                  "wq_gemm_f8f8_skinny_direct", "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny",
+                                  "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny"};
 const char* const kF8F8Instances[] = {"256, 128, 128, 128, AnyAlignment", "256, 64, 64, 128, LdsDma", "256, 64, 128, 128, LdsDma", "256, 128, 128, 128, LdsDma", "512, 128, 128, 128, LdsDma", "512, 128, 256, 128, LdsDma", "512, 256, 256, 128, LdsDma",
                                       "1024, 16, 16, 128, WavesSplitK, Direct", "512, 16, 16, 128, WavesSplitK, LdsDma",
-                                      "256, 16, 64, 128, WavesSplitK, LdsDma", "512, 32, 16, 128, WavesSplitK, LdsDma"};
+                                      "512, 16, 32, 128, WavesSplitK, LdsDma", "256, 16, 64, 128, WavesSplitK, LdsDma",
+                                      "512, 32, 16, 128, WavesSplitK, LdsDma", "512, 32, 32, 128, WavesSplitK, LdsDma"};
 
 wq::F8F8Params f8f8_params(const wqgemm_problem* p)
 {

@@ -127,6 +127,18 @@ def test_sizes(m, n, k, dtype):
     check_exact(launch(P, torch.bfloat16 if k > 4000 else dtype), P)  # (sums up to 64 * K would leave fp16's range)
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 400), (4, 4000, 3968), (3, 8200, 272), (2, 8321, 1040), (5, 4090, 2048), (16, 4104, 640), (9, 8192, 8192),
+                                   (12, 5001, 144), (16, 8208, 1936), (17, 4096, 2064), (32, 4100, 640), (25, 8190, 1168), (32, 8192, 4096)])
+def test_few_rows(m, n, k):
+    """Every kernel for few rows, with columns and rows past the edge and K tiles that do not fill the waves' turns."""
+    P = problem(m, n, k, m + n + k, exact=True)
+    p = capi.f8_problem(P["a_ptr"], P["sa"].data_ptr(), P["b_ptr"], P["sb"].data_ptr(), P["a_ptr"], m, n, k, scale_block=P["block"])
+    assert "skinny" in capi.kernel_name(p)
+    check_exact(launch(P, torch.bfloat16), P)
+    P = problem(m, n, k, m + n)
+    check(launch(P, torch.float16, k_batch=3 if n % 4 == 0 else 1), P, torch.float16)
+
+
 @pytest.mark.parametrize("kernel,m,n,k", [
     ("64x64", 40, 520, 2048), ("64x64", 100, 1040, 656), ("64x64", 257, 514, 1040), ("64", 520, 6000, 656), ("64", 400, 8191, 656),
     ("128_w8", 640, 5000, 1024), ("128_w8", 600, 4999, 1040), ("128", 400, 8192, 1024), ("128", 390, 8190, 1040), ("128x256", 512, 11008, 656),
