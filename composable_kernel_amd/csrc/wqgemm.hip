@@ -218,25 +218,25 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
         plan.route = ROUTE_F8F8;
         return WQ_OK;
     }
-    // Tile kernels: the kernel and the number of K slices with the shortest estimate, in microseconds.  Fitted to 6 weight shapes
-    // (1024 x 8192 .. 28672 x 8192) x 15 row counts (20 .. 4096) x up to 8 slice counts of each kernel, 1500 timings: the choice is on
-    // average 1.4 % and at most 16 % behind the best of them.  A K tile takes first + fill * (the filled part of the 256 CUs) with one
-    // workgroup per CU, more[j] with j + 2; a launch takes whole rounds of the workgroups that the chip holds, and no less than its
-    // bytes do; slices write and re-read fp32 slabs and need a second kernel.
+    // Tile kernels: the kernel and the number of K slices with the shortest estimate, in microseconds.  Fitted to 9 weight shapes
+    // (1024 x 8192 .. 28672 x 8192) x 13 to 15 row counts (20 .. 4096) x up to 8 slice counts of each kernel, 2700 timings with the weights
+    // in the last-level cache and out of it: the choice is on average 1 % and at most 15 % behind the best of them.  A K tile
+    // takes first + fill * (the filled part of the 256 CUs) with one workgroup per CU, more[j] with j + 2; a launch takes whole rounds of
+    // the workgroups that the chip holds; it hides behind its bytes, or they behind it, but for a corner (the fourth root); slices
+    // write and re-read fp32 slabs and need a second kernel.
     struct Cost
     {
         int kernel, resident;
         double fixed, first, fill, more[2];
     };
     static const Cost costs[] = {{wq::F8F8_ANY, 1, 8, 1.5, 0.1, {}},
-                                 {wq::F8F8_64X64, 3, 5.64, 0.258, 0.044, {0.432, 0.661}},
-                                 {wq::F8F8_64, 2, 7.18, 0.345, 0.030, {0.657}},
-                                 {wq::F8F8_128, 2, 7.91, 0.497, 0.057, {0.984}},
-                                 {wq::F8F8_128_W8, 1, 7.67, 0.402, 0.203, {}},
-                                 {wq::F8F8_128X256, 1, 7.38, 0.710, 0.268, {}},
-                                 {wq::F8F8_256, 1, 7.57, 1.257, 0.358, {}}};
+                                 {wq::F8F8_64X64, 3, 2.83, 0.435, 0.004, {0.584, 0.876}},
+                                 {wq::F8F8_64, 2, 5.05, 0.507, 0, {0.816}},
+                                 {wq::F8F8_128, 2, 6.11, 0.595, 0, {1.106}},
+                                 {wq::F8F8_128X256, 1, 5.66, 0.920, 0.109, {}},
+                                 {wq::F8F8_256, 1, 6.83, 1.342, 0.250, {}}};
     const int klen = plan.k_end - plan.k_begin, ktiles = (klen + 127) / 128;
-    const double floor = 7.2 + ((double)p->N * klen + (double)p->M * klen + 2.0 * p->M * p->N) / 8.1e6;
+    const double bytes = 8.2 + ((double)p->N * klen + (double)p->M * klen + 2.0 * p->M * p->N) / 6.48e6, bytes4 = bytes * bytes * bytes * bytes;
     double best    = 1e30;
     int slices     = plan.k_batch;
     for(const Cost& k : costs)
@@ -253,17 +253,22 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
         const bool may_split = !plan.partial && !pinned && have_workspace && grid < 1 << 16;
         for(int c : {1, 2, 3, 4, 6, 8, 12, 16}) // (a factor of what the caller fixed)
         {
-            if(c > 1 && (!may_split || ktiles / c < 2))
+            if(c > 1 && (!may_split || ktiles / c < 2 || grid * c > 1100)) // (more of them were never the best)
                 break;
             const double units = grid * c * plan.k_batch, round = 256.0 * k.resident;
             auto tile_time = [&](double n) { return n <= 256 ? k.first + k.fill * n / 256 : k.more[(int)std::ceil(n / 256) - 2]; };
             const double rounds = std::floor(units / round), rest = units - rounds * round;
             const double chain  = (ktiles + c * plan.k_batch - 1) / (c * plan.k_batch);
-            double t = std::max(floor, k.fixed + chain * (rounds * tile_time(round) + (rest > 0 ? tile_time(rest) : 0)));
+            const double work   = k.fixed + chain * (rounds * tile_time(round) + (rest > 0 ? tile_time(rest) : 0));
+            double t            = std::sqrt(std::sqrt(work * work * work * work + bytes4));
             if(c > 1)
-                t += 1.89 + c * (double)p->M * p->N * 1.31e-6;
+                t += 1.89 + c * (double)p->M * p->N * 1.454e-6;
             if(t < best)
-                best = t, plan.f8f8 = k.kernel, slices = c * plan.k_batch;
+            {
+                // (128 x 128 with one workgroup per CU: eight waves, on average 2 to 6 % faster there and 15 % slower beyond)
+                best = t, slices = c * plan.k_batch;
+                plan.f8f8 = k.kernel == wq::F8F8_128 && units <= 256 ? (int)wq::F8F8_128_W8 : k.kernel;
+            }
         }
     }
     if(best == 1e30)

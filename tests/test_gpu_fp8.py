@@ -140,8 +140,8 @@ def test_few_rows(m, n, k):
 
 
 @pytest.mark.parametrize("kernel,m,n,k", [
-    ("64x64", 40, 520, 2048), ("64x64", 100, 1040, 656), ("64x64", 257, 514, 1040), ("64", 520, 6000, 656), ("64", 400, 8191, 656),
-    ("128_w8", 640, 5000, 1024), ("128_w8", 600, 4999, 1040), ("128", 400, 8192, 1024), ("128", 390, 8190, 1040), ("128x256", 512, 11008, 656),
+    ("64x64", 40, 520, 2048), ("64x64", 100, 1040, 656), ("64x64", 257, 514, 1040), ("64", 300, 11008, 656), ("64", 300, 11003, 1040),
+    ("128_w8", 640, 5000, 1024), ("128_w8", 600, 4999, 1040), ("128", 1536, 11008, 656), ("128", 1530, 11003, 656), ("128x256", 512, 11008, 656),
     ("128x256", 500, 11003, 656), ("256", 768, 11008, 656), ("256", 760, 11001, 1040)])
 def test_every_tile_kernel(kernel, m, n, k):
     P = problem(m, n, k, m + n + k, exact=True)
