@@ -192,6 +192,20 @@ def test_tensors_that_need_gradients_are_refused():
             call()
 
 
+def test_the_short_way_leaves_the_rest_to_the_long_one():
+    from composable_kernel_amd import _torch_front as front
+
+    x, w = torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(256)
+    assert front.quantized(capi.QUANT_ROWS, x, None, None, 0, 0.0, 128, 0) is None          # not on a GPU
+    assert front.quantized(capi.QUANT_RMSNORM, "x", x, w, 0, 1e-6, 128, 0) is None          # not a tensor
+    assert front.quantized("op", x, None, None, 0, 0.0, 128, 0) is None
+    assert front.linear(x, w, x, w, None, 0, torch.bfloat16, 0) is None
+    assert front.linear(x, w, x, w, None, "none", "bf16", 0) is None
+    for call in (front.quantized, front.linear, front.bind):
+        with pytest.raises(TypeError):
+            call(x)
+
+
 def test_shapes_under_fake_tensors():
     from torch._subclasses.fake_tensor import FakeTensorMode
 

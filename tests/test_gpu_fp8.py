@@ -578,6 +578,18 @@ def test_both_ways_into_the_library(shape, group):
         assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
 
 
+def test_gradients_are_refused():
+    x = torch.randn(4, 256, device="cuda").bfloat16().requires_grad_()
+    w = torch.ones(256, device="cuda", requires_grad=True)
+    y = x.detach()
+    calls = [lambda: torch_ops.quantize_fp8(x), lambda: torch_ops.gated_fp8(y, x), lambda: torch_ops.rmsnorm_fp8(y, w), lambda: torch_ops.rmsnorm_fp8(y, w.detach(), x)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="inference-only"):
+            call()
+        with torch.no_grad():
+            assert not any(t.requires_grad for t in call() if t is not None)
+
+
 def test_two_threads():
     """Each on its own stream, with its own errors."""
     x = torch.randn(300, 1024, device="cuda").bfloat16()
