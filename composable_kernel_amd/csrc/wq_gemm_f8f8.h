@@ -203,7 +203,8 @@ __global__ __launch_bounds__(256) void wq_gemm_f8f8_any(const F8F8Params p)
 //     the old one, so that their slot is free for most of it.  Activations are read LEAD row blocks ahead;
 //   * scales: once per four K tiles the row scales of those four travel as one 16-byte LDS-DMA piece per row (every row's scales
 //     lie in a cache line of their own, so fetching them tile by tile would move a line per row and tile, as much as the
-//     activations themselves), and the column blocks' the same way; needs four K tiles in all, K > 384;
+//     activations themselves), and the column blocks' the same way.  A table row of fewer than four scales (K <= 384) is copied by
+//     ordinary loads instead, to the end of the same 16 bytes;
 //   * a block sum is one MFMA from a zero accumulator.  The sums of a row block are folded into the accumulators,
 //     acc = fma(sum, sa * sb, acc), each just in front of the next row block's MFMA that overwrites it: NT MFMAs after it was
 //     issued, so that neither waits for the other.
@@ -395,6 +396,8 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
     int m0, n0, z, ntiles, kt0, s_end;
     __amdgpu_buffer_rsrc_t a_rsrc, b_rsrc, s_rsrc;
     uint32_t a_run[2][T::A_DMA], b_run[T::B_DMA], s_lane;
+    const float* s_table; // this lane's table row, and its place in LDS
+    int s_at;
     bool past;
     auto set_unit = [&](int unit) __attribute__((always_inline)) {
         int tm, tn;
@@ -426,6 +429,9 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
         const int row = min(m0 + (s_is_row ? wave : 0) * 64 + lane, p.M - 1) / p.bm - ra;
         const int blk = min(n0 + lane * 32, p.N - 1) / p.bn - rb;
         s_lane = s_is_row ? (uint32_t)row * (uint32_t)p.ld_sa * 4u : lane < T::BN / 32 ? (uint32_t)blk * (uint32_t)p.ld_sb * 4u : OUT;
+        // (the waves behind the row pieces all fetch the same piece: one of them writes by hand)
+        s_table = s_is_row ? p.sa + (size_t)(ra + row) * (size_t)p.ld_sa : p.sb + (size_t)(rb + blk) * (size_t)p.ld_sb;
+        s_at    = s_is_row ? T::S_OFF + (wave * 64 + lane) * 16 : wave == T::BM / 64 && lane < T::BN / 32 ? T::S_OFF + T::S_ROWS + lane * 16 : -1;
     };
     auto lds_at = [&](int at) __attribute__((always_inline)) { return (__attribute__((address_space(3))) void*)(lds + at); };
     auto dma_a = [&](const __amdgpu_buffer_rsrc_t& rsrc, int slot, int h, int i, bool last) __attribute__((always_inline)) {
@@ -476,8 +482,12 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
     constexpr int G0 = 1 + T::A_DMA + T::B_DMA, G1 = T::A_DMA;
 
     auto prologue = [&]() __attribute__((always_inline)) {
+        const bool wide = kblocks >= 4;
+        if(!wide && s_at >= 0)
+            for(int i = 0; i < kblocks; ++i)
+                *(float*)(lds + s_at + (4 - kblocks + i) * 4) = s_table[i];
         __builtin_amdgcn_sched_barrier(0); // (issue order is part of the vmcnt arithmetic)
-        group0(0, true, 0, 0, G0);
+        group0(0, wide, 0, 0, G0);
         __builtin_amdgcn_sched_barrier(0);
         group1(0, 0, 0, G1);
         __builtin_amdgcn_sched_barrier(0);
@@ -575,6 +585,7 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
     // the K loop of the unit whose first loads are in flight (ntiles > 0); every wave is done with the slots at its end
     auto multiply = [&]() __attribute__((always_inline)) {
         wait_vmcnt<G0 + 2 * G1>(); // group (0, 0) done (the stores of the tile before are younger: they only add to the wait)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // (scales copied by hand)
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
         a_lo = f_lo + wr * (MT * 2048), a_hi = f_hi + wr * (MT * 2048);

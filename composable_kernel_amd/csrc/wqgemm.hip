@@ -199,10 +199,10 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
     const int ld_sa = std::max(p->ld_a_scale, (p->K - 1) / 128 + 1), ld_sb = std::max(p->ld_b_scale, (p->K - 1) / 128 + 1);
     const bool rows16 = p->lda % 16 == 0 && p->ldb % 16 == 0 && (uintptr_t)p->a % 16 == 0 && (uintptr_t)p->b % 16 == 0 &&
                         plan.k_end % 16 == 0 && p->lda <= 1 << 22 && p->ldb <= 1 << 22 && p->K <= 1 << 26;
-    const bool tiles = rows16 && ld_sa <= 1 << 20 && ld_sb <= 1 << 20 && p->K > 384;
+    const bool tiles = rows16 && ld_sa <= 1 << 20 && ld_sb <= 1 << 20;
     const int pinned = p->flags & (WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256);
     if(pinned && !tiles)
-        return fail(WQ_ERR_UNSUPPORTED, "fp8 weights: WQ_FLAG_TILE_* needs 16-byte aligned rows and K a multiple of 16 above 384");
+        return fail(WQ_ERR_UNSUPPORTED, "fp8 weights: WQ_FLAG_TILE_* needs 16-byte aligned rows and K a multiple of 16");
     // Few rows: one pass over the weights, K dealt to the waves of a workgroup.  16 columns a workgroup as long as that is at most one
     // per CU, 32 up to 8192 columns (the activations are read once per workgroup; 5000 x 4096 at M = 16: 8.5 us, 16 columns 10.9),
     // 64 beyond (28672 x 8192: 44.5; 32 columns 47.4).  Straight to registers with up to 4 rows in the first range (4096 x 4096 at

@@ -163,6 +163,20 @@ def test_chosen_tile_sizes(flags, m, n, k, act):
     check(launch(P, torch.bfloat16, bias=bias, act=act, flags=flags | capi.FLAG_BF16_RTN), P, torch.bfloat16, bias, act)
 
 
+@pytest.mark.parametrize("flags", [0, capi.FLAG_TILE_128, capi.FLAG_TILE_256, capi.FLAG_TILE_128 | capi.FLAG_TILE_256])
+@pytest.mark.parametrize("k", [16, 128, 144, 256, 368, 384])
+@pytest.mark.parametrize("m,n,bm,bn", [(40, 200, 1, 128), (300, 700, 1, 32), (513, 1030, 128, 128), (4300, 4616, 3, 96)])
+def test_short_rows(flags, k, m, n, bm, bn):
+    """K of at most three scale blocks in the tile kernels, the largest with more tiles than resident workgroups."""
+    P = problem(m, n, k, m + k, exact=True, bm=bm, bn=bn)
+    p = capi.f8_problem(P["a_ptr"], P["sa"].data_ptr(), P["b_ptr"], P["sb"].data_ptr(), P["a_ptr"], m, n, k, scale_block=P["block"], flags=flags)
+    assert capi.kernel_name(p) not in ("wq_gemm_f8f8_any", "wq_gemm_generic")
+    check_exact(launch(P, torch.bfloat16, flags=flags | capi.FLAG_BF16_RTN), P)
+    if k == 384:
+        Q = problem(m, n, k, m, bm=bm, bn=bn)
+        check(launch(Q, torch.float16, flags=flags, k_batch=2 if n % 4 == 0 else 1), Q, torch.float16)
+
+
 @pytest.mark.parametrize("m,n,k", [(3, 257, 384), (40, 512, 640), (150, 384, 272), (300, 515, 1024)])
 @pytest.mark.parametrize("act", ["fastgelu", "add", "add_fastgelu"])
 def test_epilogues(m, n, k, act):
