@@ -218,25 +218,26 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
         plan.route = ROUTE_F8F8;
         return WQ_OK;
     }
-    // Tile kernels: the kernel and the number of K slices with the shortest estimate, in microseconds.  Fitted to 9 weight shapes
-    // (1024 x 8192 .. 28672 x 8192) x 13 to 15 row counts (20 .. 4096) x up to 8 slice counts of each kernel, 2700 timings with the weights
-    // in the last-level cache and out of it: the choice is on average 1 % and at most 15 % behind the best of them.  A K tile
-    // takes first + fill * (the filled part of the 256 CUs) with one workgroup per CU, more[j] with j + 2; a launch takes whole rounds of
-    // the workgroups that the chip holds; it hides behind its bytes, or they behind it, but for a corner (the fourth root); slices
-    // write and re-read fp32 slabs and need a second kernel.
+    // Tile kernels: the kernel and the number of K slices with the shortest estimate, in microseconds.  Fitted to 22 weight shapes
+    // (512 x 256 .. 28672 x 8192) x 7 to 15 row counts (20 .. 8192) x up to 6 slice counts of each kernel, 3000 timings with the weights in
+    // the last-level cache and out of it: the choice is on average 0.7 % and at most 18 % behind the best of them.  A K tile takes
+    // tile[j] with j + 1 workgroups per CU; a launch takes whole rounds of the workgroups that the chip holds, and outputs for every
+    // workgroup of a CU behind the first; it hides behind its bytes, or they behind it, but for a corner (the fourth root); slices write
+    // and re-read fp32 slabs and need a second kernel.
     struct Cost
     {
         int kernel, resident;
-        double fixed, first, fill, more[2];
+        double fixed, outputs, tile[3];
     };
-    static const Cost costs[] = {{wq::F8F8_ANY, 1, 8, 1.5, 0.1, {}},
-                                 {wq::F8F8_64X64, 3, 2.83, 0.435, 0.004, {0.584, 0.876}},
-                                 {wq::F8F8_64, 2, 5.05, 0.507, 0, {0.816}},
-                                 {wq::F8F8_128, 2, 6.11, 0.595, 0, {1.106}},
-                                 {wq::F8F8_128X256, 1, 5.66, 0.920, 0.109, {}},
-                                 {wq::F8F8_256, 1, 6.83, 1.342, 0.250, {}}};
+    static const Cost costs[] = {{wq::F8F8_ANY, 1, 8, 2, {1.5}},
+                                 {wq::F8F8_64X64, 3, 3.37, 1.09, {0.423, 0.525, 0.718}},
+                                 {wq::F8F8_64, 2, 4.64, 1.70, {0.516, 0.711}},
+                                 {wq::F8F8_128, 2, 5.07, 2.33, {0.625, 1.058}},
+                                 {wq::F8F8_128X256, 1, 6.75, 4.56, {0.956}},
+                                 {wq::F8F8_256, 1, 9.88, 9.21, {1.469}}};
     const int klen = plan.k_end - plan.k_begin, ktiles = (klen + 127) / 128;
-    const double bytes = 8.2 + ((double)p->N * klen + (double)p->M * klen + 2.0 * p->M * p->N) / 6.48e6, bytes4 = bytes * bytes * bytes * bytes;
+    const double outputs = (double)p->M * p->N;
+    const double bytes   = 3.6 + ((double)p->N * klen + (double)p->M * klen) / 5.95e6 + 2 * outputs / 3e6, bytes4 = bytes * bytes * bytes * bytes;
     double best    = 1e30;
     int slices     = plan.k_batch;
     for(const Cost& k : costs)
@@ -247,22 +248,25 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
                                                          : 0;
         if((k.kernel == wq::F8F8_ANY) == tiles || (pinned && pinned != flags))
             continue;
-        const double grid = (double)((p->M - 1) / wq::f8f8_bm(k.kernel) + 1) * ((p->N - 1) / wq::f8f8_bn(k.kernel) + 1);
+        const long grid = (long)((p->M - 1) / wq::f8f8_bm(k.kernel) + 1) * ((p->N - 1) / wq::f8f8_bn(k.kernel) + 1), round = 256 * k.resident;
         if(grid * plan.k_batch >= 1 << 23) // (work items along x)
             continue;
         const bool may_split = !plan.partial && !pinned && have_workspace && grid < 1 << 16;
-        for(int c : {1, 2, 3, 4, 6, 8, 12, 16}) // (a factor of what the caller fixed)
+        for(int c : {1, 2, 3, 4, 6, 8}) // (a factor of what the caller fixed)
         {
             if(c > 1 && (!may_split || ktiles / c < 2 || grid * c > 1100)) // (more of them were never the best)
                 break;
-            const double units = grid * c * plan.k_batch, round = 256.0 * k.resident;
-            auto tile_time = [&](double n) { return n <= 256 ? k.first + k.fill * n / 256 : k.more[(int)std::ceil(n / 256) - 2]; };
-            const double rounds = std::floor(units / round), rest = units - rounds * round;
-            const double chain  = (ktiles + c * plan.k_batch - 1) / (c * plan.k_batch);
-            const double work   = k.fixed + chain * (rounds * tile_time(round) + (rest > 0 ? tile_time(rest) : 0));
-            double t            = std::sqrt(std::sqrt(work * work * work * work + bytes4));
+            const long units = grid * c * plan.k_batch, full = units / round;
+            const int last   = (int)((units - full * round + 255) / 256); // workgroups of the busiest CU in the last round
+            const int chain  = (ktiles + c * plan.k_batch - 1) / (c * plan.k_batch);
+            const double work = k.fixed + chain * (full * k.tile[k.resident - 1] + (last ? k.tile[last - 1] : 0)) +
+                                k.outputs * (full * k.resident + last - 1);
+            if(work >= best) // (the estimate is not below it)
+                continue;
+            double t = std::sqrt(std::sqrt(work * work * work * work + bytes4));
             if(c > 1)
-                t += 1.89 + c * (double)p->M * p->N * 1.454e-6;
+                t += 2.37 + c * (outputs * 1.086e-6 + 0.2);
+            t *= 1 + 0.0075 * c; // (between near equals the one with less scratch)
             if(t < best)
             {
                 // (128 x 128 with one workgroup per CU: eight waves, on average 2 to 6 % faster there and 15 % slower beyond)
