@@ -21,6 +21,8 @@ enum F8F8Kernel
     F8F8_SKINNY_32,     // M <= 32: 16 columns, eight waves
     F8F8_SKINNY_32X32   // M <= 32: 32 columns, eight waves
 };
+// K of operands copied to aligned rows
+inline int f8f8_padded_k(int K) { return (K + 15) & ~15; }
 constexpr int f8f8_bm(int kernel) { return kernel == F8F8_256 ? 256 : kernel == F8F8_64 || kernel == F8F8_64X64 ? 64 : 128; }
 constexpr int f8f8_bn(int kernel)
 {
@@ -47,6 +49,7 @@ struct F8F8Params
 };
 
 int launch_f8f8(int kernel, const F8F8Params& p, hipStream_t s);
+void launch_pad_f8(const wqgemm_problem* p, uint8_t* rows, hipStream_t s);
 void launch_reduce_f8f8(const float* slabs, int k_batch, int ld_part, const F8F8Params& p, hipStream_t s);
 
 } // namespace wq

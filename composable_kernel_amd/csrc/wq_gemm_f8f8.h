@@ -934,6 +934,19 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny(const F8F8Para
     }
 }
 
+// Rows of both operands, of any alignment, to rows of whole 16-byte pieces, zeros behind their last byte; a wave per row.
+__global__ __launch_bounds__(256) void wq_pad_rows_f8(const uint8_t* __restrict__ a, long lda, int M, const uint8_t* __restrict__ b, long ldb, int N, int K,
+                                                      uint8_t* __restrict__ rows)
+{
+    const int pieces = (K + 15) >> 4;
+    for(long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6); row < (long)M + N; row += (long)gridDim.x * 4)
+    {
+        const uint8_t* src = row < M ? a + row * lda : b + (row - M) * ldb;
+        for(int i = threadIdx.x & 63; i < pieces; i += 64)
+            *(u4_t*)(rows + (row * pieces + i) * 16) = f8f8_load16(src, i * 16, K);
+    }
+}
+
 // Split-K: out[m, n] = epilogue(sum_z slab[z][m][n]), z ascending, for any N (ld_part is N rounded up to 4).
 __global__ __launch_bounds__(256) void wq_reduce_f8f8(const float* __restrict__ slabs, int k_batch, int ld_part, F8F8Params p)
 {

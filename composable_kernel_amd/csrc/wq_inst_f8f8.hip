@@ -69,6 +69,12 @@ int launch_f8f8(int kernel, const F8F8Params& p, hipStream_t s)
     }
 }
 
+void launch_pad_f8(const wqgemm_problem* p, uint8_t* rows, hipStream_t s)
+{
+    hipLaunchKernelGGL(wq_pad_rows_f8, dim3((unsigned)std::min(((long)p->M + p->N + 3) / 4, 1L << 16)), dim3(256), 0, s, (const uint8_t*)p->a, (long)p->lda, p->M,
+                       (const uint8_t*)p->b, (long)p->ldb, p->N, p->K, rows);
+}
+
 void launch_reduce_f8f8(const float* slabs, int k_batch, int ld_part, const F8F8Params& p, hipStream_t s)
 {
     const long blocks = ((long)p.M * (ld_part / 4) + 255) / 256;

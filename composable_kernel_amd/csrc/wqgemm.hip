@@ -88,6 +88,7 @@ struct Plan
     bool f8_fused   = false; // fp8 activations widened inside the small-M whole-image kernel (no image in the workspace)
     bool split_256  = false; // the planner's split-K is what put this problem on the 256-tile kernel
     int f8f8       = 0;     // ROUTE_F8F8: wq::F8F8Kernel
+    bool pad_rows  = false; // ROUTE_F8F8: both operands are copied to aligned rows in the workspace first
     bool via_colb = false; // row-major 8-bit B: transpose into the workspace, then the K-contiguous matrix-core kernels
     bool via_f16  = false; // fp8 FNUZ activations: convert to fp16 in the workspace, then the fp16 MFMA kernel
 };
@@ -209,12 +210,14 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
     // M = 1: 6.5, through LDS 6.9) and up to 2 in the last (28672 x 8192 at M = 1: 38.3 against 43.1, at M = 4: 45.6 against 43.2).
     // With 17 .. 32 rows up to 8192 columns (32 rows, 4096 x 4096: 9.0, the best tile kernel 10.2; 5000 x 4096: 10.7), beyond them
     // the tile kernels (28672 x 8192: 59 against 54), and so from 33 rows (64 rows, 4096 x 11008: 27 against 16.2).
-    if(rows16 && !pinned && p->M <= (p->N <= 8192 ? 32 : 16) && p->N <= 1 << 25) // (64 work items per column: as above)
+    const bool few = p->N <= 4096, many = p->N > 8192;
+    const bool few_rows    = !pinned && p->M <= (many ? 16 : 32) && p->N <= 1 << 25; // (64 work items per column: as above)
+    const int few_rows_k   = (few && p->M <= 4) || (many && p->M <= 2) ? wq::F8F8_SKINNY_DIRECT
+                             : p->M > 16 ? (few ? wq::F8F8_SKINNY_32 : wq::F8F8_SKINNY_32X32)
+                             : few ? wq::F8F8_SKINNY_16 : many ? wq::F8F8_SKINNY_16X64 : wq::F8F8_SKINNY_16X32;
+    if(rows16 && few_rows)
     {
-        const bool few = p->N <= 4096, many = p->N > 8192;
-        plan.f8f8      = (few && p->M <= 4) || (many && p->M <= 2) ? wq::F8F8_SKINNY_DIRECT
-                         : p->M > 16 ? (few ? wq::F8F8_SKINNY_32 : wq::F8F8_SKINNY_32X32)
-                         : few ? wq::F8F8_SKINNY_16 : many ? wq::F8F8_SKINNY_16X64 : wq::F8F8_SKINNY_16X32;
+        plan.f8f8  = few_rows_k;
         plan.route = ROUTE_F8F8;
         return WQ_OK;
     }
@@ -229,7 +232,7 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
         int kernel, resident;
         double fixed, outputs, tile[3];
     };
-    static const Cost costs[] = {{wq::F8F8_ANY, 1, 8, 2, {1.5}},
+    static const Cost costs[] = {{wq::F8F8_ANY, 1, 8, 4, {2.65}},
                                  {wq::F8F8_64X64, 3, 3.37, 1.09, {0.423, 0.525, 0.718}},
                                  {wq::F8F8_64, 2, 4.64, 1.70, {0.516, 0.711}},
                                  {wq::F8F8_128, 2, 5.07, 2.33, {0.625, 1.058}},
@@ -240,40 +243,53 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
     const double bytes   = 3.6 + ((double)p->N * klen + (double)p->M * klen) / 5.95e6 + 2 * outputs / 3e6, bytes4 = bytes * bytes * bytes * bytes;
     double best    = 1e30;
     int slices     = plan.k_batch;
-    for(const Cost& k : costs)
-    {
-        const int flags = k.kernel == wq::F8F8_256       ? WQ_FLAG_TILE_256
-                          : k.kernel == wq::F8F8_128X256 ? WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256
-                          : k.kernel >= wq::F8F8_128     ? WQ_FLAG_TILE_128
-                                                         : 0;
-        if((k.kernel == wq::F8F8_ANY) == tiles || (pinned && pinned != flags))
-            continue;
-        const long grid = (long)((p->M - 1) / wq::f8f8_bm(k.kernel) + 1) * ((p->N - 1) / wq::f8f8_bn(k.kernel) + 1), round = 256 * k.resident;
-        if(grid * plan.k_batch >= 1 << 23) // (work items along x)
-            continue;
-        const bool may_split = !plan.partial && !pinned && have_workspace && grid < 1 << 16;
-        for(int c : {1, 2, 3, 4, 6, 8}) // (a factor of what the caller fixed)
+    const auto choose = [&](bool aligned, double before) {
+        for(const Cost& k : costs)
         {
-            if(c > 1 && (!may_split || ktiles / c < 2 || grid * c > 1100)) // (more of them were never the best)
-                break;
-            const long units = grid * c * plan.k_batch, full = units / round;
-            const int last   = (int)((units - full * round + 255) / 256); // workgroups of the busiest CU in the last round
-            const int chain  = (ktiles + c * plan.k_batch - 1) / (c * plan.k_batch);
-            const double work = k.fixed + chain * (full * k.tile[k.resident - 1] + (last ? k.tile[last - 1] : 0)) +
-                                k.outputs * (full * k.resident + last - 1);
-            if(work >= best) // (the estimate is not below it)
+            const int flags = k.kernel == wq::F8F8_256       ? WQ_FLAG_TILE_256
+                              : k.kernel == wq::F8F8_128X256 ? WQ_FLAG_TILE_128 | WQ_FLAG_TILE_256
+                              : k.kernel >= wq::F8F8_128     ? WQ_FLAG_TILE_128
+                                                             : 0;
+            if((k.kernel == wq::F8F8_ANY) == aligned || (pinned && pinned != flags))
                 continue;
-            double t = std::sqrt(std::sqrt(work * work * work * work + bytes4));
-            if(c > 1)
-                t += 2.37 + c * (outputs * 1.086e-6 + 0.2);
-            t *= 1 + 0.0075 * c; // (between near equals the one with less scratch)
-            if(t < best)
+            const long grid = (long)((p->M - 1) / wq::f8f8_bm(k.kernel) + 1) * ((p->N - 1) / wq::f8f8_bn(k.kernel) + 1), round = 256 * k.resident;
+            if(grid * plan.k_batch >= 1 << 23) // (work items along x)
+                continue;
+            const bool may_split = !plan.partial && !pinned && have_workspace && grid < 1 << 16;
+            for(int c : {1, 2, 3, 4, 6, 8}) // (a factor of what the caller fixed)
             {
-                // (128 x 128 with one workgroup per CU: eight waves, on average 2 to 6 % faster there and 15 % slower beyond)
-                best = t, slices = c * plan.k_batch;
-                plan.f8f8 = k.kernel == wq::F8F8_128 && units <= 256 ? (int)wq::F8F8_128_W8 : k.kernel;
+                if(c > 1 && (!may_split || ktiles / c < 2 || grid * c > 1100)) // (more of them were never the best)
+                    break;
+                const long units = grid * c * plan.k_batch, full = units / round;
+                const int last   = (int)((units - full * round + 255) / 256); // workgroups of the busiest CU in the last round
+                const int chain  = (ktiles + c * plan.k_batch - 1) / (c * plan.k_batch);
+                const double work = before + k.fixed + chain * (full * k.tile[k.resident - 1] + (last ? k.tile[last - 1] : 0)) +
+                                    k.outputs * (full * k.resident + last - 1);
+                if(work >= best) // (the estimate is not below it)
+                    continue;
+                double t = std::sqrt(std::sqrt(work * work * work * work + bytes4));
+                if(c > 1)
+                    t += 2.37 + c * (outputs * 1.086e-6 + 0.2);
+                t *= 1 + 0.0075 * c; // (between near equals the one with less scratch)
+                if(t < best)
+                {
+                    // (128 x 128 with one workgroup per CU: eight waves, on average 2 to 6 % faster there and 15 % slower beyond)
+                    best = t, slices = c * plan.k_batch;
+                    plan.f8f8 = k.kernel == wq::F8F8_128 && units <= 256 ? (int)wq::F8F8_128_W8 : k.kernel, plan.pad_rows = before > 0;
+                }
             }
         }
+    };
+    choose(tiles, 0);
+    // Rows that are not aligned: most often it is shorter to copy both operands to aligned ones first, a launch and their bytes twice
+    // (777 x 5000 x 4111: 51 us, the kernel for any alignment 134; 1 x 4096 x 4095: 15.5 and 80; 300 x 300 x 130: 10 and 22).
+    if(!tiles && !plan.partial && !pinned && have_workspace && p->K <= 1 << 22 && ld_sa <= 1 << 20 && ld_sb <= 1 << 20)
+    {
+        const double copy = 3 + 2.0 * ((double)p->M + p->N) * wq::f8f8_padded_k(p->K) / 5e6;
+        if(!few_rows)
+            choose(true, copy);
+        else if(const double t = copy + 3.5 + (double)p->N * p->K / 5.2e6; t < best)
+            best = t, slices = 1, plan.f8f8 = few_rows_k, plan.pad_rows = true;
     }
     if(best == 1e30)
         return fail(WQ_ERR_UNSUPPORTED, "too many tiles for one launch");
@@ -819,6 +835,12 @@ void f16_image_of_a(const wqgemm_problem* p, void* workspace, hipStream_t s, wq:
 // Columns of a split-K slab of the fp8 x fp8 kernels: whole groups of four, so that odd N splits like any other.
 int f8f8_ld_part(const wqgemm_problem* p) { return (p->N + 3) & ~3; }
 
+// Bytes of the slabs in the workspace, in whole cache lines (the copied rows follow).
+size_t f8f8_slab_bytes(const wqgemm_problem* p, const Plan& plan)
+{
+    return plan.partial && !plan.to_c ? ((size_t)plan.k_batch * p->M * f8f8_ld_part(p) * sizeof(float) + 127) & ~(size_t)127 : 0;
+}
+
 const char* const kF8F8Names[] = {"wq_gemm_f8f8_any", "wq_gemm_f8f8_64x64", "wq_gemm_f8f8_64", "wq_gemm_f8f8_128", "wq_gemm_f8f8_128_w8", "wq_gemm_f8f8_128x256", "wq_gemm_f8f8_256",
                                   "wq_gemm_f8f8_skinny_direct", "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny",
                                   "wq_gemm_f8f8_skinny", "wq_gemm_f8f8_skinny"};
@@ -1078,6 +1100,15 @@ int launch_main(const wqgemm_problem* p, const Plan& plan, void* workspace, hipS
         gp.c       = out;
         if(plan.partial && !plan.to_c)
             gp.ldc = f8f8_ld_part(p);
+        if(plan.pad_rows)
+        {
+            uint8_t* rows = (uint8_t*)workspace + f8f8_slab_bytes(p, plan);
+            wq::launch_pad_f8(p, rows, s);
+            gp.K = gp.lda = gp.ldb = gp.k_end = wq::f8f8_padded_k(p->K);
+            gp.a = rows, gp.b = rows + (size_t)p->M * gp.K;
+            if(!plan.partial)
+                gp.k_per_z = gp.K;
+        }
         const int bm = wq::f8f8_bm(plan.f8f8), bn = wq::f8f8_bn(plan.f8f8);
         gp.tiles_m = (p->M - 1) / bm + 1, gp.tiles_n = (p->N - 1) / bn + 1;
         // (group_m as for the other tile kernels: g rows of A plus run / g columns of B per XCD)
@@ -1245,6 +1276,8 @@ int wqgemm_is_supported(const wqgemm_problem* p)
 
 static size_t plan_workspace_bytes(const wqgemm_problem* p, const Plan& plan)
 {
+    if(plan.route == ROUTE_F8F8 && plan.pad_rows)
+        return f8f8_slab_bytes(p, plan) + ((size_t)p->M + p->N) * wq::f8f8_padded_k(p->K);
     if(plan.partial && !plan.to_c && plan.route == ROUTE_F8F8)
         return (size_t)plan.k_batch * p->M * f8f8_ld_part(p) * sizeof(float);
     if(plan.partial && !plan.to_c)
@@ -1501,8 +1534,8 @@ int wqgemm_type_string(const wqgemm_problem* p, char* buf, size_t n)
                  dt_name(p->a_dtype), dt_name(p->b_dtype), dt_name(p->c_dtype), plan.k_batch,
                  !has_block_scales(p) ? "" : p->scale_block_m % 128 == 0 ? ", ABScalePer128K" : ", ABScalePer128K_RowScaleA");
     else if(plan.route == ROUTE_F8F8)
-        snprintf(buf, n, "DeviceGemmMultiD_ABScale_Mfma_gfx950<%s, 16x16x128_f8f6f4, %s, %s, %s, KBatch%d>",
-                 kF8F8Instances[plan.f8f8],
+        snprintf(buf, n, "DeviceGemmMultiD_ABScale_Mfma_gfx950<%s%s, 16x16x128_f8f6f4, %s, %s, %s, KBatch%d>",
+                 kF8F8Instances[plan.f8f8], plan.pad_rows ? ", PaddedRows" : "",
                  dt_name(p->a_dtype), dt_name(p->b_dtype), dt_name(p->c_dtype), plan.k_batch);
     else if(plan.route == ROUTE_SKINNY_WS)
         snprintf(buf, n, "DeviceFpAintBGemm_SmallM_gfx950<256, 16, 16, 16x16x32, %s, %s, %s, StreamB, WavesSplitK>",

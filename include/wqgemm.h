@@ -204,6 +204,8 @@ int wqgemm_is_supported(const wqgemm_problem* p);
  *  - K*N for tile-aligned row-major (K x N) 8-bit weights (optional: holds the K-contiguous transpose the
  *    matrix-core kernels read);
  *  - kb*M*roundup(N, 4)*4 for fp8 weights, k_batch > 1 or the planner's own split (optional: without it one slice);
+ *    plus (M + N)*roundup(K, 16) where their rows are not 16-byte aligned and copying both operands first is shorter
+ *    (optional: without it the kernel for any alignment);
  *  - else 0.
  * The answer is for *p as it stands: strides and the alignment of its pointers choose the kernel, so ask with the problem that
  * will be launched.

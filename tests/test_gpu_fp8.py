@@ -163,6 +163,23 @@ def test_chosen_tile_sizes(flags, m, n, k, act):
     check(launch(P, torch.bfloat16, bias=bias, act=act, flags=flags | capi.FLAG_BF16_RTN), P, torch.bfloat16, bias, act)
 
 
+@pytest.mark.parametrize("m,n,k,lda,ldb,offset", [
+    (1, 4096, 4095, None, None, 0), (4, 300, 117, 119, 130, 1), (16, 9000, 1000, 1004, None, 3), (30, 5000, 2047, None, 2049, 0), (64, 500, 1001, None, None, 5),
+    (300, 700, 1040, 1041, 1040, 0), (257, 1030, 4096, None, None, 8), (700, 3000, 130, None, 133, 0), (100, 1024, 8191, None, None, 1)])
+def test_rows_of_any_alignment(m, n, k, lda, ldb, offset):
+    """Operands that are copied to aligned rows first, and the kernel that needs no copy (and no workspace) on the same ones."""
+    P = problem(m, n, k, m + n, lda=lda, ldb=ldb, offset=offset, exact=True)
+    kw = dict(lda=P["lda"], ldb=P["ldb"], scale_block=P["block"])
+    p = capi.f8_problem(P["a_ptr"], P["sa"].data_ptr(), P["b_ptr"], P["sb"].data_ptr(), P["sa"].data_ptr(), m, n, k, **kw)
+    assert "PaddedRows" in capi.type_string(p) and capi.workspace_bytes(p) >= (m + n) * (-(-k // 16) * 16)
+    check_exact(launch(P, torch.bfloat16), P)
+    check_exact(launch(P, torch.bfloat16, workspace=False), P)
+    if capi.workspace_bytes(p) < capi.NOALLOC_SCRATCH_BYTES:
+        check_exact(launch(P, torch.bfloat16, noalloc=True), P)
+    Q = problem(m, n, k, m, lda=lda, ldb=ldb, offset=offset)
+    check(launch(Q, torch.float16), Q, torch.float16)
+
+
 @pytest.mark.parametrize("flags", [0, capi.FLAG_TILE_128, capi.FLAG_TILE_256, capi.FLAG_TILE_128 | capi.FLAG_TILE_256])
 @pytest.mark.parametrize("k", [16, 128, 144, 256, 368, 384])
 @pytest.mark.parametrize("m,n,bm,bn", [(40, 200, 1, 128), (300, 700, 1, 32), (513, 1030, 128, 128), (4300, 4616, 3, 96)])
