@@ -1102,7 +1102,7 @@ int launch_main(const wqgemm_problem* p, const Plan& plan, void* workspace, hipS
             gp.ldc = f8f8_ld_part(p);
         if(plan.pad_rows)
         {
-            uint8_t* rows = (uint8_t*)workspace + f8f8_slab_bytes(p, plan);
+            uint8_t* rows = (uint8_t*)(((uintptr_t)workspace + f8f8_slab_bytes(p, plan) + 15) & ~(uintptr_t)15);
             wq::launch_pad_f8(p, rows, s);
             gp.K = gp.lda = gp.ldb = gp.k_end = wq::f8f8_padded_k(p->K);
             gp.a = rows, gp.b = rows + (size_t)p->M * gp.K;
@@ -1277,7 +1277,7 @@ int wqgemm_is_supported(const wqgemm_problem* p)
 static size_t plan_workspace_bytes(const wqgemm_problem* p, const Plan& plan)
 {
     if(plan.route == ROUTE_F8F8 && plan.pad_rows)
-        return f8f8_slab_bytes(p, plan) + ((size_t)p->M + p->N) * wq::f8f8_padded_k(p->K);
+        return f8f8_slab_bytes(p, plan) + ((size_t)p->M + p->N) * wq::f8f8_padded_k(p->K) + 16; // (a workspace of any alignment)
     if(plan.partial && !plan.to_c && plan.route == ROUTE_F8F8)
         return (size_t)plan.k_batch * p->M * f8f8_ld_part(p) * sizeof(float);
     if(plan.partial && !plan.to_c)

@@ -180,6 +180,20 @@ def test_rows_of_any_alignment(m, n, k, lda, ldb, offset):
     check(launch(Q, torch.float16), Q, torch.float16)
 
 
+@pytest.mark.parametrize("m,n,k,off", [(70, 300, 1001, 4), (40, 520, 2049, 12), (300, 515, 700, 8)])
+def test_workspace_of_any_alignment(m, n, k, off):
+    P = problem(m, n, k, m, exact=True)
+    c = torch.full((m, n), -77.0, dtype=torch.bfloat16, device="cuda")
+    p = capi.f8_problem(P["a_ptr"], P["sa"].data_ptr(), P["b_ptr"], P["sb"].data_ptr(), c.data_ptr(), m, n, k, scale_block=P["block"], flags=capi.FLAG_BF16_RTN)
+    nbytes = capi.workspace_bytes(p)
+    assert "PaddedRows" in capi.type_string(p)
+    ws = torch.full((nbytes + 64,), 0xFF, dtype=torch.uint8, device="cuda")
+    capi.launch(p, ws.data_ptr() + off, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    check_exact(c, P)
+    assert bool((ws[:off] == 0xFF).all()) and bool((ws[off + nbytes:] == 0xFF).all())
+
+
 @pytest.mark.parametrize("flags", [0, capi.FLAG_TILE_128, capi.FLAG_TILE_256, capi.FLAG_TILE_128 | capi.FLAG_TILE_256])
 @pytest.mark.parametrize("k", [16, 128, 144, 256, 368, 384])
 @pytest.mark.parametrize("m,n,bm,bn", [(40, 200, 1, 128), (300, 700, 1, 32), (513, 1030, 128, 128), (4300, 4616, 3, 96)])
