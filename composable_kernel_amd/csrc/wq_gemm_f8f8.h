@@ -11,6 +11,7 @@
 #include <utility>
 
 #include "wq_f8f8.h"
+#include "wq_f8f8_walk.h"
 #include "wq_gemm_256_f8.h"
 
 namespace wq {
@@ -701,8 +702,7 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny_direct(const F
     const int n0 = blockIdx.x * (NB * 16), z = blockIdx.y;
     const int k0 = p.k_begin + z * p.k_per_z, k1 = min(p.k_end, k0 + p.k_per_z);
     const int ntiles = (k1 - k0 + 127) >> 7; // (empty slices: <= 0)
-    const int turn   = ntiles > 0 && gridDim.x <= 256 ? (int)(blockIdx.x * kF8F8Turn % (unsigned)ntiles) : 0;
-    auto turned      = [&](int tile) __attribute__((always_inline)) { return tile + turn < ntiles ? tile + turn : tile + turn - ntiles; };
+    const F8F8Walk walk(ntiles, gridDim.x <= 256 ? blockIdx.x * kF8F8Turn : 0);
     constexpr uint32_t OUT = 0x80000000u;
 
     const long a_bytes = (long)(p.M - 1) * p.lda + p.K, b_bytes = (long)(p.N - n0 - 1) * p.ldb + p.K;
@@ -744,7 +744,7 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny_direct(const F
         for(int i = 0; i < P; ++i)
             if(i < tiles)
             {
-                const int tile = turned(first + i * WAVES);
+                const int tile = walk.tile(first + i * WAVES);
 #pragma unroll
                 for(int nb = 0; nb < NB; ++nb)
                     w[i][nb] = load(b_rsrc, b_lane, (uint32_t)(nb * 16) * (uint32_t)p.ldb, tile);
@@ -759,7 +759,7 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny_direct(const F
         for(int i = 0; i < P; ++i)
             if(i < tiles)
             {
-                const int tile = turned(first + i * WAVES);
+                const int tile = walk.tile(first + i * WAVES);
 #pragma unroll
                 for(int nb = 0; nb < NB; ++nb)
                 {
@@ -819,8 +819,7 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny(const F8F8Para
     const int k0 = p.k_begin + z * p.k_per_z, k1 = min(p.k_end, k0 + p.k_per_z);
     const int ntiles = (k1 - k0 + 127) >> 7; // (empty slices: <= 0)
     const int mine   = ntiles > wave ? (ntiles - wave + WAVES - 1) / WAVES : 0;
-    const int turn   = ntiles > 0 ? (int)(blockIdx.x * kF8F8Turn % (unsigned)ntiles) : 0;
-    auto turned      = [&](int tile) __attribute__((always_inline)) { return tile + turn < ntiles ? tile + turn : tile + turn - ntiles; };
+    const F8F8Walk walk(ntiles, blockIdx.x * kF8F8Turn);
     constexpr uint32_t OUT = 0x80000000u;
 
     auto resource = [](const void* base, long bytes) __attribute__((always_inline)) {
@@ -852,7 +851,7 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny(const F8F8Para
     uint8_t* ring = lds + wave * (D * T::SLOT);
     // (tiles past the wave's last one: scales of its last, pieces of zeros without a memory access)
     auto fetch = [&](int i, int j) __attribute__((always_inline)) {
-        const int step = wave + j * WAVES, tile = turned(step), known = turned(min(step, max(ntiles - 1, 0)));
+        const int step = wave + j * WAVES, tile = walk.tile(step), known = walk.scales(step);
 #pragma unroll
         for(int mt = 0; mt < MT; ++mt)
             ra[i][mt] = sa[mt][known];
@@ -872,16 +871,17 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny(const F8F8Para
     };
     const int f_lo = fr * 128 + (((2 * fq) ^ f8_a_swz(fr)) << 4), f_hi = fr * 128 + (((2 * fq + 1) ^ f8_a_swz(fr)) << 4);
 
+    if(!walk.empty())
 #pragma unroll
-    for(int i = 0; i < D; ++i)
-        fetch(i, i);
+        for(int i = 0; i < D; ++i)
+            fetch(i, i);
     for(int j = 0; j < mine; j += D)
     {
 #pragma unroll
         for(int i = 0; i < D; ++i)
             if(j + i < mine)
             {
-                const int tile = turned(wave + (j + i) * WAVES);
+                const int tile = walk.tile(wave + (j + i) * WAVES);
                 wait_vmcnt<(D - 1) * T::OPS>();
                 __builtin_amdgcn_sched_barrier(0);
                 i8v_t w[NB], a[MT];
