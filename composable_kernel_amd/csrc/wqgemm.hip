@@ -180,11 +180,11 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
     if((uintptr_t)p->c % (slice ? 4 : 2) != 0)
         return fail(WQ_ERR_INVALID, "C must be aligned to its elements");
     // The matrix core decodes E4M3FN; of FNUZ it cannot express three encodings.  A K step is one scale block, a wave's 32
-    // columns lie in one column block.
+    // columns lie in one column block.  (Its kernels step K by 128 in 32 bits.)
     const bool fnuz = p->a_dtype == WQ_F8_FNUZ || p->b_dtype == WQ_F8_FNUZ;
     const bool mfma = !(p->flags & WQ_FLAG_GENERIC) && (!fnuz || (p->flags & WQ_FLAG_F8_NO_SPECIALS)) && p->a_layout == WQ_ROW_MAJOR &&
                       p->b_layout == WQ_COL_MAJOR && p->scale_block_k == 128 && p->scale_block_n % 32 == 0 &&
-                      plan.k_begin % 128 == 0; // (k_batch slices are whole blocks: k_per_z is a multiple of 128 there)
+                      plan.k_begin % 128 == 0 && p->K <= 0x7FFFFF00; // (k_batch slices are whole blocks: k_per_z is a multiple of 128 there)
     if(!mfma)
     {
         if((p->M + 15) / 16 > 65535)
@@ -351,6 +351,8 @@ int make_plan(const wqgemm_problem* p, Plan& plan, bool have_workspace = true)
     // (slices in whole K tiles of the kernel that will run them: 128 k on the fp8 matrix core, 64 k elsewhere)
     const int k_tile = p->a_dtype == WQ_F8_FNUZ || p->a_dtype == WQ_F8_E4M3FN ? 128 : 64;
     plan.k_per_z     = kb > 1 ? wqgemm_splitk_kread(klen, kb, k_tile) : klen;
+    if((long)kb * plan.k_per_z > INT32_MAX && kb > 1)
+        return fail(WQ_ERR_UNSUPPORTED, "K = %d in %d slices of %d passes 2^31 - 1", klen, kb, plan.k_per_z);
     // (trailing slices may be empty when K is small: they store zero partials)
     if(plan.partial && (p->N % 4 != 0 || p->ldc % 4 != 0))
         return fail(WQ_ERR_UNSUPPORTED, "split-K needs N and ldc to be multiples of 4");
