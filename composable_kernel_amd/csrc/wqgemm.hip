@@ -141,6 +141,9 @@ int check_fp_epilogue(const wqgemm_problem* p)
     return WQ_OK;
 }
 
+// Scale blocks along K (one for any block longer than K, up to 2^31 - 1).
+int scale_blocks_k(const wqgemm_problem* p) { return (p->K - 1) / p->scale_block_k + 1; }
+
 // Both block-scale tables present and well formed.
 int check_block_scales(const wqgemm_problem* p)
 {
@@ -148,7 +151,7 @@ int check_block_scales(const wqgemm_problem* p)
         return fail(WQ_ERR_INVALID, "block-wise scales come in pairs: a_block_scale and b_block_scale");
     if(p->scale_block_m < 1 || p->scale_block_n < 1 || p->scale_block_k < 1)
         return fail(WQ_ERR_INVALID, "scale_block_m / _n / _k must be positive");
-    const int kblocks = (p->K - 1) / p->scale_block_k + 1;
+    const int kblocks = scale_blocks_k(p);
     if(p->ld_a_scale < 0 || p->ld_b_scale < 0 || (p->ld_a_scale != 0 && p->ld_a_scale < kblocks) ||
        (p->ld_b_scale != 0 && p->ld_b_scale < kblocks))
         return fail(WQ_ERR_INVALID, "ld_a_scale / ld_b_scale must be 0 or at least ceil(K / scale_block_k) = %d", kblocks);
@@ -785,7 +788,7 @@ void set_block_scales(Params& gp, const wqgemm_problem* p)
     gp.sa         = on ? (const float*)p->a_block_scale : nullptr;
     gp.sb         = on ? (const float*)p->b_block_scale : nullptr;
     gp.bm = on ? p->scale_block_m : 1, gp.bn = on ? p->scale_block_n : 1;
-    const int kblocks = on ? (p->K + p->scale_block_k - 1) / p->scale_block_k : 1;
+    const int kblocks = on ? scale_blocks_k(p) : 1;
     gp.ld_sa = on && p->ld_a_scale > 0 ? p->ld_a_scale : kblocks;
     gp.ld_sb = on && p->ld_b_scale > 0 ? p->ld_b_scale : kblocks;
     if constexpr(std::is_same_v<Params, wq::GenericParams>)

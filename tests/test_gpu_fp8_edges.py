@@ -2,7 +2,10 @@
 import pytest
 import torch
 
-from test_gpu_fp8 import check, check_exact, launch, problem
+from composable_kernel_amd import capi
+import fp8_ref
+from fp8_ref import U32
+from test_gpu_fp8 import check, check_exact, launch, problem, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -15,3 +18,19 @@ def test_slices_behind_the_end_of_k(m, n, k, k_batch):
     check_exact(launch(P, torch.bfloat16, k_batch=k_batch), P)
     P = problem(m, n, k, m + k_batch)
     check(launch(P, torch.float16, k_batch=k_batch), P, torch.float16)
+
+
+@pytest.mark.parametrize("block", [(1, 128, 2 ** 31 - 1), (3, 40, 2 ** 31 - 1), (2 ** 31 - 1, 7, 2 ** 31 - 100), (2, 2 ** 31 - 1, 200)])
+def test_scale_blocks_longer_than_the_operands(block):
+    """One scale along K, as a block of any length says it: each row and column block with its own."""
+    bm, bn, bk = block
+    m, n, k = 10, 320, 384
+    P = problem(m, n, k, 7, bm=min(bm, m), bn=min(bn, n), bk=min(bk, k))
+    want, size = reference(P)
+    P["block"] = block
+    got = launch(P, torch.float16)
+    # (the general kernel sums the K products one by one: K additions in place of 128 and the blocks')
+    bound = fp8_ref.linear_bound(want, size, k, torch.float16) + 3 * k * U32 * size
+    assert bool(((got.double() - want).abs() <= bound).all())
+    Q = problem(m, n, k, 7, bm=min(bm, m), bn=min(bn, n), bk=min(bk, k))
+    assert torch.equal(got, launch(Q, torch.float16, flags=capi.FLAG_GENERIC | capi.FLAG_BF16_RTN))
