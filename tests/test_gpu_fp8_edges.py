@@ -2,10 +2,10 @@
 import pytest
 import torch
 
-from composable_kernel_amd import capi
+from composable_kernel_amd import capi, torch_ops
 import fp8_ref
 from fp8_ref import U32
-from test_gpu_fp8 import check, check_exact, launch, problem, reference
+from test_gpu_fp8 import check, check_exact, gen, launch, problem, reference, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,32 @@ def test_scale_blocks_longer_than_the_operands(block):
     assert bool(((got.double() - want).abs() <= bound).all())
     Q = problem(m, n, k, 7, bm=min(bm, m), bn=min(bn, n), bk=min(bk, k))
     assert torch.equal(got, launch(Q, torch.float16, flags=capi.FLAG_GENERIC | capi.FLAG_BF16_RTN))
+
+
+def same_bits(got, want):
+    return all(torch.equal(g.view(torch.uint8), w.view(torch.uint8)) for g, w in zip(got, want) if w is not None)
+
+
+@pytest.mark.parametrize("k", [300, 4096, 4097, 5000, 5120, 8192, 8200, 16384, 20000, 40000])
+@pytest.mark.parametrize("group", [128, 0])
+@pytest.mark.parametrize("residual", [False, True])
+def test_a_row_of_the_norm_is_the_same_in_every_batch(k, group, residual):
+    """A token of a prefill and the same token alone: equal bytes and scales, whatever the launch's workgroups look like."""
+    x, r = rows(600, k, k, torch.bfloat16), rows(600, k, k + 1, torch.bfloat16) if residual else None
+    w = (1 + 0.3 * torch.randn(k, device="cuda", generator=gen(3))).to(torch.bfloat16)
+    whole = torch_ops.rmsnorm_fp8(x, w, r, 1e-6, group)
+    for a, b in ((0, 1), (599, 600), (37, 300), (0, 511), (1, 513), (88, 600)):
+        part = torch_ops.rmsnorm_fp8(x[a:b], w, r[a:b] if residual else None, 1e-6, group)
+        assert same_bits(part, [t[a:b] if t is not None else None for t in whole]), (a, b)
+
+
+def test_the_rows_behind_the_last_full_launch_are_no_others():
+    """2^21 rows go in one launch: the few behind them take the same sums."""
+    k, many = 5000, 2 ** 21 + 5
+    part = rows(1021, k, 8, torch.bfloat16)
+    x = part.repeat(many // 1021 + 1, 1)[:many]
+    w = torch.randn(k, device="cuda", generator=gen(2)).bfloat16()
+    whole = torch_ops.rmsnorm_fp8(x, w)[:2]
+    for a in (0, 2 ** 21 - 700, many - 700):
+        alone = torch_ops.rmsnorm_fp8(x[a:a + 700].clone(), w)[:2]
+        assert same_bits([t[a:a + 700] for t in whole], alone), a
