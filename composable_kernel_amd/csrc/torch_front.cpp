@@ -2,14 +2,17 @@
 //
 // A small call is bound by the host: of the 11 us that rmsnorm_fp8 of one row took from Python, its kernel runs 3; three output
 // tensors cost 4 there and 2 here, reading and checking the operands 4 and under 1.  This module takes the plain calls: plain
-// torch.Tensor operands of the right types and shapes on the current device, contiguous or (the row operands) strided by rows.  It
-// answers None to everything else -- what has to be copied, converted or refused goes the long way in torch_ops.py, which says why.
-// Outputs come from torch's caching allocator, the launch goes to the stream whose handle the caller passes.
+// torch.Tensor operands of the right types and shapes on the current device, contiguous or (the row operands) strided by rows, while
+// nothing records, transforms or fakes the calls of this thread.  It answers None to everything else -- what has to be copied,
+// converted or refused goes the long way in torch_ops.py, which says why, and what is recorded or transformed goes to the
+// registered operators.  Outputs come from torch's caching allocator, the launch goes to the current stream of the operands' device.
 #define PY_SSIZE_T_CLEAN
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 
 #include "wqgemm.h"
@@ -28,6 +31,18 @@ bool current_device_is(c10::Device d)
     return d.is_cuda() && c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getDevice().index() == d.index();
 }
 
+// A dispatch mode (fake tensors, a tracer's proxies), a functorch transform or torch.jit.trace stands between this thread's calls and
+// the kernels: it has to see the registered operator, not the allocations of its outputs.
+bool intercepted()
+{
+    using K = c10::DispatchKey;
+    constexpr c10::DispatchKeySet k({K::Python, K::PythonTLSSnapshot, K::PythonDispatcher, K::PreDispatch, K::Tracer, K::Functionalize,
+                                     K::FuncTorchDynamicLayerFrontMode, K::FuncTorchDynamicLayerBackMode, K::FuncTorchVmapMode,
+                                     K::FuncTorchBatched, K::FuncTorchGradWrapper});
+    const auto tls = c10::impl::tls_local_dispatch_key_set();
+    return c10::impl::TorchDispatchModeTLS::any_modes_set() || (tls.included_ - tls.excluded_).has_any(k);
+}
+
 // rows of `cols` contiguous elements: (rows, distance between them), or false where the layout cannot be read as such
 bool as_rows(const at::Tensor& t, int64_t cols, int64_t& rows, int64_t& ld)
 {
@@ -40,14 +55,14 @@ bool as_rows(const at::Tensor& t, int64_t cols, int64_t& rows, int64_t& ld)
     return rows > 0 && rows <= INT32_MAX && ld <= INT32_MAX;
 }
 
-// a plain torch.Tensor (no subclass) on device d (any GPU if d is null) that needs no gradient
+// a plain torch.Tensor (no subclass) on device d (any GPU if d is null) that needs no gradient and carries no tangent
 const at::Tensor* plain(PyObject* o, const c10::Device* d)
 {
     if(!THPVariable_CheckExact(o))
         return nullptr;
     const at::Tensor& t = THPVariable_Unpack(o);
     if(!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || (d && t.device() != *d) || t.is_conj() || t.is_neg() ||
-       (t.requires_grad() && c10::GradMode::is_enabled()))
+       (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined())
         return nullptr;
     return &t;
 }
@@ -58,6 +73,21 @@ struct WithoutGil
     PyThreadState* state = PyEval_SaveThread();
     ~WithoutGil() { PyEval_RestoreThread(state); }
 };
+
+// the raw handle of the device's current stream, from the function that the caller passes; false with an exception set, or if it is none
+bool current_stream(PyObject* f, c10::Device d, void*& stream)
+{
+    if(!PyCallable_Check(f))
+        return false;
+    PyObject* index = PyLong_FromLong(d.index());
+    PyObject* raw   = index ? PyObject_CallOneArg(f, index) : nullptr;
+    Py_XDECREF(index);
+    if(!raw)
+        return false;
+    stream = PyLong_AsVoidPtr(raw);
+    Py_DECREF(raw);
+    return !PyErr_Occurred();
+}
 
 int dtype_of(at::ScalarType s) { return s == at::kHalf ? (int)WQ_F16 : s == at::kBFloat16 ? (int)WQ_BF16 : -1; }
 
@@ -71,7 +101,7 @@ PyObject* raise(int status)
     return nullptr;
 }
 
-// quantized(op, x, x2 | None, weight | None, activation, eps, group_k, stream) -> (q, scale, residual_out | None), or None
+// quantized(op, x, x2 | None, weight | None, activation, eps, group_k, stream of a device) -> (q, scale, residual_out | None), or None
 PyObject* quantized(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
     if(n != 8 || !quantize)
@@ -83,14 +113,14 @@ PyObject* quantized(PyObject*, PyObject* const* a, Py_ssize_t n)
         d.activation = (int32_t)PyLong_AsLong(a[4]);
         const double eps = PyFloat_AsDouble(a[5]);
         const long group = PyLong_AsLong(a[6]);
-        void* stream     = PyLong_AsVoidPtr(a[7]);
+        void* stream     = nullptr;
         if(PyErr_Occurred())
         {
             PyErr_Clear();
             Py_RETURN_NONE;
         }
         const at::Tensor* x = plain(a[1], nullptr);
-        if(!x || x->dim() < 1 || (group != 128 && group != 0) || !(eps >= 0) || !current_device_is(x->device()))
+        if(intercepted() || !x || x->dim() < 1 || (group != 128 && group != 0) || !(eps >= 0) || !current_device_is(x->device()))
             Py_RETURN_NONE;
         const c10::Device dev = x->device();
         const int64_t K       = x->size(-1);
@@ -113,6 +143,8 @@ PyObject* quantized(PyObject*, PyObject* const* a, Py_ssize_t n)
                 Py_RETURN_NONE;
             d.weight = w->data_ptr(), d.weight_dtype = w->scalar_type() == at::kFloat ? (int)WQ_F32 : d.dtype;
         }
+        if(!current_stream(a[7], dev, stream))
+            return PyErr_Occurred() ? nullptr : (Py_INCREF(Py_None), Py_None);
         const int64_t groups = group ? (K + 127) / 128 : 1;
         c10::SmallVector<int64_t, 6> shape(x->sizes().begin(), x->sizes().end());
         at::Tensor q, scale, out;
@@ -143,7 +175,7 @@ PyObject* quantized(PyObject*, PyObject* const* a, Py_ssize_t n)
     }
 }
 
-// linear(x, x_scale, weight, weight_scale, bias | None, epilogue, out_dtype, stream) -> y, or None
+// linear(x, x_scale, weight, weight_scale, bias | None, epilogue, out_dtype, stream of a device) -> y, or None
 PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
     if(n != 8 || !launch)
@@ -151,13 +183,13 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n)
     try
     {
         const at::Tensor* x = plain(a[0], nullptr);
-        if(!x || x->dim() < 1 || x->scalar_type() != at::kFloat8_e4m3fn || !current_device_is(x->device()) || !THPDtype_Check(a[6]))
+        if(intercepted() || !x || x->dim() < 1 || x->scalar_type() != at::kFloat8_e4m3fn || !current_device_is(x->device()) || !THPDtype_Check(a[6]))
             Py_RETURN_NONE;
         const c10::Device dev         = x->device();
         const at::Tensor *xs = plain(a[1], &dev), *w = plain(a[2], &dev), *ws = plain(a[3], &dev);
         const at::ScalarType out_type = reinterpret_cast<THPDtype*>(a[6])->scalar_type;
         const long epilogue           = PyLong_AsLong(a[5]);
-        void* stream                  = PyLong_AsVoidPtr(a[7]);
+        void* stream                  = nullptr;
         if(PyErr_Occurred())
         {
             PyErr_Clear();
@@ -192,6 +224,8 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n)
                 Py_RETURN_NONE;
             p.d0 = bias->data_ptr();
         }
+        if(!current_stream(a[7], dev, stream))
+            return PyErr_Occurred() ? nullptr : (Py_INCREF(Py_None), Py_None);
         c10::SmallVector<int64_t, 6> shape(x->sizes().begin(), x->sizes().end());
         shape.back()   = N;
         p.a_dtype = p.b_dtype = p.scale_dtype = WQ_F8_E4M3FN;
@@ -220,6 +254,15 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n)
     }
 }
 
+// direct(tensor | None, ...) -> whether a call with these tensors goes to the device as it stands: nothing intercepts it, none is a subclass
+PyObject* direct(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    bool yes = !intercepted();
+    for(Py_ssize_t i = 0; i < n; ++i)
+        yes = yes && (a[i] == Py_None || THPVariable_CheckExact(a[i]));
+    return PyBool_FromLong(yes);
+}
+
 // bind(quantize, launch, workspace_bytes, last_error, error type): addresses of the library's functions
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
@@ -240,6 +283,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n)
 
 PyMethodDef methods[] = {{"quantized", (PyCFunction)(void (*)(void))quantized, METH_FASTCALL, nullptr},
                          {"linear", (PyCFunction)(void (*)(void))linear, METH_FASTCALL, nullptr},
+                         {"direct", (PyCFunction)(void (*)(void))direct, METH_FASTCALL, nullptr},
                          {"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_front", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

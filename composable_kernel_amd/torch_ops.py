@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import capi
 from .weights import BlockF8Weights, PackedWeights
@@ -112,8 +113,9 @@ class WqLinear(torch.nn.Module):
 # The operators of an 8-bit layer: rmsnorm_fp8, gated_fp8 and quantize_fp8 make e4m3fn activations with fp32 scales (one per
 # 128 consecutive values, or one per row), fp8_linear multiplies them with e4m3fn weights that carry one scale per 128 x 128
 # block.  All are inference-only, run on the current stream of the operands' device, allocate through torch's caching
-# allocator only, and can be captured into a graph.  Called plainly they go straight to the C ABI; while torch.compile
-# traces, and as torch.ops.wqgemm.*, they are the custom operators registered below.
+# allocator only, and can be captured into a graph.  Called plainly they go straight to the C ABI; where something records,
+# fakes or transforms the call (torch.compile, torch.jit.trace, make_fx, fake tensors, functorch, tensor subclasses), and as
+# torch.ops.wqgemm.*, they are the custom operators registered below.
 
 _F8 = torch.float8_e4m3fn
 _ACTIVATIONS = {"silu": capi.ACT_SILU, "fastgelu": capi.ACT_FASTGELU}
@@ -134,8 +136,16 @@ _torch_front.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (capi.lib.wqg
                                                                    capi.lib.wqgemm_workspace_bytes, capi.lib.wqgemm_last_error)), capi.WqError)
 
 
-def _needs_gradients(name):
-    raise RuntimeError(f"{name} is inference-only: call it under torch.no_grad() or with tensors that need no gradient")
+def _no_gradients(name, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} is inference-only: call it under torch.no_grad() or with tensors that need no gradient")
+    if not torch.compiler.is_compiling() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} is inference-only: its operands must carry no forward-mode tangent")
+
+
+def _direct(*tensors):
+    """Whether a call goes to the device as it stands, rather than to the registered operator."""
+    return not torch.compiler.is_compiling() and tensors[0].is_cuda and _torch_front.direct(*tensors)
 
 
 def _same_device(name, x, **others):
@@ -339,15 +349,12 @@ def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
     fp32, one rounding to nearest even into out_dtype (float16 or bfloat16).  Any N and K; fastest where K is a multiple of 16
     and the rows are 16-byte aligned."""
     if not torch.compiler.is_compiling() and x.is_cuda and epilogue in _EPILOGUES:
-        y = _torch_front.linear(x, x_scale, weight, weight_scale, bias, _EPILOGUES[epilogue], out_dtype, _raw_stream(x.get_device()))
+        y = _torch_front.linear(x, x_scale, weight, weight_scale, bias, _EPILOGUES[epilogue], out_dtype, _raw_stream)
         if y is not None:
             return y
-    if torch.is_grad_enabled() and (x.requires_grad or x_scale.requires_grad or weight.requires_grad or weight_scale.requires_grad or
-                                    (bias is not None and bias.requires_grad)):
-        _needs_gradients("fp8_linear")
-    if torch.compiler.is_compiling():
-        return _fp8_linear_op(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype)
-    return _fp8_linear(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype)
+    _no_gradients("fp8_linear", x, x_scale, weight, weight_scale, bias)
+    call = _fp8_linear if _direct(x, x_scale, weight, weight_scale, bias) else _fp8_linear_op
+    return call(x, x_scale, weight, weight_scale, bias, epilogue, out_dtype)
 
 
 def quantize_fp8(x: torch.Tensor, group_k: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
@@ -355,12 +362,11 @@ def quantize_fp8(x: torch.Tensor, group_k: int = 128) -> tuple[torch.Tensor, tor
     (..., ceil(K / 128)), one per 128 consecutive values, or (..., 1) for group_k = 0.  scale = max|x| / 448 of its group
     (groups below 1e-12: as if the maximum were that); a NaN makes its whole group NaN."""
     if not torch.compiler.is_compiling() and x.is_cuda:
-        r = _torch_front.quantized(capi.QUANT_ROWS, x, None, None, 0, 0.0, group_k, _raw_stream(x.get_device()))
+        r = _torch_front.quantized(capi.QUANT_ROWS, x, None, None, 0, 0.0, group_k, _raw_stream)
         if r is not None:
             return r[:2]
-    if torch.is_grad_enabled() and x.requires_grad:
-        _needs_gradients("quantize_fp8")
-    return _quantize_fp8_op(x, group_k) if torch.compiler.is_compiling() else _quantize_fp8(x, group_k)
+    _no_gradients("quantize_fp8", x)
+    return (_quantize_fp8 if _direct(x) else _quantize_fp8_op)(x, group_k)
 
 
 def gated_fp8(gate: torch.Tensor, up: torch.Tensor, activation: str = "silu",
@@ -368,12 +374,11 @@ def gated_fp8(gate: torch.Tensor, up: torch.Tensor, activation: str = "silu",
     """quantize_fp8 of activation(gate) * up, evaluated in fp32 (activation "silu" or "fastgelu").  gate and up may be the
     two halves of one projection's output (row-strided views are read in place)."""
     if not torch.compiler.is_compiling() and gate.is_cuda and activation in _ACTIVATIONS:
-        r = _torch_front.quantized(capi.QUANT_GATED, gate, up, None, _ACTIVATIONS[activation], 0.0, group_k, _raw_stream(gate.get_device()))
+        r = _torch_front.quantized(capi.QUANT_GATED, gate, up, None, _ACTIVATIONS[activation], 0.0, group_k, _raw_stream)
         if r is not None:
             return r[:2]
-    if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
-        _needs_gradients("gated_fp8")
-    return (_gated_fp8_op if torch.compiler.is_compiling() else _gated_fp8)(gate, up, activation, group_k)
+    _no_gradients("gated_fp8", gate, up)
+    return (_gated_fp8 if _direct(gate, up) else _gated_fp8_op)(gate, up, activation, group_k)
 
 
 def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
@@ -381,15 +386,14 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | 
     """h = x + residual; returns (q, scale) = quantize_fp8 of h / sqrt(mean(h^2) + eps) * weight, and h rounded to x's dtype
     (None without a residual).  The norm sees h unrounded; weight (K,) has x's dtype or float32."""
     if not torch.compiler.is_compiling() and x.is_cuda:
-        r = _torch_front.quantized(capi.QUANT_RMSNORM, x, residual, weight, 0, eps, group_k, _raw_stream(x.get_device()))
+        r = _torch_front.quantized(capi.QUANT_RMSNORM, x, residual, weight, 0, eps, group_k, _raw_stream)
         if r is not None:
             return r
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
-        _needs_gradients("rmsnorm_fp8")
-    if torch.compiler.is_compiling():
-        q, scale, out = _rmsnorm_fp8_op(x, weight, residual, eps, group_k)
-        return q, scale, out if residual is not None else None
-    return _rmsnorm_fp8(x, weight, residual, eps, group_k)
+    _no_gradients("rmsnorm_fp8", x, weight, residual)
+    if _direct(x, weight, residual):
+        return _rmsnorm_fp8(x, weight, residual, eps, group_k)
+    q, scale, out = _rmsnorm_fp8_op(x, weight, residual, eps, group_k)
+    return q, scale, out if residual is not None else None
 
 
 class Fp8Linear(torch.nn.Module):

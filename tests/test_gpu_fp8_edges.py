@@ -63,3 +63,53 @@ def test_the_rows_behind_the_last_full_launch_are_no_others():
     for a in (0, 2 ** 21 - 700, many - 700):
         alone = torch_ops.rmsnorm_fp8(x[a:a + 700].clone(), w)[:2]
         assert same_bits([t[a:a + 700] for t in whole], alone), a
+
+
+# ---- calls that something records or transforms ----
+
+def layer(x, norm, wt, ws):
+    q, s, h = torch_ops.rmsnorm_fp8(x, norm, x)
+    q2, s2 = torch_ops.quantize_fp8(h)
+    q3, s3 = torch_ops.gated_fp8(x, h, "fastgelu")
+    return torch_ops.fp8_linear(q, s, wt, ws) + torch_ops.fp8_linear(q2, s2, wt, ws), q3, s3
+
+
+def operands(seed, m=6, k=512, n=72):
+    g = gen(seed)
+    return (torch.randn(m, k, device="cuda", generator=g).bfloat16(), 1 + 0.1 * torch.randn(k, device="cuda", generator=g),
+            torch.randn(n, k, device="cuda", generator=g).to(torch.float8_e4m3fn), torch.rand(1, k // 128, device="cuda", generator=g))
+
+
+@pytest.mark.parametrize("way", ["compile", "make_fx", "jit"])
+def test_a_recorded_program_computes(way):
+    """What a tracer has recorded holds the operators, and gives with other inputs what the plain calls give with them."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    first = operands(1)
+    if way == "compile":
+        torch._dynamo.reset()
+        program = torch.compile(layer, backend="eager", fullgraph=True)
+    else:
+        program = make_fx(layer)(*first) if way == "make_fx" else torch.jit.trace(layer, first, check_trace=False)
+        text = str(program.graph)
+        assert all(f"wqgemm{sep}{op}" in text for op in ("rmsnorm_fp8", "quantize_fp8", "gated_fp8", "fp8_linear") for sep in (["."] if way == "make_fx" else ["::"]))
+    for seed in (1, 2, 3):
+        args = operands(seed)
+        assert same_bits(program(*args), layer(*args))
+
+
+def test_tangents_and_fake_tensors_of_a_gpu():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.autograd import forward_ad
+
+    x, w = operands(1)[:2]
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: torch_ops.quantize_fp8(d), lambda: torch_ops.gated_fp8(x, d), lambda: torch_ops.rmsnorm_fp8(d, w)):
+            with pytest.raises(RuntimeError, match="inference-only"):
+                call()
+        assert same_bits(torch_ops.quantize_fp8(x), torch_ops.quantize_fp8(x.clone()))
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        q, s = torch_ops.quantize_fp8(x)
+        assert type(q).__name__ == type(s).__name__ == "FakeTensor" and s.shape == (6, 4)
+    assert type(torch_ops.quantize_fp8(x)[0]) is torch.Tensor
