@@ -8,6 +8,7 @@
 // registered operators.  Outputs come from torch's caching allocator, the launch goes to the current stream of the operands' device.
 #define PY_SSIZE_T_CLEAN
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
@@ -106,7 +107,7 @@ PyObject* quantized(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
     if(n != 8 || !quantize)
         return PyErr_Format(PyExc_TypeError, "quantized takes 8 arguments, after bind()");
-    try
+    HANDLE_TH_ERRORS // (what torch throws here, out of memory first of all, arrives as the exception that its own functions raise)
     {
         wqgemm_quant d{};
         d.op         = (int32_t)PyLong_AsLong(a[0]);
@@ -169,10 +170,7 @@ PyObject* quantized(PyObject*, PyObject* const* a, Py_ssize_t n)
         PyTuple_SET_ITEM(r, 2, out.defined() ? THPVariable_Wrap(std::move(out)) : (Py_INCREF(Py_None), Py_None));
         return r;
     }
-    catch(const std::exception& e)
-    {
-        return PyErr_Format(PyExc_RuntimeError, "%s", e.what());
-    }
+    END_HANDLE_TH_ERRORS
 }
 
 // linear(x, x_scale, weight, weight_scale, bias | None, epilogue, out_dtype, stream of a device) -> y, or None
@@ -180,7 +178,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
     if(n != 8 || !launch)
         return PyErr_Format(PyExc_TypeError, "linear takes 8 arguments, after bind()");
-    try
+    HANDLE_TH_ERRORS
     {
         const at::Tensor* x = plain(a[0], nullptr);
         if(intercepted() || !x || x->dim() < 1 || x->scalar_type() != at::kFloat8_e4m3fn || !current_device_is(x->device()) || !THPDtype_Check(a[6]))
@@ -248,10 +246,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n)
             return raise(rc);
         return THPVariable_Wrap(std::move(y));
     }
-    catch(const std::exception& e)
-    {
-        return PyErr_Format(PyExc_RuntimeError, "%s", e.what());
-    }
+    END_HANDLE_TH_ERRORS
 }
 
 // direct(tensor | None, ...) -> whether a call with these tensors goes to the device as it stands: nothing intercepts it, none is a subclass

@@ -65,6 +65,17 @@ def test_the_rows_behind_the_last_full_launch_are_no_others():
         assert same_bits([t[a:a + 700] for t in whole], alone), a
 
 
+def test_out_of_memory_is_torchs_own_error():
+    """Outputs that do not fit the card, in both ways into the library."""
+    m, n, k = 2 ** 24, 2 ** 14, 16
+    q, s = torch.zeros(m, k, device="cuda").to(torch.float8_e4m3fn), torch.ones(m, 1, device="cuda")
+    w, ws = torch.zeros(n, k, device="cuda").to(torch.float8_e4m3fn), torch.ones(n // 128, 1, device="cuda")
+    for call in (torch_ops.fp8_linear, lambda *a: torch_ops._fp8_linear(*a, None, "none", torch.bfloat16)):
+        with pytest.raises(torch.OutOfMemoryError):
+            call(q, s, w, ws)
+    assert torch_ops.fp8_linear(q[:5], s[:5], w, ws).shape == (5, n)
+
+
 # ---- calls that something records or transforms ----
 
 def layer(x, norm, wt, ws):
