@@ -7,6 +7,8 @@ PyTorch supplies device memory and the stream; the arithmetic is the HIP kernels
 from __future__ import annotations
 
 import ctypes
+import os
+import warnings
 
 import torch
 from torch.autograd import forward_ad
@@ -127,13 +129,23 @@ _INT_MAX = 2 ** 31 - 1
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+class _NoFront:
+    """In place of the short way where it was not built: every call goes through the registered operators."""
+    linear = quantized = staticmethod(lambda *args: None)
+    direct = staticmethod(lambda *tensors: False)
+
+
 # (a call with nothing to copy, convert or refuse goes the short way, in C++: csrc/torch_front.cpp.  It answers None to the others)
 try:
     from . import _torch_front
 except ImportError as e:
-    raise ImportError(f"composable_kernel_amd/_torch_front.so cannot be loaded ({e}): build it with `make -C composable_kernel_amd/csrc`") from e
-_torch_front.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (capi.lib.wqgemm_quantize, capi.lib.wqgemm_launch,
-                                                                   capi.lib.wqgemm_workspace_bytes, capi.lib.wqgemm_last_error)), capi.WqError)
+    if os.path.exists(os.path.join(os.path.dirname(__file__), "_torch_front.so")):
+        warnings.warn(f"composable_kernel_amd/_torch_front.so cannot be loaded ({e}); calls of the fp8 operators take longer on the host "
+                      "without it: build it again with `make -C composable_kernel_amd/csrc`", RuntimeWarning)
+    _torch_front = _NoFront
+else:
+    _torch_front.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (capi.lib.wqgemm_quantize, capi.lib.wqgemm_launch,
+                                                                       capi.lib.wqgemm_workspace_bytes, capi.lib.wqgemm_last_error)), capi.WqError)
 
 
 def _no_gradients(name, *tensors):

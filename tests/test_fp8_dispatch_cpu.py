@@ -1,4 +1,8 @@
 """Calls of the fp8 operators that something records, fakes or transforms reach the registered operators.  No GPU call is made here."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -103,3 +107,46 @@ def test_what_is_intercepted():
     with torch.no_grad(), torch.inference_mode(), torch.autocast("cpu"):
         assert front.direct(x)
     assert front.direct(x)
+
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.parametrize("built", [False, True])
+def test_the_module_does_without_its_short_way(built):
+    """Not built, or built for another torch: the operators, and those for int4 / int8 weights, are there all the same."""
+    code = f"""
+import os, sys, warnings
+import composable_kernel_amd
+sys.modules["composable_kernel_amd._torch_front"] = None  # (an import of it fails)
+exists = os.path.exists
+os.path.exists = lambda p: {built} if str(p).endswith("_torch_front.so") else exists(p)
+with warnings.catch_warnings(record=True) as seen:
+    warnings.simplefilter("always")
+    from composable_kernel_amd import torch_ops
+assert ["_torch_front" in str(w.message) for w in seen if w.category is RuntimeWarning] == [True] * {built}, seen
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+x = torch.zeros(4, 256, dtype=torch.bfloat16)
+with FakeTensorMode():
+    f = torch.empty(4, 256, dtype=torch.bfloat16, device="cuda")
+    q, s, h = torch_ops.rmsnorm_fp8(f, f[0], f)
+    assert s.shape == (4, 2) and torch_ops.fp8_linear(q, s, q, s[:1]).shape == (4, 4)
+for call in (lambda: torch_ops.quantize_fp8(x), lambda: torch_ops.fpaintb_linear(x, x, x[0], 4, "none", None)):
+    try:
+        call()
+    except RuntimeError as e:
+        assert "GPU only" in str(e), e
+print("served")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=200)
+    assert r.returncode == 0 and "served" in r.stdout, r.stdout + r.stderr
+
+
+def test_the_build_leaves_the_short_way_out_without_torch():
+    front = os.path.join(ROOT, "composable_kernel_amd", "_torch_front.so")
+    before = os.stat(front).st_mtime_ns
+    r = subprocess.run(["make", "-C", os.path.join(ROOT, "composable_kernel_amd", "csrc"), "PYTHON=/bin/false", "-W",
+                        os.path.join(ROOT, "composable_kernel_amd", "csrc") + "/torch_front.cpp", front], capture_output=True, text=True)
+    assert r.returncode == 0 and "left out" in r.stdout, r.stdout + r.stderr
+    assert os.stat(front).st_mtime_ns == before

@@ -76,6 +76,19 @@ def test_out_of_memory_is_torchs_own_error():
     assert torch_ops.fp8_linear(q[:5], s[:5], w, ws).shape == (5, n)
 
 
+def test_without_the_short_way(monkeypatch):
+    """Where the C++ front was not built, the registered operators answer, with the same bits."""
+    args = operands(4)
+    want = layer(*args)
+    monkeypatch.setattr(torch_ops, "_torch_front", torch_ops._NoFront)
+    assert same_bits(layer(*args), want)
+    x = args[0].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="inference-only"):
+        torch_ops.quantize_fp8(x)
+    with pytest.raises(ValueError):
+        torch_ops.quantize_fp8(args[0], 64)
+
+
 # ---- calls that something records or transforms ----
 
 def layer(x, norm, wt, ws):
