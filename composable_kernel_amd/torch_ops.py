@@ -413,7 +413,9 @@ class Fp8Linear(torch.nn.Module):
     ``weights.load_fp8_blocks``).
 
     forward takes float16 / bfloat16 activations, which it quantises by 128 itself and answers in their dtype, or an already
-    quantised pair (q, scale) -- what rmsnorm_fp8, gated_fp8 and quantize_fp8 return first -- answered in ``out_dtype``."""
+    quantised pair (q, scale) -- what rmsnorm_fp8, gated_fp8 and quantize_fp8 return first -- answered in ``out_dtype``.
+
+    .half(), .bfloat16() and the like leave the weight's bytes and scales as they are."""
 
     def __init__(self, bw: BlockF8Weights, bias: torch.Tensor | None = None, epilogue: str = "none", device="cuda",
                  out_dtype: torch.dtype = torch.bfloat16):
@@ -425,6 +427,19 @@ class Fp8Linear(torch.nn.Module):
         self.register_buffer("weight_scale", torch.from_numpy(bw.scale.copy()).to(device))
         self.register_buffer("bias", None if bias is None else bias.to(device=device, dtype=torch.float32))
         self.epilogue = epilogue if bias is None else {"none": "add", "fastgelu": "add_fastgelu"}[epilogue]
+
+    def _apply(self, fn, recurse=True):
+        # (casts of a model take whatever is floating point: the weight and its scales pass through them as bytes)
+        exact = (self.weight, self.weight_scale)
+
+        def apply(t):
+            if not any(t is e for e in exact):
+                return fn(t)
+            as_bytes = t.contiguous().view(torch.uint8)
+            out = fn(as_bytes)
+            return (out if out.dtype == torch.uint8 else as_bytes.to(out.device)).view(t.dtype)
+
+        return super()._apply(apply, recurse)
 
     def forward(self, x):
         if isinstance(x, (tuple, list)):

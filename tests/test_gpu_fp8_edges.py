@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from composable_kernel_amd import capi, torch_ops
+from composable_kernel_amd import capi, torch_ops, weights
 import fp8_ref
 from fp8_ref import U32
 from test_gpu_fp8 import check, check_exact, gen, launch, problem, reference, rows
@@ -87,6 +87,20 @@ def test_without_the_short_way(monkeypatch):
         torch_ops.quantize_fp8(x)
     with pytest.raises(ValueError):
         torch_ops.quantize_fp8(args[0], 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("stored", [torch.float32])
+def test_a_cast_layer_computes_as_before(dtype, stored):
+    """A model's .half() or .bfloat16() behind the layer's making; biases of every type, rounded once to the output's."""
+    w = torch.randn(300, 400, generator=torch.Generator().manual_seed(1)).numpy()
+    bias = torch.randn(300, generator=torch.Generator().manual_seed(2)).to(stored)
+    layer = torch_ops.Fp8Linear(weights.quantize_fp8_blocks(w), bias, "fastgelu")
+    x = torch.randn(7, 400, device="cuda", generator=gen(3)).to(dtype)
+    want = torch_ops.fp8_linear(*torch_ops.quantize_fp8(x), layer.weight, layer.weight_scale, bias.cuda().to(dtype), "add_fastgelu", dtype)
+    assert torch.equal(layer(x), want)
+    cast = layer.half() if dtype == torch.float16 else layer.bfloat16()
+    assert cast.bias.dtype == dtype and torch.equal(cast(x), want)
 
 
 # ---- calls that something records or transforms ----
