@@ -415,7 +415,8 @@ class Fp8Linear(torch.nn.Module):
     forward takes float16 / bfloat16 activations, which it quantises by 128 itself and answers in their dtype, or an already
     quantised pair (q, scale) -- what rmsnorm_fp8, gated_fp8 and quantize_fp8 return first -- answered in ``out_dtype``.
 
-    .half(), .bfloat16() and the like leave the weight's bytes and scales as they are."""
+    .half(), .bfloat16() and the like leave the weight's bytes and scales as they are.  The bias keeps the type it comes in
+    (float16, bfloat16 or float32) and is rounded to the output's: one of that type already costs no launch of its own."""
 
     def __init__(self, bw: BlockF8Weights, bias: torch.Tensor | None = None, epilogue: str = "none", device="cuda",
                  out_dtype: torch.dtype = torch.bfloat16):
@@ -425,7 +426,7 @@ class Fp8Linear(torch.nn.Module):
         self.in_features, self.out_features, self.out_dtype = bw.K, bw.N, out_dtype
         self.register_buffer("weight", torch.from_numpy(bw.weight.copy()).view(_F8).to(device))
         self.register_buffer("weight_scale", torch.from_numpy(bw.scale.copy()).to(device))
-        self.register_buffer("bias", None if bias is None else bias.to(device=device, dtype=torch.float32))
+        self.register_buffer("bias", None if bias is None else bias.to(device=device, dtype=bias.dtype if bias.dtype in _DT else torch.float32))
         self.epilogue = epilogue if bias is None else {"none": "add", "fastgelu": "add_fastgelu"}[epilogue]
 
     def _apply(self, fn, recurse=True):

@@ -56,3 +56,9 @@ def test_a_layer_moves_between_devices():
     assert layer.weight.device.type == layer.weight_scale.device.type == "meta" and layer.weight.dtype == torch.float8_e4m3fn
     layer = layer.to_empty(device="cpu")
     assert layer.weight.shape == (130, 200) and layer.weight_scale.shape == (2, 2) and layer.weight_scale.dtype == torch.float32
+
+
+@pytest.mark.parametrize("dtype,kept", [(torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32), (torch.float64, torch.float32)])
+def test_a_bias_keeps_its_type(dtype, kept):
+    bw = weights.quantize_fp8_blocks(np.ones((130, 200), np.float32))
+    assert torch_ops.Fp8Linear(bw, torch.zeros(130, dtype=dtype), device="cpu").bias.dtype == kept

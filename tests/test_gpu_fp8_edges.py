@@ -90,7 +90,7 @@ def test_without_the_short_way(monkeypatch):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("stored", [torch.float32])
+@pytest.mark.parametrize("stored", [torch.float16, torch.bfloat16, torch.float32])
 def test_a_cast_layer_computes_as_before(dtype, stored):
     """A model's .half() or .bfloat16() behind the layer's making; biases of every type, rounded once to the output's."""
     w = torch.randn(300, 400, generator=torch.Generator().manual_seed(1)).numpy()
