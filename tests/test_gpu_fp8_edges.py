@@ -65,6 +65,70 @@ def test_the_rows_behind_the_last_full_launch_are_no_others():
         assert same_bits([t[a:a + 700] for t in whole], alone), a
 
 
+def ties(m, k, group, dtype, seed):
+    """Rows whose quotients by their scale lie halfway between two e4m3 values, but for the largest of each group.  The scale is s = odd
+    * 2^e: the largest value, 448 s, and t s for a t of 5 significant bits have at most 8 bits, so they are bf16 and fp16 values."""
+    g = gen(seed)
+    width = group or k
+    n = -(-k // width)
+    pick = lambda lo, hi, shape: torch.randint(lo, hi + 1, shape, device="cuda", generator=g).double()  # noqa: E731
+    s = (2 * pick(0, 3, (m, n)) + 1) * torch.exp2(pick(-3, 2, (m, n)))  # 1, 3, 5, 7
+    wide = s.repeat_interleave(width, 1)[:, :k]
+    t = (2 * pick(8, 15, (m, k)) + 1) * torch.exp2(pick(-10, 3, (m, k)))  # 17 .. 31, odd, up to 248: halfway between two normal values
+    low = (2 * pick(0, 7, (m, k)) + 1) * 2.0 ** -10                       # and between two subnormal ones
+    t = torch.where(torch.rand(m, k, device="cuda", generator=g) < 0.1, low, t)
+    y = t * wide * torch.where(torch.rand(m, k, device="cuda", generator=g) < 0.5, -1.0, 1.0)
+    for i in range(n):
+        at = i * width + int(torch.randint(0, min(width, k - i * width), (1,), device="cuda", generator=g))
+        y[:, at] = 448 * s[:, i]
+    x = y.to(dtype)
+    assert torch.equal(x.double(), y)
+    return x
+
+
+@pytest.mark.parametrize("m,k", [(3, 128), (40, 1000), (600, 640), (7, 9001), (2, 40000)])
+@pytest.mark.parametrize("group", [128, 0])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_ties_of_the_8_bit_format(m, k, group, dtype):
+    """Quotients as an IEEE division gives them, rounded to nearest even: bytes and scales bit for bit (the division on the host).  A
+    product with the rounded reciprocal would fall to either side of a tie."""
+    width = group or k
+    n = -(-k // width)
+    as_bytes = lambda v: v.view(m, n * width)[:, :k].to(torch.float8_e4m3fn).view(torch.uint8)  # noqa: E731
+    for name, x in (("ties", ties(m, k, group, dtype, m + k)), ("any", rows(m, k, m * k, dtype))):
+        v = torch.nn.functional.pad(x.float().cpu(), (0, n * width - k)).view(m, n, width)
+        want_s = v.abs().amax(2).clamp(min=torch.tensor(1e-12)) / torch.tensor(448.0)
+        want = as_bytes(v / want_s[:, :, None])
+        if name == "ties" and bool((torch.frexp(want_s)[0] == 7 / 8).any()):  # (of the reciprocals of 1, 3, 5 and 7 only that of 7 misses ties, a quarter of them)
+            assert not torch.equal(as_bytes(v * (1 / want_s)[:, :, None]), want)
+        q, s = torch_ops.quantize_fp8(x, group)
+        assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu().view(torch.uint8), want)
+
+
+@pytest.mark.parametrize("flags", [capi.FLAG_TILE_128, capi.FLAG_TILE_256, capi.FLAG_TILE_128 | capi.FLAG_TILE_256])
+@pytest.mark.parametrize("m,n,k", [(513, 512, 1024), (300, 520, 400)])
+def test_a_row_of_the_product_is_the_same_anywhere(flags, m, n, k):
+    """Rows in another order, and some of them alone, on the same kernel: the same bits."""
+    P = problem(m, n, k, m + 1)
+    whole = launch(P, torch.float16, flags=flags)
+    order = torch.randperm(m, device="cuda", generator=gen(4))
+    for at in (order, order[:200], order[:77]):
+        bits, sa = P["a_bits"][at].contiguous(), P["sa"][at].contiguous()
+        part = dict(P, m=len(at), a_bits=bits, a_ptr=bits.data_ptr(), sa=sa)
+        assert torch.equal(launch(part, torch.float16, flags=flags), whole[at])
+
+
+@pytest.mark.parametrize("m,few,n,k", [(4, 3, 4096, 2064), (16, 9, 4096, 640), (16, 7, 5000, 1040), (16, 5, 8200, 400), (32, 20, 4096, 784), (32, 17, 5000, 656)])
+def test_a_row_of_few_is_the_same_anywhere(m, few, n, k):
+    P = problem(m, n, k, m + 1)
+    whole = launch(P, torch.float16)
+    order = torch.randperm(m, device="cuda", generator=gen(4))
+    for at in (order, order[:few]):
+        bits, sa = P["a_bits"][at].contiguous(), P["sa"][at].contiguous()
+        part = dict(P, m=len(at), a_bits=bits, a_ptr=bits.data_ptr(), sa=sa)
+        assert torch.equal(launch(part, torch.float16), whole[at])
+
+
 def test_out_of_memory_is_torchs_own_error():
     """Outputs that do not fit the card, in both ways into the library."""
     m, n, k = 2 ** 24, 2 ** 14, 16
