@@ -696,14 +696,14 @@ __global__ __launch_bounds__(256, 2) void wq_gemm_f8f8_64(const F8F8Params p) { 
 // ---------------------------------------------------------------------------------------------
 constexpr unsigned kF8F8Turn = 11; // (3, 5, 13 and 21 within 3 % of it)
 
-template <int MT, int NB, int WAVES, int P>
+template <int WAVES, int P>
 __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny_direct(const F8F8Params p)
 {
-    __shared__ __attribute__((aligned(16))) f4_t sums[WAVES][MT * NB][64];
+    __shared__ __attribute__((aligned(16))) f4_t sums[WAVES][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int fr = lane & 15, fq = lane >> 4;
-    const int n0 = blockIdx.x * (NB * 16), z = blockIdx.y;
+    const int n0 = blockIdx.x * 16, z = blockIdx.y;
     const int k0 = p.k_begin + z * p.k_per_z, k1 = min(p.k_end, k0 + p.k_per_z);
     const int ntiles = (k1 - k0 + 127) >> 7; // (empty slices: <= 0)
     const F8F8Walk walk(ntiles, gridDim.x <= 256 ? blockIdx.x * kF8F8Turn : 0);
@@ -717,66 +717,38 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny_direct(const F
     const uint32_t a_lane = (uint32_t)fr * (uint32_t)p.lda + fq * 32, b_lane = (uint32_t)fr * (uint32_t)p.ldb + fq * 32;
     const int k_last      = k1 - k0 - (ntiles - 1) * 128;
     const uint32_t bad_lo = fq * 32 < k_last ? 0u : OUT, bad_hi = fq * 32 + 16 < k_last ? 0u : OUT;
-    const int kt0 = k0 >> 7;
-    const float* sa[MT]; // (rows past M repeat the last one: their results are not stored)
-    const float* sb[NB];
-#pragma unroll
-    for(int mt = 0; mt < MT; ++mt)
-        sa[mt] = p.sa + (size_t)(min(mt * 16 + fr, p.M - 1) / p.bm) * (size_t)p.ld_sa + kt0;
-#pragma unroll
-    for(int nb = 0; nb < NB; ++nb)
-        sb[nb] = p.sb + (size_t)(min(n0 + nb * 16, p.N - 1) / p.bn) * (size_t)p.ld_sb + kt0;
+    const int kt0   = k0 >> 7;
+    const float* sa = p.sa + (size_t)(min(fr, p.M - 1) / p.bm) * (size_t)p.ld_sa + kt0; // (rows past M repeat the last one: their results are not stored)
+    const float* sb = p.sb + (size_t)(n0 / p.bn) * (size_t)p.ld_sb + kt0;
 
-    f4_t acc[MT][NB];
-#pragma unroll
-    for(int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for(int nb = 0; nb < NB; ++nb)
-            acc[mt][nb] = f4_t{0.f, 0.f, 0.f, 0.f};
-
-    auto load = [&](const __amdgpu_buffer_rsrc_t& rsrc, uint32_t off, uint32_t row_block, int tile) __attribute__((always_inline)) {
+    f4_t acc  = {0.f, 0.f, 0.f, 0.f};
+    auto load = [&](const __amdgpu_buffer_rsrc_t& rsrc, uint32_t off, int tile) __attribute__((always_inline)) {
         const bool last     = tile == ntiles - 1;
-        const uint32_t soff = row_block + k0 + tile * 128;
+        const uint32_t soff = k0 + tile * 128;
         const u4_t lo = __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, last ? off | bad_lo : off, soff, 0));
         const u4_t hi = __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, last ? off | bad_hi : off, soff + 16, 0));
         return f8f8_frag(lo, hi);
     };
     auto step = [&](int first, int tiles) __attribute__((always_inline)) {
-        i8v_t w[P][NB], a[P][MT];
-        float ra[P][MT];
+        i8v_t w[P], a[P];
+        float ra[P];
 #pragma unroll
         for(int i = 0; i < P; ++i)
             if(i < tiles)
             {
                 const int tile = walk.tile(first + i * WAVES);
-#pragma unroll
-                for(int nb = 0; nb < NB; ++nb)
-                    w[i][nb] = load(b_rsrc, b_lane, (uint32_t)(nb * 16) * (uint32_t)p.ldb, tile);
-#pragma unroll
-                for(int mt = 0; mt < MT; ++mt)
-                {
-                    a[i][mt]  = load(a_rsrc, a_lane, (uint32_t)(mt * 16) * (uint32_t)p.lda, tile);
-                    ra[i][mt] = sa[mt][tile];
-                }
+                w[i]  = load(b_rsrc, b_lane, tile);
+                a[i]  = load(a_rsrc, a_lane, tile);
+                ra[i] = sa[tile];
             }
 #pragma unroll
         for(int i = 0; i < P; ++i)
             if(i < tiles)
             {
-                const int tile = walk.tile(first + i * WAVES);
-#pragma unroll
-                for(int nb = 0; nb < NB; ++nb)
-                {
-                    const float cs = sb[nb][tile] * p.fnuz;
-#pragma unroll
-                    for(int mt = 0; mt < MT; ++mt)
-                    {
-                        const float s   = ra[i][mt] * cs;
-                        const f4_t zero = {0.f, 0.f, 0.f, 0.f};
-                        const f4_t sum  = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i][nb], a[i][mt], zero, 0, 0, 0, 0, 0, 0);
-                        acc[mt][nb]     = __builtin_elementwise_fma(sum, f4_t{s, s, s, s}, acc[mt][nb]);
-                    }
-                }
+                const float cs  = sb[walk.tile(first + i * WAVES)] * p.fnuz, s = ra[i] * cs;
+                const f4_t zero = {0.f, 0.f, 0.f, 0.f};
+                const f4_t sum  = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i], a[i], zero, 0, 0, 0, 0, 0, 0);
+                acc             = __builtin_elementwise_fma(sum, f4_t{s, s, s, s}, acc);
             }
     };
     int tile = wave;
@@ -785,20 +757,15 @@ __global__ __launch_bounds__(WAVES * 64) void wq_gemm_f8f8_skinny_direct(const F
     for(; tile < ntiles; tile += WAVES)
         step(tile, 1);
 
-#pragma unroll
-    for(int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for(int nb = 0; nb < NB; ++nb)
-            sums[wave][mt * NB + nb][lane] = acc[mt][nb];
+    sums[wave][lane] = acc;
     __syncthreads();
-    for(int u = threadIdx.x; u < MT * NB * 64; u += WAVES * 64)
+    if(wave == 0)
     {
-        const int block = u >> 6, l = u & 63;
-        f4_t v = sums[0][block][l];
+        f4_t v = sums[0][lane];
 #pragma unroll
         for(int w = 1; w < WAVES; ++w)
-            v += sums[w][block][l];
-        f8f8_store4(p, v, block / NB * 16 + (l & 15), n0 + block % NB * 16 + (l >> 4) * 4, z);
+            v += sums[w][lane];
+        f8f8_store4(p, v, fr, n0 + fq * 4, z);
     }
 }
 

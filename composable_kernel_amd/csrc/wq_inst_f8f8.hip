@@ -57,7 +57,7 @@ int launch_f8f8(int kernel, const F8F8Params& p, hipStream_t s)
         F8F8_TILE_CASE(F8F8_64, F8F8Tile64, wq_gemm_f8f8_64, 512)
         F8F8_TILE_CASE(F8F8_64X64, F8F8Tile64x64, wq_gemm_f8f8_64x64, 768)
 #undef F8F8_TILE_CASE
-    case F8F8_SKINNY_DIRECT: hipLaunchKernelGGL((wq_gemm_f8f8_skinny_direct<1, 1, 16, 2>), strips, dim3(1024), 0, s, p); return WQ_OK;
+    case F8F8_SKINNY_DIRECT: hipLaunchKernelGGL((wq_gemm_f8f8_skinny_direct<16, 2>), strips, dim3(1024), 0, s, p); return WQ_OK;
     case F8F8_SKINNY_16: return launch_tile<F8F8Skinny<1, 1, 8, 2>, wq_gemm_f8f8_skinny<1, 1, 8, 2>>(p, strips, s);
     case F8F8_SKINNY_16X64: return launch_tile<F8F8Skinny<1, 4, 4, 2>, wq_gemm_f8f8_skinny<1, 4, 4, 2>>(p, strips, s);
     case F8F8_SKINNY_16X32: return launch_tile<F8F8Skinny<1, 2, 8, 1>, wq_gemm_f8f8_skinny<1, 2, 8, 1>>(p, strips, s);

@@ -210,7 +210,9 @@ int make_plan_f8f8(const wqgemm_problem* p, Plan& plan, bool have_workspace)
     // Few rows: one pass over the weights, K dealt to the waves of a workgroup.  16 columns a workgroup as long as that is at most one
     // per CU, 32 up to 8192 columns (the activations are read once per workgroup; 5000 x 4096 at M = 16: 8.5 us, 16 columns 10.9),
     // 64 beyond (28672 x 8192: 44.5; 32 columns 47.4).  Straight to registers with up to 4 rows in the first range (4096 x 4096 at
-    // M = 1: 6.5, through LDS 6.9) and up to 2 in the last (28672 x 8192 at M = 1: 38.3 against 43.1, at M = 4: 45.6 against 43.2).
+    // M = 1: 6.5, through LDS 6.9) and up to 2 in the last (28672 x 8192 at M = 1: 38.3 against 43.1, at M = 4: 45.6 against 43.2);
+    // between them never (at M = 1, weights out of the last-level cache: 4224 x 8192 13.8, through LDS 11.2; 5120 x 4096 9.0 and 7.5; 8192 x 4096
+    // 9.2 and 8.9; 8192 x 8192 15.1 either way; more rows widen it).
     // With 17 .. 32 rows up to 8192 columns (32 rows, 4096 x 4096: 9.0, the best tile kernel 10.2; 5000 x 4096: 10.7), beyond them
     // the tile kernels (28672 x 8192: 59 against 54), and so from 33 rows (64 rows, 4096 x 11008: 27 against 16.2).
     const bool few = p->N <= 4096, many = p->N > 8192;
