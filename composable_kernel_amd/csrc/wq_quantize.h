@@ -219,10 +219,11 @@ __global__ __launch_bounds__(256) void wq_quantize_groups(const QuantParams p, i
 // One workgroup per row: the norm, and one scale per row.  R 8-element pieces per thread stay in registers between the
 // statistics and the conversion (R = 0: any width, the operands are read again).
 // ---------------------------------------------------------------------------------------------
-// sum over the wave, in all lanes: halves, rows of 16, then inside a row lanes 8, 4, 2, 1 apart (row_ror: once both halves of a row
-// are equal, a rotation by 4 is an exchange of lanes 4 apart, and so on).  Six steps through LDS instead: norm of 4096 x 8192 with two
-// sums per wave 40.5 us, this way 39.7.
-__device__ __forceinline__ float wave_sum(float v)
+// Sums over the wave: of a in the lanes of its lower half, of b in those of its upper half.  Halves, rows of 16, then inside a row
+// lanes 8, 4, 2, 1 apart (row_ror: once both halves of a row are equal, a rotation by 4 is an exchange of lanes 4 apart, and so on).
+// The exchange of the halves brings both sums into one register; six exchanges through LDS for each sum made the norm of
+// 4096 x 8192 2 % longer, two sums one beside the other that of 777 x 5000 per token (6.7 us).
+__device__ __forceinline__ float wave_sums(float a, float b)
 {
     const auto add = [](auto two) __attribute__((always_inline)) {
         return __builtin_bit_cast(float, (uint32_t)two[0]) + __builtin_bit_cast(float, (uint32_t)two[1]);
@@ -230,8 +231,8 @@ __device__ __forceinline__ float wave_sum(float v)
     const auto ror = [](float x, auto dpp) __attribute__((always_inline)) {
         return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(dpp)::value, 0xF, 0xF, true));
     };
-    v = add(__builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false));
-    v = add(__builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false));
+    float v = add(__builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false));
+    v       = add(__builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false));
     v = ror(v, std::integral_constant<int, 0x128>{});
     v = ror(v, std::integral_constant<int, 0x124>{});
     v = ror(v, std::integral_constant<int, 0x122>{});
@@ -318,15 +319,11 @@ __global__ void wq_quantize_row(const QuantParams p)
                 for(int j = 0; j < 8; ++j)
                     ss = __builtin_fmaf(y[0][j], y[0][j], ss);
             }
-        ss = wave_sum(ss);
-        if constexpr(R == 2)
-            first = wave_sum(first);
-        if(lane == 0)
-        {
+        ss = wave_sums(R == 2 ? first : ss, ss);
+        if(lane == 32)
             part[apart ? 8 + wave : wave] = ss;
-            if(apart)
-                part[wave] = first;
-        }
+        if(lane == 0 && apart)
+            part[wave] = ss;
         __syncthreads();
         ss = 0.f;
         for(int w = 0; w < (apart ? 16 : waves); ++w)
