@@ -1456,6 +1456,9 @@ int wqgemm_run_timed_rotating(const wqgemm_problem* p, void* workspace, void* st
     const size_t na = a_span_bytes(p), nb = b_span_bytes(p);
     const void* a_copies[64];
     const void* b_copies[64];
+    void *a_base[64], *b_base[64];
+    // (each copy lies as its original does to 256 bytes: alignment takes part in the choice of the kernel and of its workspace)
+    const size_t a_at = (uintptr_t)p->a % 256, b_at = (uintptr_t)p->b % 256;
     a_copies[0] = p->a, b_copies[0] = p->b;
     int made = 1, status = WQ_OK;
     hipEvent_t e0 = nullptr, e1 = nullptr;
@@ -1472,11 +1475,12 @@ int wqgemm_run_timed_rotating(const wqgemm_problem* p, void* workspace, void* st
     for(; made < rotating_count && status == WQ_OK; ++made)
     {
         void *pa = nullptr, *pb = nullptr;
-        WQ_TRY(hipMalloc(&pa, na));
-        WQ_TRY(hipMalloc(&pb, nb));
-        a_copies[made] = pa, b_copies[made] = pb;
-        WQ_TRY(hipMemcpy(pa, p->a, na, hipMemcpyDeviceToDevice));
-        WQ_TRY(hipMemcpy(pb, p->b, nb, hipMemcpyDeviceToDevice));
+        WQ_TRY(hipMalloc(&pa, na + a_at));
+        WQ_TRY(hipMalloc(&pb, nb + b_at));
+        a_base[made] = pa, b_base[made] = pb;
+        a_copies[made] = (char*)pa + a_at, b_copies[made] = (char*)pb + b_at;
+        WQ_TRY(hipMemcpy((char*)pa + a_at, p->a, na, hipMemcpyDeviceToDevice));
+        WQ_TRY(hipMemcpy((char*)pb + b_at, p->b, nb, hipMemcpyDeviceToDevice));
         if(status != WQ_OK)
         {
             (void)hipFree(pa);
@@ -1508,8 +1512,8 @@ int wqgemm_run_timed_rotating(const wqgemm_problem* p, void* workspace, void* st
         (void)hipEventDestroy(e1);
     for(int i = 1; i < made; ++i)
     {
-        (void)hipFree(const_cast<void*>(a_copies[i]));
-        (void)hipFree(const_cast<void*>(b_copies[i]));
+        (void)hipFree(a_base[i]);
+        (void)hipFree(b_base[i]);
     }
     if(status != WQ_OK)
         return status;

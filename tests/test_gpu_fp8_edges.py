@@ -129,6 +129,22 @@ def test_a_row_of_few_is_the_same_anywhere(m, few, n, k):
         assert torch.equal(launch(part, torch.float16), whole[at])
 
 
+@pytest.mark.parametrize("off", [0, 1, 8, 16])
+def test_timing_over_copies_stays_in_the_workspace(off):
+    """Copies of operands of any alignment: the kernel, and the workspace it asks for, are those of the problem itself.  (1528 x 3265 x 6640
+    takes 57 MiB with aligned rows and 30 without.)"""
+    m, n, k = 1528, 3265, 6640
+    P = problem(m, n, k, 3, offset=off, exact=True)
+    c = torch.full((m, n), -77.0, dtype=torch.bfloat16, device="cuda")
+    p = capi.f8_problem(P["a_ptr"], P["sa"].data_ptr(), P["b_ptr"], P["sb"].data_ptr(), c.data_ptr(), m, n, k, flags=capi.FLAG_BF16_RTN)
+    nbytes = capi.workspace_bytes(p)
+    ws = torch.full((nbytes + (64 << 20),), 0xFF, dtype=torch.uint8, device="cuda")
+    assert capi.run_timed_rotating(p, ws.data_ptr(), torch.cuda.current_stream().cuda_stream, 1, 5, 3) > 0
+    torch.cuda.synchronize()
+    assert bool((ws[nbytes:] == 0xFF).all())
+    check_exact(c, P)
+
+
 def test_out_of_memory_is_torchs_own_error():
     """Outputs that do not fit the card, in both ways into the library."""
     m, n, k = 2 ** 24, 2 ** 14, 16
