@@ -856,6 +856,7 @@ const char* const kF8F8Instances[] = {"256, 128, 128, 128, AnyAlignment", "256, 
                                       "512, 16, 32, 128, WavesSplitK, LdsDma", "256, 16, 64, 128, WavesSplitK, LdsDma",
                                       "512, 32, 16, 128, WavesSplitK, LdsDma", "512, 32, 32, 128, WavesSplitK, LdsDma"};
 
+// (without the scales: slabs carry them already, and wqgemm_reduce_finalize has not looked at their description)
 wq::F8F8Params f8f8_params(const wqgemm_problem* p)
 {
     wq::F8F8Params gp{};
@@ -865,7 +866,6 @@ wq::F8F8Params f8f8_params(const wqgemm_problem* p)
     gp.fnuz     = (p->a_dtype == WQ_F8_FNUZ ? 0.5f : 1.f) * (p->b_dtype == WQ_F8_FNUZ ? 0.5f : 1.f);
     gp.bf16_rtn = (p->flags & WQ_FLAG_BF16_RTN) ? 1 : 0;
     gp.epi      = epilogue_of(p);
-    set_block_scales(gp, p);
     return gp;
 }
 
@@ -1101,6 +1101,7 @@ int launch_main(const wqgemm_problem* p, const Plan& plan, void* workspace, hipS
     else if(plan.route == ROUTE_F8F8)
     {
         wq::F8F8Params gp = f8f8_params(p);
+        set_block_scales(gp, p);
         gp.k_begin = plan.k_begin, gp.k_end = plan.k_end, gp.k_per_z = plan.k_per_z;
         gp.partial = plan.partial ? 1 : 0;
         gp.slices  = plan.k_batch;

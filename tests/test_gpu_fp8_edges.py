@@ -129,6 +129,19 @@ def test_a_row_of_few_is_the_same_anywhere(m, few, n, k):
         assert torch.equal(launch(part, torch.float16), whole[at])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_reduction_needs_no_scales(dtype):
+    """The slabs carry the scales: what the problem says of the tables, or does not say, is not looked at."""
+    m, n = 37, 64
+    slabs = torch.randint(-8, 9, (3, m, n), device="cuda", generator=gen(1)).float()
+    out = torch.empty(m, n, dtype=dtype, device="cuda")
+    for tables, block in ((slabs.data_ptr(), (0, 0, 0)), (None, (0, 0, 0)), (slabs.data_ptr(), (1, 128, 128))):
+        p = capi.f8_problem(slabs.data_ptr(), tables, slabs.data_ptr(), tables, out.fill_(-77).data_ptr(), m, n, 384,
+                            c_dtype=capi.F16 if dtype == torch.float16 else capi.BF16, scale_block=block)
+        capi.reduce_finalize(p, slabs.data_ptr(), 3, torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(out, slabs.sum(0).to(dtype))
+
+
 @pytest.mark.parametrize("off", [0, 1, 8, 16])
 def test_timing_over_copies_stays_in_the_workspace(off):
     """Copies of operands of any alignment: the kernel, and the workspace it asks for, are those of the problem itself.  (1528 x 3265 x 6640
