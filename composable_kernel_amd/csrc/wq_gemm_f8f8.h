@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256) void wq_gemm_f8f8_any(const F8F8Params p)
 //
 // Bound by the matrix core with one fused multiply-add per output and K tile beside it: in registers alone 3440 TFLOP/s on random
 // bits (4080 without the folds).  256 x 256 reaches 2100 (4096 x 4096 x 4096 65 us, 4096 x 11008 x 4096 175; 145 on zeros, where the
-// clock holds): MFMAs take 64 % of a busy CU's cycles, 5.4 vector instructions go with each, LDS is busy 36 % of them.
+// clock holds): MFMAs take 63 % of a busy CU's cycles, 5.4 vector instructions go with each, LDS is busy 36 % of them.
 //
 // Both operands pass through LDS (LDS-DMA, 8 rows of 128 bytes per piece).  Weights fetched straight into the registers of the
 // MFMA were slower: a wave's load then touches 16 rows, and the vector cache takes one access per lane instead of one per 64
@@ -383,7 +383,9 @@ __device__ __forceinline__ void f8f8_tile_body(const F8F8Params& p)
     constexpr uint32_t OUT = 0x80000000u; // an offset past every resource
 
     // A piece: 8 rows of 128 bytes, a row's 16-byte chunks permuted on the source side (f8_a_swz) so that the fragment reads are
-    // free of bank conflicts.  Half h of A: row blocks h * MH .. of every wave row.
+    // free of bank conflicts (the kernel for few rows makes the same reads and counts none).  What the counters show here, 16 cycles
+    // a wave and K tile beside 132 of LDS work, is two for each of the eight reads of a row block's scales, 16 bytes apart; 192 more
+    // per wave go to the outputs' way through LDS.  Half h of A: row blocks h * MH .. of every wave row.
     const int chunk       = ((lane & 7) ^ f8_a_swz(lane >> 3)) << 4;
     const uint32_t a_lane = (uint32_t)(lane >> 3) * (uint32_t)p.lda + chunk;
     const uint32_t b_lane = (uint32_t)(lane >> 3) * (uint32_t)p.ldb + chunk;

@@ -36,7 +36,7 @@ void launch_row(QuantParams p, hipStream_t s)
         p.residual_out = p.residual_out ? (uint16_t*)p.residual_out + MOST * p.ld_res : nullptr;
     }
     // Threads: 512 with up to two pieces each in registers (norm of 4096 x 8192: 51.8 us = 4.5 TB/s; 256 threads 60, 1024 54), 1024
-    // for longer rows, and while there are few rows, where the latency of one counts (64 x 8192: 4.1 us, 512 threads 4.8).  The norm's
+    // for longer rows, and while there are few rows, where the latency of one counts (64 x 8192: 3.9 us, 512 threads 4.3).  The norm's
     // sums do not see which: only T = 512 with two pieces stands for another T, and wq_quantize_row sums those two apart.
     const long pieces = ((long)p.K + 7) / 8;
     int T             = p.M >= 512 ? 512 : 1024;

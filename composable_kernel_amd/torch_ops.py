@@ -374,8 +374,9 @@ def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
 
 def quantize_fp8(x: torch.Tensor, group_k: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
     """x (..., K) float16 / bfloat16 -> (q, scale) with x ~ q * scale: q float8_e4m3fn of x's shape, scale float32 of shape
-    (..., ceil(K / 128)), one per 128 consecutive values, or (..., 1) for group_k = 0.  scale = max|x| / 448 of its group
-    (groups below 1e-12: as if the maximum were that); a NaN makes its whole group NaN."""
+    (..., ceil(K / 128)), one per 128 consecutive values, or (..., 1) for group_k = 0 (what the C ABI's fp8 x int4
+    MultiplyMultiply problems take as d1; fp8_linear takes scales by 128).  scale = max|x| / 448 of its group (groups below
+    1e-12: as if the maximum were that); a NaN makes its whole group NaN."""
     if not torch.compiler.is_compiling() and x.is_cuda:
         r = _torch_front.quantized(capi.QUANT_ROWS, x, None, None, 0, 0.0, group_k, _raw_stream)
         if r is not None:

@@ -331,7 +331,7 @@ def one_case_f8f8(rng) -> dict:
     off = [pick(0, 0, 0, 1, 16), pick(0, 0, 0, 3, 32)]
     lda, ldb, ldc = K + pick(0, 0, 16, 128, 5), K + pick(0, 0, 16, 64, 3), N + pick(0, 0, 8, 3)
     epi = pick(capi.EPI_PASSTHROUGH, capi.EPI_PASSTHROUGH, capi.EPI_FASTGELU, capi.EPI_ADD, capi.EPI_ADD_FASTGELU)
-    k_batch = pick(2, 3, 5) if rng.integers(0, 5) == 0 and N % 4 == 0 and ldc % 4 == 0 else 1
+    k_batch = pick(2, 3, 5, 40) if rng.integers(0, 5) == 0 and N % 4 == 0 and ldc % 4 == 0 else 1  # (40: mostly more than K has blocks)
     pin = pick(0, 0, 0, capi.FLAG_TILE_128, capi.FLAG_TILE_256, capi.FLAG_TILE_128 | capi.FLAG_TILE_256)
     g = torch.Generator(device="cuda")
     g.manual_seed(int(rng.integers(0, 1 << 30)))
