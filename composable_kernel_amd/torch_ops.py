@@ -138,6 +138,8 @@ class _NoFront:
 # (a call with nothing to copy, convert or refuse goes the short way, in C++: csrc/torch_front.cpp.  It answers None to the others)
 try:
     from . import _torch_front
+    if not hasattr(_torch_front, "direct"):
+        raise ImportError("built from an earlier source")
 except ImportError as e:
     if os.path.exists(os.path.join(os.path.dirname(__file__), "_torch_front.so")):
         warnings.warn(f"composable_kernel_amd/_torch_front.so cannot be loaded ({e}); calls of the fp8 operators take longer on the host "

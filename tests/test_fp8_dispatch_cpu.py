@@ -150,3 +150,20 @@ def test_the_build_leaves_the_short_way_out_without_torch():
                         os.path.join(ROOT, "composable_kernel_amd", "csrc") + "/torch_front.cpp", front], capture_output=True, text=True)
     assert r.returncode == 0 and "left out" in r.stdout, r.stdout + r.stderr
     assert os.stat(front).st_mtime_ns == before
+
+
+def test_a_short_way_of_an_earlier_build_is_left_alone():
+    code = """
+import sys, types, warnings
+import composable_kernel_amd
+old = types.ModuleType("composable_kernel_amd._torch_front")
+old.bind = old.linear = old.quantized = lambda *a: None
+sys.modules[old.__name__] = old
+with warnings.catch_warnings(record=True) as seen:
+    warnings.simplefilter("always")
+    from composable_kernel_amd import torch_ops
+assert torch_ops._torch_front is torch_ops._NoFront and any("earlier source" in str(w.message) for w in seen)
+print("served")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=200)
+    assert r.returncode == 0 and "served" in r.stdout, r.stdout + r.stderr
