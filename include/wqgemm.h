@@ -292,7 +292,8 @@ int wqgemm_pack_int4_host(const int8_t* q, int32_t ldq, int32_t K, int32_t N, ui
  * few fp32 steps).  group_k = 128: ceil(K / 128) scales per row -- with
  * ld_scale = ld_a_scale the a_block_scale table of a problem with scale_block_m = 1, scale_block_k = 128; group_k = 0: one
  * scale per row (ld_scale = 1 makes it the d1 operand of the MultiplyMultiply epilogues).  A NaN anywhere in a group makes
- * its scale and all its bytes NaN; an infinity makes the scale infinite and its own bytes NaN.
+ * its scale and all its bytes NaN; an infinity makes the scale infinite and its own bytes NaN.  The norm's squares are summed in
+ * fp32: a row whose sum passes its range (values about 1e19) comes out as zeros, a row of zeros with eps = 0 as NaN.
  * All strides count elements of their tensor and no alignment beyond an element's own is required (16-byte aligned rows
  * are fastest).  residual_out may be x or x2 themselves (same pointer and stride); no other outputs may overlap an input.
  * Rows are independent: a row's result does not depend on M.  K up to 2^30. */
